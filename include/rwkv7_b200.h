@@ -42,6 +42,7 @@ extern "C" {
 /* element types accepted by rwkv7_b200_model_set_tensor */
 #define RWKV7_B200_DT_F16 0
 #define RWKV7_B200_DT_BF16 1
+#define RWKV7_B200_DT_F32 2      /* logits of rwkv7_b200_token_logprobs only */
 
 /* input activations / epilogues of rwkv7_b200_linear_* */
 #define RWKV7_B200_ACT_NONE 0
@@ -182,6 +183,28 @@ int rwkv7_b200_sample(void* stream, int B, int V, const float* logits, float* pe
  * penalty update above; next_tokens (int64 [B], may be NULL) receives the same ids. */
 int rwkv7_b200_greedy_pick(void* stream, int B, int V, const float* logits, float* penalties, float presence_penalty,
                            float repetition_penalty, float penalty_decay, int* out, int64_t* next_tokens);
+
+/* Log probabilities over logits (no counterpart in the reference, whose sampler keeps its probabilities to itself):
+ * for every row of logits ([rows] rows of V values, `ld` elements apart, fp32 or half) under softmax(row)
+ *   logprobs [rows][n_tokens]      of the given tokens [rows][n_tokens] (n_tokens == 0: none)
+ *   entropy, lse [rows]            -sum p ln p and ln sum exp(z); either may be NULL
+ *   top_ids, top_logprobs [rows][top_k]   the likeliest tokens, likeliest first, equal ones by index (top_k in 0..32)
+ * A logit of -inf is a masked token: probability 0, never an alternative (missing alternatives are id -1, log
+ * probability -inf).  A row of masked tokens has lse -inf, log probabilities -inf and entropy 0.  A row with a NaN or
+ * +inf has no distribution: NaN, ids -1 (the sampler, which has to answer, reads NaN as 0 instead).  A token id below 0
+ * asks for nothing and gets 0 (padding of a batch); one of V or more gets NaN. */
+int rwkv7_b200_token_logprobs(void* stream, int rows, int V, const void* logits, int dtype, long long ld,
+                              const int64_t* tokens, int n_tokens, int top_k, float* logprobs, float* entropy, float* lse,
+                              int* top_ids, float* top_logprobs);
+/* The same answers for x W^T without writing the logits: one given token per row (tokens and logprobs may both be NULL),
+ * x [rows][K] half, weight [V][K] in `format` (RWKV7_B200_FMT_*; W8A16: scale [V]; W4A16: scale and zero
+ * [V][ceil(K / group)], group 32, 64 or 128, zero NULL: 8).  Logits are fp32 sums, not rounded to half as forward's are;
+ * 4-bit weights count as half((q - zero) * scale).  K % 32 == 0; x, weight and workspace 16-byte aligned.  workspace is
+ * scratch of the size the first function returns; calls that may overlap on the GPU need one each. */
+int rwkv7_b200_head_logprobs_workspace(int rows, int V, size_t* bytes);
+int rwkv7_b200_head_logprobs(void* stream, int rows, int K, int V, const uint16_t* x, const void* weight, int format,
+                             const uint16_t* scale, const uint16_t* zero, int group, const int64_t* tokens, float* logprobs,
+                             float* entropy, float* lse, void* workspace, size_t workspace_bytes);
 
 /* Replaces ModelBackend::copy_state_slice (src/rwkv7_fast_v4.cu:1421-1504): copies `count`
  * sequences from a state of batch size src_B (starting at src_offset) into a state of batch size
@@ -350,6 +373,17 @@ int rwkv7_b200_linear_w8a16(void* stream, int M, int K, int N, const uint16_t* x
                             const uint16_t* scale, int epilogue, void* y);
 int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q,
                             const uint16_t* scale, const uint16_t* zero, int epilogue, void* y);
+/* 4-bit weights with group scales (no counterpart in the reference): W[n,k] = (q[n,k] - zero[n,g]) * scale[n,g] with
+ * g = k / group, group 32, 64 or 128, a short last group allowed (scale and zero are [N][ceil(K / group)]), zero NULL: 8
+ * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x and q 16-byte aligned.  Up to a few rows (see
+ * csrc/w4_group.cu) the scale multiplies the group's fp32 sum, so no weight is rounded. */
+int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q,
+                                  const uint16_t* scale, const uint16_t* zero, int group, int epilogue, void* y);
+/* zero NULL: symmetric, scale = max |W| / 7, codes around 8; otherwise as W4A16 over groups of `group`. */
+int rwkv7_b200_quant_pack_w4_group(void* stream, int N, int K, int group, const uint16_t* W, uint8_t* q, uint16_t* scale,
+                                   uint16_t* zero);
+int rwkv7_b200_quant_unpack_w4_group(void* stream, int N, int K, int group, const uint8_t* q, const uint16_t* scale,
+                                     const uint16_t* zero, uint16_t* W);
 int rwkv7_b200_quant_pack_w8(void* stream, int N, int K, const uint16_t* W, int8_t* q, uint16_t* scale);
 int rwkv7_b200_quant_unpack_w8(void* stream, int N, int K, const int8_t* q, const uint16_t* scale, uint16_t* W);
 int rwkv7_b200_quant_pack_w4(void* stream, int N, int K, const uint16_t* W, uint8_t* q, uint16_t* scale,

@@ -147,6 +147,30 @@ int rwkv7_b200_greedy_pick(void* stream, int B, int V, const float* logits, floa
                          next_tokens);
 }
 
+int rwkv7_b200_token_logprobs(void* stream, int rows, int V, const void* logits, int dtype, long long ld, const int64_t* tokens,
+                              int n_tokens, int top_k, float* logprobs, float* entropy, float* lse, int* top_ids,
+                              float* top_logprobs) {
+  RK_REQUIRE(dtype == RWKV7_B200_DT_F32 || dtype == RWKV7_B200_DT_F16, kBadArg, "token_logprobs: unknown dtype %d", dtype);
+  rk::TokenLogprobsArgs a;
+  a.rows = rows; a.V = V; a.logits = logits; a.is_half = dtype == RWKV7_B200_DT_F16; a.ld = ld;
+  a.tokens = tokens; a.n_tokens = n_tokens; a.top_k = top_k;
+  a.logprobs = logprobs; a.entropy = entropy; a.lse = lse; a.top_ids = top_ids; a.top_logprobs = top_logprobs;
+  return rk::token_logprobs(st(stream), a);
+}
+int rwkv7_b200_head_logprobs_workspace(int rows, int V, size_t* bytes) {
+  RK_REQUIRE(rows > 0 && V > 0 && bytes, kBadArg, "head_logprobs_workspace: bad argument");
+  *bytes = rk::head_logprobs_workspace(rows, V);
+  return kOk;
+}
+int rwkv7_b200_head_logprobs(void* stream, int rows, int K, int V, const uint16_t* x, const void* weight, int format,
+                             const uint16_t* scale, const uint16_t* zero, int group, const int64_t* tokens, float* logprobs,
+                             float* entropy, float* lse, void* workspace, size_t workspace_bytes) {
+  rk::HeadLogprobsArgs a;
+  a.rows = rows; a.K = K; a.V = V; a.x = h(x); a.w = weight; a.fmt = format; a.group = group; a.scale = h(scale); a.zero = h(zero);
+  a.tokens = tokens; a.logprobs = logprobs; a.entropy = entropy; a.lse = lse;
+  return rk::head_logprobs(st(stream), a, workspace, workspace_bytes);
+}
+
 int rwkv7_b200_copy_state_slice(const rwkv7_b200_model* m, const void* src_shift, const void* src_wkv, const int* src_elapsed,
                                 int src_B, int src_offset, void* dst_shift, void* dst_wkv, int* dst_elapsed, int dst_B,
                                 int dst_offset, int count, void* stream) {
@@ -334,6 +358,20 @@ int rwkv7_b200_linear_w8a16(void* stream, int M, int K, int N, const uint16_t* x
 int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q, const uint16_t* scale,
                             const uint16_t* zero, int epilogue, void* y) {
   return linear_common(stream, M, K, N, x, q, RWKV7_B200_FMT_W4A16, scale, zero, 0, epilogue, y);
+}
+int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q, const uint16_t* scale,
+                                  const uint16_t* zero, int group, int epilogue, void* y) {
+  rk::W4GroupArgs a;
+  a.M = M; a.K = K; a.N = N; a.group = group; a.x = h(x); a.q = q; a.scale = h(scale); a.zero = h(zero); a.epi = epilogue; a.y = y;
+  return rk::w4_group_linear(st(stream), a);
+}
+int rwkv7_b200_quant_pack_w4_group(void* stream, int N, int K, int group, const uint16_t* W, uint8_t* q, uint16_t* scale,
+                                   uint16_t* zero) {
+  return rk::quant_pack_w4_group(st(stream), N, K, group, h(W), q, h(scale), h(zero));
+}
+int rwkv7_b200_quant_unpack_w4_group(void* stream, int N, int K, int group, const uint8_t* q, const uint16_t* scale,
+                                     const uint16_t* zero, uint16_t* W) {
+  return rk::quant_unpack_w4_group(st(stream), N, K, group, q, h(scale), h(zero), h(W));
 }
 int rwkv7_b200_quant_pack_w8(void* stream, int N, int K, const uint16_t* W, int8_t* q, uint16_t* scale) {
   return rk::quant_pack_w8(st(stream), N, K, h(W), q, h(scale));

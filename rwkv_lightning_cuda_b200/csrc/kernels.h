@@ -103,6 +103,39 @@ int greedy_pick(cudaStream_t stream, int B, int V, const float* logits, float* p
 int sample_tokens(cudaStream_t stream, int B, int V, const float* logits, float* penalties, float* probs, float presence,
                   float repetition, float decay, float temperature, int top_k, float top_p, unsigned long long seed,
                   unsigned long long offset, int* out, int64_t* next_tokens);
+// Log probabilities of given tokens, entropy, log-sum-exp and the likeliest alternatives over logits (logprobs.cu).
+constexpr int kMaxTopLogprobs = 32;
+struct TokenLogprobsArgs {
+  int rows = 0, V = 0;
+  const void* logits = nullptr;  // fp32 or half [rows, V], rows ld elements apart
+  bool is_half = false;
+  long long ld = 0;
+  const int64_t* tokens = nullptr;  // [rows, n_tokens]; < 0: nothing asked
+  int n_tokens = 0, top_k = 0;
+  float* logprobs = nullptr;      // [rows, n_tokens]
+  float* entropy = nullptr;       // [rows], optional
+  float* lse = nullptr;           // [rows], optional
+  int* top_ids = nullptr;         // [rows, top_k]
+  float* top_logprobs = nullptr;  // [rows, top_k]
+};
+int token_logprobs(cudaStream_t stream, const TokenLogprobsArgs& args);
+// The head product reduced to the same answers where it is computed (head_logprobs.cu).
+struct HeadLogprobsArgs {
+  int rows = 0, K = 0, V = 0;
+  const half* x = nullptr;  // [rows, K]
+  const void* w = nullptr;  // [V, K] in format fmt (as LinearArgs)
+  int fmt = 0, group = 128;
+  const half* scale = nullptr;  // W8: [V]; W4: [V, ceil(K / group)]
+  const half* zero = nullptr;   // W4: as scale, or nullptr: 8
+  const int64_t* tokens = nullptr;  // [rows]; < 0: nothing asked
+  float* logprobs = nullptr;        // [rows]
+  float* entropy = nullptr;         // [rows], optional
+  float* lse = nullptr;             // [rows], optional
+  float4* part = nullptr;           // set by head_logprobs: (m, s, t) of a tile's part of a row, [tiles, rows]
+  float* given = nullptr;           // set by head_logprobs: the given token's logit, [rows]
+};
+size_t head_logprobs_workspace(int rows, int V);
+int head_logprobs(cudaStream_t stream, HeadLogprobsArgs args, void* workspace, size_t workspace_bytes);
 // src [G][B][Vl] (one block per rank, as an all-gather leaves it) -> dst [B][G*Vl]
 int interleave_gathered(cudaStream_t stream, const float* src, float* dst, int G, int B, int Vl);
 int relu_square(cudaStream_t stream, const half* x, half* out, long long n);
@@ -181,6 +214,20 @@ struct TmixDecodeArgs {
 };
 bool tmix_decode_supported(const TmixDecodeArgs& args);
 int tmix_decode(cudaStream_t stream, const TmixDecodeArgs& args);
+
+// ---- w4_group.cu : 4-bit weights with group scales, scales applied to the fp32 sums of the groups
+struct W4GroupArgs {
+  int M = 0, K = 0, N = 0, group = 0;
+  const half* x = nullptr;      // [M, K]
+  const uint8_t* q = nullptr;   // [N, K/2]
+  const half* scale = nullptr;  // [N, ceil(K / group)]
+  const half* zero = nullptr;   // as scale, or nullptr: 8
+  int epi = kEpiNone;           // kEpiNone, kEpiRelu2 or kEpiF32
+  void* y = nullptr;            // half [M, N], or float for kEpiF32
+};
+int w4_group_linear(cudaStream_t stream, const W4GroupArgs& args);
+int quant_pack_w4_group(cudaStream_t stream, int N, int K, int group, const half* W, uint8_t* q, half* scale, half* zero);
+int quant_unpack_w4_group(cudaStream_t stream, int N, int K, int group, const uint8_t* q, const half* scale, const half* zero, half* W);
 
 // ---- quant.cu
 int quant_pack_w8(cudaStream_t stream, int N, int K, const half* W, int8_t* q, half* scale);

@@ -8,7 +8,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 
 FMT_F16, FMT_W8A16, FMT_W4A16 = 0, 1, 2
-DT_F16, DT_BF16 = 0, 1
+DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 ACT_NONE, ACT_TANH, ACT_SIGMOID = 0, 1, 2
 EPI_NONE, EPI_RELU2, EPI_F32 = 0, 1, 3
 
@@ -59,6 +59,9 @@ SIGNATURES = {
     "rwkv7_b200_greedy_pick": [_vp, _i, _i, _vp, _vp, _f, _f, _f, _vp, _vp],
     "rwkv7_b200_decode_sample": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, C.POINTER(Sampling), _vp, _vp, _vp],
     "rwkv7_b200_sample": [_vp, _i, _i, _vp, _vp, _vp, _f, _f, _f, C.POINTER(Sampling), _vp, _vp],
+    "rwkv7_b200_token_logprobs": [_vp, _i, _i, _vp, _i, _ll, _vp, _i, _i] + [_vp] * 5,
+    "rwkv7_b200_head_logprobs_workspace": [_i, _i, C.POINTER(C.c_size_t)],
+    "rwkv7_b200_head_logprobs": [_vp, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _i] + [_vp] * 5 + [C.c_size_t],
     "rwkv7_b200_copy_state_slice": [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
     "rwkv7_b200_state_blob_sizes": [_vp, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)],
     "rwkv7_b200_state_export": [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp],
@@ -92,6 +95,9 @@ SIGNATURES = {
     "rwkv7_b200_linear_f16_orig_static": [_vp, _i, _i, _i, _vp, _vp, _i, _vp],
     "rwkv7_b200_linear_w8a16": [_vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp],
     "rwkv7_b200_linear_w4a16": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp],
+    "rwkv7_b200_linear_w4a16_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _vp],
+    "rwkv7_b200_quant_pack_w4_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp],
+    "rwkv7_b200_quant_unpack_w4_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp],
     "rwkv7_b200_quant_pack_w8": [_vp, _i, _i, _vp, _vp, _vp],
     "rwkv7_b200_quant_unpack_w8": [_vp, _i, _i, _vp, _vp, _vp],
     "rwkv7_b200_quant_pack_w4": [_vp, _i, _i, _vp, _vp, _vp, _vp],

@@ -206,3 +206,128 @@ def sample(logits, penalties=None, presence=0.0, repetition=0.0, decay=1.0, temp
     L.check(L.load_library().rwkv7_b200_sample(_s(), B, V, _p(logits), _p(penalties), _p(probs), presence, repetition, decay,
                                                 C.byref(sp), _p(out), _p(next_tokens)))
     return out
+
+
+def _need(ok, message, status=1):
+    if not ok:
+        raise L.Rwkv7B200Error(status, message)
+
+
+def _tensor(name, t, dtypes, device, shape=None, contiguous=True):
+    """Checks one argument of the functions below: its type, device, shape and layout."""
+    dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
+    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{name}: {' or '.join(str(d) for d in dtypes)} tensor expected")
+    _need(t.is_cuda and (device is None or t.device == device), f"{name}: must be on the device of the other arguments")
+    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {tuple(shape or ())}", 2)
+    _need(not contiguous or t.is_contiguous(), f"{name}: must be contiguous")
+
+
+def token_logprobs(logits, tokens=None, top_k=0):
+    """Log probabilities under softmax(logits [rows, V]) (fp32 or fp16; rows may be strided): of the given ``tokens`` (int64
+    [rows] or [rows, n]; an id below 0 asks for nothing and gets 0, one beyond the vocabulary NaN), and of the ``top_k``
+    (at most 32) likeliest tokens, likeliest first, equal ones by index.  Returns (logprobs, entropy, lse, top_ids,
+    top_logprobs): fp32 shaped like ``tokens``, fp32 [rows], fp32 [rows], int32 and fp32 [rows, top_k]; None for what was not
+    asked.  -inf masks a token; a row with a NaN or +inf answers NaN."""
+    _need(isinstance(logits, torch.Tensor) and logits.dim() == 2, "token_logprobs: logits [rows, V] expected", 2)
+    _tensor("token_logprobs: logits", logits, (torch.float32, torch.float16), None, contiguous=False)
+    rows, V = logits.shape
+    _need(rows > 0 and V > 0, "token_logprobs: logits must not be empty")
+    _need((logits.stride(1) == 1 or V == 1) and (rows == 1 or logits.stride(0) >= V), "token_logprobs: a row's logits must be contiguous, rows must not overlap")
+    ld = logits.stride(0) if rows > 1 else V
+    dev = logits.device
+    n = 0
+    if tokens is not None:
+        _need(isinstance(tokens, torch.Tensor) and tokens.dim() in (1, 2), "token_logprobs: tokens [rows] or [rows, n] expected", 2)
+        n = tokens.shape[1] if tokens.dim() == 2 else 1
+        _tensor("token_logprobs: tokens", tokens, torch.int64, dev, (rows, n) if tokens.dim() == 2 else (rows,))
+    _need(isinstance(top_k, int) and 0 <= top_k <= 32, "token_logprobs: top_k outside [0, 32]")
+    with torch.cuda.device(dev):
+        f32 = dict(dtype=torch.float32, device=dev)
+        logprobs = torch.empty(tokens.shape, **f32) if tokens is not None else None
+        entropy, lse = torch.empty(rows, **f32), torch.empty(rows, **f32)
+        ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev) if top_k else None
+        top = torch.empty((rows, top_k), **f32) if top_k else None
+        L.check(L.load_library().rwkv7_b200_token_logprobs(
+            _s(), rows, V, C.c_void_p(logits.data_ptr()), L.DT_F16 if logits.dtype == torch.float16 else L.DT_F32, ld, _p(tokens), n,
+            top_k, _p(logprobs), _p(entropy), _p(lse), _p(ids), _p(top)))
+    return logprobs, entropy, lse, ids, top
+
+
+def _w4_group_params(what, scale, zero, rows, K, group, dev):
+    _need(group in (32, 64, 128), f"{what}: groups of 32, 64 or 128", 2)
+    groups = -(-K // group)
+    _tensor(f"{what}: scale", scale, torch.float16, dev, (rows, groups))
+    if zero is not None:
+        _tensor(f"{what}: zero", zero, torch.float16, dev, (rows, groups))
+
+
+def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128):
+    """``token_logprobs`` of x W^T (x fp16 [rows, K]) without writing the logits: one given token per row (int64 [rows] or
+    None).  ``weight`` is fp16 [V, K], int8 [V, K] with ``scale`` fp16 [V], or uint8 [V, K/2] (two 4-bit codes a byte) with
+    ``scale`` and ``zero`` (None: 8) fp16 [V, ceil(K / group_size)].  Returns (logprobs, entropy, lse), fp32 [rows]."""
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "head_logprobs: x [rows, K] expected", 2)
+    _tensor("head_logprobs: x", x, torch.float16, None)
+    rows, K = x.shape
+    dev = x.device
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] > 0, "head_logprobs: weight [V, K] expected", 2)
+    V = weight.shape[0]
+    _tensor("head_logprobs: weight", weight, (torch.float16, torch.int8, torch.uint8), dev, (V, K // 2 if weight.dtype == torch.uint8 else K))
+    fmt = {torch.float16: L.FMT_F16, torch.int8: L.FMT_W8A16, torch.uint8: L.FMT_W4A16}[weight.dtype]
+    if fmt == L.FMT_W8A16:
+        _tensor("head_logprobs: scale", scale, torch.float16, dev, (V,))
+    elif fmt == L.FMT_W4A16:
+        _w4_group_params("head_logprobs", scale, zero, V, K, group_size, dev)
+    if tokens is not None:
+        _tensor("head_logprobs: tokens", tokens, torch.int64, dev, (rows,))
+    lib = L.load_library()
+    with torch.cuda.device(dev):
+        need = C.c_size_t()
+        L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(need)))
+        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if tokens is not None else None
+        entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+        L.check(lib.rwkv7_b200_head_logprobs(_s(), rows, K, V, _p(x), _p(weight), fmt, _p(scale) if fmt else None, _p(zero) if fmt == 2 else None,
+                                             group_size, _p(tokens), _p(logprobs), _p(entropy), _p(lse), _p(work), need.value))
+    return logprobs, entropy, lse
+
+
+def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NONE):
+    """x W^T for 4-bit weights with group scales: W = (q - zero) * scale per group of 32, 64 or 128 inputs; x fp16 [M, K], q
+    uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N."""
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "linear_w4a16_group: x [M, K] expected", 2)
+    _tensor("linear_w4a16_group: x", x, torch.float16, None)
+    M, K = x.shape
+    _need(isinstance(q, torch.Tensor) and q.dim() == 2 and q.shape[0] > 0, "linear_w4a16_group: q [N, K/2] expected", 2)
+    N = q.shape[0]
+    _tensor("linear_w4a16_group: q", q, torch.uint8, x.device, (N, K // 2))
+    _w4_group_params("linear_w4a16_group", scale, zero, N, K, group_size, x.device)
+    with torch.cuda.device(x.device):
+        y = _out(x, N, epilogue)
+        L.check(L.load_library().rwkv7_b200_linear_w4a16_group(_s(), M, K, N, _p(x), _p(q), _p(scale), _p(zero), group_size, epilogue, _p(y)))
+    return y
+
+
+def quant_pack_w4_group(W, group_size=128, symmetric=False):
+    """4-bit codes, scales and zeros (None when ``symmetric``) of W fp16 [N, K] over groups of ``group_size`` inputs."""
+    _need(isinstance(W, torch.Tensor) and W.dim() == 2, "quant_pack_w4_group: W [N, K] expected", 2)
+    _tensor("quant_pack_w4_group: W", W, torch.float16, None)
+    N, K = W.shape
+    _need(group_size in (32, 64, 128), "quant_pack_w4_group: groups of 32, 64 or 128", 2)
+    with torch.cuda.device(W.device):
+        q = torch.empty((N, K // 2), dtype=torch.uint8, device=W.device)
+        s = torch.empty((N, -(-K // group_size)), dtype=torch.float16, device=W.device)
+        z = None if symmetric else torch.empty_like(s)
+        L.check(L.load_library().rwkv7_b200_quant_pack_w4_group(_s(), N, K, group_size, _p(W), _p(q), _p(s), _p(z)))
+    return q, s, z
+
+
+def quant_unpack_w4_group(q, scale, zero=None, group_size=128):
+    """The weights that the codes stand for, rounded to fp16 [N, K]."""
+    _need(isinstance(q, torch.Tensor) and q.dim() == 2, "quant_unpack_w4_group: q [N, K/2] expected", 2)
+    _tensor("quant_unpack_w4_group: q", q, torch.uint8, None)
+    N, K = q.shape[0], q.shape[1] * 2
+    _w4_group_params("quant_unpack_w4_group", scale, zero, N, K, group_size, q.device)
+    with torch.cuda.device(q.device):
+        W = torch.empty((N, K), dtype=torch.float16, device=q.device)
+        L.check(L.load_library().rwkv7_b200_quant_unpack_w4_group(_s(), N, K, group_size, _p(q), _p(scale), _p(zero), _p(W)))
+    return W

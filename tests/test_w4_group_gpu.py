@@ -1,0 +1,172 @@
+"""4-bit weights with group scales: packing, the product and the whole head end, against 64-bit references."""
+import numpy as np
+import pytest
+import torch
+
+from tests.head_end import U16, U32, check_logprobs, random_w4, ref_logprobs, softmax_tolerance, w4_weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from rwkv_lightning_cuda_b200 import ops as o
+    return o
+
+
+def check_product(y, x, weight, group, what):
+    """fp32 sums of K products: at most K / 16 additions to one running sum and 64 more in the merges, each off by at most one step of what has
+    been added up, codes and zeros apart: sum |x| (q + zero) scale.  Then one rounding to half (half a step, or of the smallest subnormal)."""
+    x64 = x.cpu().double()
+    want = x64 @ w4_weights(*weight, group).T
+    size = x64.abs() @ w4_weights(*weight, group, parts=True).T
+    bound = size * (x.shape[1] / 16 + 64) * 2 * U32 + want.abs() * U16 * (1 + 1e-3) + 2.0 ** -25
+    got = y.detach().cpu().double()
+    assert got.shape == want.shape
+    off = (got - want).abs() - bound
+    assert float(off.max()) <= 0, f"{what}: off by {float((got - want).abs().max()):.3g}"
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("N,K", [(1, 32), (5, 96), (16, 256), (33, 1056)])
+def test_pack_and_unpack(ops, N, K, group, symmetric):
+    """Scales, zeros and codes from the formulas in numpy's fp32, bit for bit; unpacking gives the codes' values rounded once."""
+    rng = np.random.default_rng(N + K + group)
+    W = (rng.standard_normal((N, K)) * 0.05).astype(np.float16)
+    W[0, :32] = 0
+    q, s, z = ops.quant_pack_w4_group(torch.from_numpy(W).cuda(), group, symmetric)
+    G = -(-K // group)
+    f = np.float32
+    for n in range(N):
+        for g in range(G):
+            w = W[n, g * group:(g + 1) * group].astype(f)
+            mn, mx = min(f(0), w.min()), max(f(0), w.max())
+            sc = np.float16(max(-mn, mx) / f(7)) if symmetric else np.float16((mx - mn) / f(15))
+            zero = f(8) if symmetric else f(0)
+            if not symmetric and sc > 0:
+                zero = f(np.clip(np.rint(-mn / f(sc)), 0, 15))
+            codes = np.clip(np.rint(w / f(sc)) + zero, 0, 15) if sc > 0 else np.full_like(w, zero)
+            assert float(s[n, g]) == float(sc) and (symmetric or float(z[n, g]) == float(zero))
+            row = q[n].cpu().numpy()[g * group // 2:(g * group + len(w)) // 2]
+            assert ((row & 15) == codes[0::2]).all() and ((row >> 4) == codes[1::2]).all()
+    back = ops.quant_unpack_w4_group(q, s, z, group).cpu().double()
+    assert torch.equal(back, w4_weights(q, s, z, group, rounded=True))
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 7, 64), (1, 300, 2080), (2, 64, 256), (3, 130, 512), (4, 2561, 1056), (5, 20, 4096), (8, 1000, 416),
+                                   (9, 33, 288), (16, 65, 2048), (1, 40, 16384), (7, 24, 16416), (16, 48, 10272)])
+def test_few_rows(ops, M, N, K, group, symmetric):
+    gen = torch.Generator().manual_seed(M + N + K + group)
+    q, s, z = random_w4(N, K, group, symmetric, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    check_product(ops.linear_w4a16_group(x, q, s, z, group), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
+
+
+def test_epilogues(ops):
+    from rwkv_lightning_cuda_b200 import lib as L
+    gen = torch.Generator().manual_seed(2)
+    q, s, z = random_w4(70, 320, 64, False, gen)
+    for M in (1, 6, 20, 70):
+        x = torch.randn(M, 320, generator=gen).half().cuda()
+        y = ops.linear_w4a16_group(x, q, s, z, 64)
+        y32 = ops.linear_w4a16_group(x, q, s, z, 64, epilogue=L.EPI_F32)
+        assert y32.dtype == torch.float32 and torch.equal(y32, y.float())
+        relu2 = ops.linear_w4a16_group(x, q, s, z, 64, epilogue=L.EPI_RELU2)
+        assert torch.equal(relu2, (y.float().clamp(min=0) ** 2).half())
+
+
+@pytest.mark.parametrize("M", [1, 3, 8, 40])
+def test_small_and_special_activations(ops, M):
+    """Activations down to the smallest subnormal half keep their value, large ones do not overflow in between, and an infinity or NaN stays in
+    its row."""
+    gen = torch.Generator().manual_seed(5)
+    q, s, z = random_w4(48, 512, 64, False, gen)
+    x = (torch.randn(M, 512, generator=gen) * 2e-6).half().cuda()
+    wide = (s.float() * 50).half()
+    check_product(ops.linear_w4a16_group(x, q, wide, z, 64), x, (q, wide, z), 64, "subnormal activations")
+    big = (torch.randn(M, 512, generator=gen) * 2000).half().cuda()
+    check_product(ops.linear_w4a16_group(big, q, s, z, 64), big, (q, s, z), 64, "large activations")
+    if M > 1:
+        x = torch.randn(M, 512, generator=gen).half().cuda()
+        clean = ops.linear_w4a16_group(x, q, s, z, 64)
+        x[1, 100] = float("nan")
+        got = ops.linear_w4a16_group(x, q, s, z, 64)
+        keep = [m for m in range(M) if m != 1]
+        assert torch.equal(got[keep], clean[keep]) and bool(torch.isnan(got[1]).all())
+
+
+def test_codes_one_at_a_time(ops):
+    """Each of the 16 codes at each place of a word, and each group's own scale: one weight at a time against one activation."""
+    K, group = 288, 32
+    for code in range(16):
+        N = K
+        w = torch.full((N, K), 3, dtype=torch.uint8)
+        w[torch.arange(K), torch.arange(K)] = code
+        q = (w[:, 0::2] | (w[:, 1::2] << 4)).cuda()
+        s = torch.linspace(0.5, 2, K // group).half().expand(N, -1).contiguous().cuda()
+        z = torch.full((N, K // group), 3.0).half().cuda()
+        x = torch.arange(1, K + 1).half()[None].cuda()
+        y = ops.linear_w4a16_group(x, q, s, z, group)
+        want = (code - 3) * torch.arange(1, K + 1).double() * s[0].cpu().double().repeat_interleave(group)
+        assert torch.equal(y[0].cpu(), want.half())
+
+
+def test_two_calls_and_replays_are_equal(ops):
+    gen = torch.Generator().manual_seed(6)
+    q, s, z = random_w4(515, 2080, 128, False, gen)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for M in (1, 5, 24, 100):
+            x = torch.randn(M, 2080, generator=gen).half().cuda()
+            a, b = ops.linear_w4a16_group(x, q, s, z, 128), ops.linear_w4a16_group(x, q, s, z, 128)
+            assert torch.equal(a, b)
+            graphs = []
+            for _ in range(2):
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=st):
+                    graphs.append((ops.linear_w4a16_group(x, q, s, z, 128), g))
+            x.mul_(0.5)
+            for _, g in graphs:
+                g.replay()
+            want = ops.linear_w4a16_group(x, q, s, z, 128)
+            for y, _ in graphs:
+                assert torch.equal(y, want)
+    st.synchronize()
+
+
+def test_refusals(ops):
+    from rwkv_lightning_cuda_b200 import lib as L
+    q, s, z = random_w4(8, 128, 64, False, torch.Generator().manual_seed(1))
+    x = torch.zeros(2, 128, dtype=torch.float16, device="cuda")
+    for bad in (lambda: ops.linear_w4a16_group(x, q, s, z, 32), lambda: ops.linear_w4a16_group(x, q, s, z[:, :1].contiguous(), 64),
+                lambda: ops.linear_w4a16_group(x.float(), q, s, z, 64), lambda: ops.linear_w4a16_group(x[:, :64], q, s, z, 64),
+                lambda: ops.linear_w4a16_group(x, q.t(), s, z, 64), lambda: ops.linear_w4a16_group(x[:0], q, s, z, 64),
+                lambda: ops.linear_w4a16_group(x, q, s.float(), z, 64), lambda: ops.linear_w4a16_group(x, q, s, z, 64, epilogue=2),
+                lambda: ops.linear_w4a16_group(x.cpu(), q, s, z, 64), lambda: ops.quant_pack_w4_group(x[:, :40].contiguous(), 32),
+                lambda: ops.quant_unpack_w4_group(q, s, z, 128)):
+        with pytest.raises(L.Rwkv7B200Error):
+            bad()
+
+
+def test_head_end_of_a_step(ops):
+    """The run a decode step ends with: a 4-bit head in fine groups, logits in fp32, then the chosen token's log probability with alternatives; and the
+    fused route over the same weights."""
+    from rwkv_lightning_cuda_b200 import lib as L
+    gen = torch.Generator().manual_seed(11)
+    W = (torch.randn(5003, 256, generator=gen) * 0.08).half().cuda()
+    x = torch.randn(3, 256, generator=gen).half().cuda()
+    q, s, z = ops.quant_pack_w4_group(W, 32)
+    logits = ops.linear_w4a16_group(x, q, s, z, 32, epilogue=L.EPI_F32)
+    chosen = ops.greedy_pick(logits)
+    got = ops.token_logprobs(logits, chosen.long(), top_k=5)
+    check_logprobs(got, ref_logprobs(logits, chosen.long(), 5), softmax_tolerance(5003, float(logits.abs().max())), "step")
+    assert torch.equal(got[3][:, 0], chosen) and torch.equal(got[4][:, 0], got[0])
+    fused = ops.head_logprobs(x, q, chosen.long(), scale=s, zero=z, group_size=32)
+    # the logits of the first route are rounded to half, the weights of the second
+    size = float((x.double().abs() @ w4_weights(q, s, z, 32).abs().T.cuda()).max())
+    slack = 2 * (float(logits.abs().max()) * U16 + size * U16) + softmax_tolerance(5003, 10)
+    assert float((fused[0] - got[0]).abs().max()) <= slack
