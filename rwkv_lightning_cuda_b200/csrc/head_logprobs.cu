@@ -380,9 +380,9 @@ int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size
              head_logprobs_workspace(a.rows, a.V));
   a.part = static_cast<float4*>(workspace);
   a.given = reinterpret_cast<float*>(a.part + (static_cast<size_t>(a.V) + kToks - 1) / kToks * a.rows);
-  int dev = 0, sms = 0;
-  RK_CUDA(cudaGetDevice(&dev));
-  RK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  int sms = 0;
+  const int status = device_sms(&sms);
+  if (status != kOk) return status;
   if (a.fmt == 1) return launch_head<1>(stream, a, sms);
   if (a.fmt == 2) return launch_head<2>(stream, a, sms);
   return launch_head<0>(stream, a, sms);

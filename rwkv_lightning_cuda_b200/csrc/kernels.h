@@ -19,6 +19,7 @@ int* timeout_word_or_null();                  // the same for launchers: nullptr
 int timeout_detail(int* out15, bool clear);   // status.cu: the first expired GEMM wait of the current device
 int timeout_read(int* flags, bool clear);     // blocking read (and reset) of the current device's word
 int timeout_status(int flags);                // kOk, or kTimeout with the message set
+int device_sms(int* sms);                     // SM count of the current device
 int wait_probe(cudaStream_t stream, unsigned polls);  // a kernel whose bounded wait runs out by construction (tests)
 
 // The few switches that exist for measurements and tests; rwkv7_b200_set_option() sets them by name.  Process-wide,

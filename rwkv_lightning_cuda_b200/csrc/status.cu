@@ -46,6 +46,13 @@ int timeout_word(int** out) {
   return kOk;
 }
 
+int device_sms(int* sms) {
+  int dev = 0;
+  RK_CUDA(cudaGetDevice(&dev));
+  RK_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return kOk;
+}
+
 int* timeout_word_or_null() {
   int* p = nullptr;
   return timeout_word(&p) == kOk ? p : nullptr;

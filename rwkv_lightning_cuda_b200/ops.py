@@ -216,10 +216,31 @@ def _need(ok, message, status=1):
 def _tensor(name, t, dtypes, device, shape=None, contiguous=True):
     """Checks one argument of the functions below: its type, device, shape and layout."""
     dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
-    _need(isinstance(t, torch.Tensor) and t.dtype in dtypes, f"{name}: {' or '.join(str(d) for d in dtypes)} tensor expected")
-    _need(t.is_cuda and (device is None or t.device == device), f"{name}: must be on the device of the other arguments")
-    _need(shape is None or tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, expected {tuple(shape or ())}", 2)
-    _need(not contiguous or t.is_contiguous(), f"{name}: must be contiguous")
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        _need(False, f"{name}: {' or '.join(str(d) for d in dtypes)} tensor expected")
+    if not t.is_cuda or (device is not None and t.device != device):
+        _need(False, f"{name}: must be on the device of the other arguments")
+    if shape is not None and t.shape != shape:
+        _need(False, f"{name}: shape {tuple(t.shape)}, expected {shape}", 2)
+    if contiguous and not t.is_contiguous():
+        _need(False, f"{name}: must be contiguous")
+
+
+def _enqueue(dev, call, *args):
+    """One library call on the current stream of ``dev``, which need not be the current device; the tensors' addresses are passed as
+    integers (None: NULL), the checks have been made."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        status = call(torch._C._cuda_getCurrentRawStream(index), *args)
+    else:
+        with torch.cuda.device(index):
+            status = call(torch._C._cuda_getCurrentRawStream(index), *args)
+    if status:
+        L.check(status)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def token_logprobs(logits, tokens=None, top_k=0):
@@ -232,24 +253,25 @@ def token_logprobs(logits, tokens=None, top_k=0):
     _tensor("token_logprobs: logits", logits, (torch.float32, torch.float16), None, contiguous=False)
     rows, V = logits.shape
     _need(rows > 0 and V > 0, "token_logprobs: logits must not be empty")
-    _need((logits.stride(1) == 1 or V == 1) and (rows == 1 or logits.stride(0) >= V), "token_logprobs: a row's logits must be contiguous, rows must not overlap")
-    ld = logits.stride(0) if rows > 1 else V
+    ld, along = logits.stride()
+    if rows == 1:
+        ld = V
+    _need((along == 1 or V == 1) and ld >= V, "token_logprobs: a row's logits must be contiguous, rows must not overlap")
     dev = logits.device
-    n = 0
+    n, logprobs, ids, top = 0, None, None, None
     if tokens is not None:
         _need(isinstance(tokens, torch.Tensor) and tokens.dim() in (1, 2), "token_logprobs: tokens [rows] or [rows, n] expected", 2)
         n = tokens.shape[1] if tokens.dim() == 2 else 1
         _tensor("token_logprobs: tokens", tokens, torch.int64, dev, (rows, n) if tokens.dim() == 2 else (rows,))
-    _need(isinstance(top_k, int) and 0 <= top_k <= 32, "token_logprobs: top_k outside [0, 32]")
-    with torch.cuda.device(dev):
-        f32 = dict(dtype=torch.float32, device=dev)
-        logprobs = torch.empty(tokens.shape, **f32) if tokens is not None else None
-        entropy, lse = torch.empty(rows, **f32), torch.empty(rows, **f32)
-        ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev) if top_k else None
-        top = torch.empty((rows, top_k), **f32) if top_k else None
-        L.check(L.load_library().rwkv7_b200_token_logprobs(
-            _s(), rows, V, C.c_void_p(logits.data_ptr()), L.DT_F16 if logits.dtype == torch.float16 else L.DT_F32, ld, _p(tokens), n,
-            top_k, _p(logprobs), _p(entropy), _p(lse), _p(ids), _p(top)))
+        logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    _need(type(top_k) is int and 0 <= top_k <= 32, "token_logprobs: top_k outside [0, 32]")
+    entropy, lse = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    if top_k:
+        ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+        top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    _enqueue(dev, L.load_library().rwkv7_b200_token_logprobs, rows, V, logits.data_ptr(),
+             L.DT_F16 if logits.dtype == torch.float16 else L.DT_F32, ld, _address(tokens), n, top_k, _address(logprobs), entropy.data_ptr(),
+             lse.data_ptr(), _address(ids), _address(top))
     return logprobs, entropy, lse, ids, top
 
 
@@ -259,6 +281,9 @@ def _w4_group_params(what, scale, zero, rows, K, group, dev):
     _tensor(f"{what}: scale", scale, torch.float16, dev, (rows, groups))
     if zero is not None:
         _tensor(f"{what}: zero", zero, torch.float16, dev, (rows, groups))
+
+
+_HEAD_FORMATS = {torch.float16: L.FMT_F16, torch.int8: L.FMT_W8A16, torch.uint8: L.FMT_W4A16}
 
 
 def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128):
@@ -271,23 +296,24 @@ def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128)
     dev = x.device
     _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] > 0, "head_logprobs: weight [V, K] expected", 2)
     V = weight.shape[0]
-    _tensor("head_logprobs: weight", weight, (torch.float16, torch.int8, torch.uint8), dev, (V, K // 2 if weight.dtype == torch.uint8 else K))
-    fmt = {torch.float16: L.FMT_F16, torch.int8: L.FMT_W8A16, torch.uint8: L.FMT_W4A16}[weight.dtype]
+    fmt = _HEAD_FORMATS.get(weight.dtype, -1)
+    _tensor("head_logprobs: weight", weight, (torch.float16, torch.int8, torch.uint8), dev, (V, K // 2 if fmt == L.FMT_W4A16 else K))
     if fmt == L.FMT_W8A16:
         _tensor("head_logprobs: scale", scale, torch.float16, dev, (V,))
     elif fmt == L.FMT_W4A16:
         _w4_group_params("head_logprobs", scale, zero, V, K, group_size, dev)
+    logprobs = None
     if tokens is not None:
         _tensor("head_logprobs: tokens", tokens, torch.int64, dev, (rows,))
+        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
     lib = L.load_library()
-    with torch.cuda.device(dev):
-        need = C.c_size_t()
-        L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if tokens is not None else None
-        entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-        L.check(lib.rwkv7_b200_head_logprobs(_s(), rows, K, V, _p(x), _p(weight), fmt, _p(scale) if fmt else None, _p(zero) if fmt == 2 else None,
-                                             group_size, _p(tokens), _p(logprobs), _p(entropy), _p(lse), _p(work), need.value))
+    need = C.c_size_t()
+    L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(need)))
+    work = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    entropy, lse = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    _enqueue(dev, lib.rwkv7_b200_head_logprobs, rows, K, V, x.data_ptr(), weight.data_ptr(), fmt, _address(scale) if fmt else None,
+             _address(zero) if fmt == L.FMT_W4A16 else None, group_size, _address(tokens), _address(logprobs), entropy.data_ptr(), lse.data_ptr(),
+             work.data_ptr(), need.value)
     return logprobs, entropy, lse
 
 
@@ -297,13 +323,14 @@ def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NO
     _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "linear_w4a16_group: x [M, K] expected", 2)
     _tensor("linear_w4a16_group: x", x, torch.float16, None)
     M, K = x.shape
+    dev = x.device
     _need(isinstance(q, torch.Tensor) and q.dim() == 2 and q.shape[0] > 0, "linear_w4a16_group: q [N, K/2] expected", 2)
     N = q.shape[0]
-    _tensor("linear_w4a16_group: q", q, torch.uint8, x.device, (N, K // 2))
-    _w4_group_params("linear_w4a16_group", scale, zero, N, K, group_size, x.device)
-    with torch.cuda.device(x.device):
-        y = _out(x, N, epilogue)
-        L.check(L.load_library().rwkv7_b200_linear_w4a16_group(_s(), M, K, N, _p(x), _p(q), _p(scale), _p(zero), group_size, epilogue, _p(y)))
+    _tensor("linear_w4a16_group: q", q, torch.uint8, dev, (N, K // 2))
+    _w4_group_params("linear_w4a16_group", scale, zero, N, K, group_size, dev)
+    y = torch.empty((M, N), dtype=torch.float32 if epilogue == L.EPI_F32 else torch.float16, device=dev)
+    _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(), _address(zero), group_size,
+             epilogue, y.data_ptr())
     return y
 
 
