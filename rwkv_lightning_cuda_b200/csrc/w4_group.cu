@@ -1,35 +1,68 @@
 // 4-bit weights with group scales: y = epi(x W^T) with W[n,k] = (q[n,k] - zero[n,g]) * scale[n,g], g = k / group, for
 // groups of 32, 64 or 128 input channels, the last of which may be short, and without zeros (then 8) or with them.
-// Packing as the other 4-bit format: byte j of a row holds q[2j] (low nibble) and q[2j + 1] (high nibble).  The scale
-// multiplies the group's sum in fp32: a weight is never rounded to half, unlike in the format of groups of 128 that the
-// models' matrices use.
-// One warp per output channel and row; lane i takes the words (8 weights) i, i + 32, ...
+// Packing as the other 4-bit format: byte j of a row holds q[2j] (low nibble) and q[2j + 1] (high nibble).
+//
+// Up to eight rows of x (one launch each): bound by the weights' bytes, and next by instruction issue, so the kernel spends as
+// little as it can on a weight.
+//   - A nibble under a mask IS a half: 0x000q is the subnormal q 2^-24 and 0x00q0 is 16 q 2^-24, which the tensor cores
+//     multiply exactly.  Turning a 32-bit word into four operand registers costs one shift and four ANDs, no conversion;
+//     low and high nibbles go to sums of their own (lo, hi), joined as lo + hi / 16.
+//   - Scales and zeros multiply the sums of a group, in fp32:  y = sum_g s_g (sum_k q x - z_g sum_k x), with the sums of x
+//     made once per CTA.  A weight is never rounded to half, unlike in the format of groups of 128 that the models use.
+//   - mma.sync m16n8k16 has eight columns.  With fewer rows of x the columns hold different 32-weight chunks (a
+//     lane whose column is another chunk's reads zeros), so that with one row eight chunks end up in eight columns and the
+//     scales are applied once for all of them.
+// One CTA of 16 warps per SM takes a contiguous range of output channels in tiles of up to 32; a tile's K extent is cut into
+// boxes of 128 bytes per row, box b going to warp b mod 16, fetched by one 2-D tensor copy into the warp's ring.  The warps'
+// partial sums of a tile are added in warp order: results do not depend on timing.
+#include <cuda.h>
+
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
+#include "tensormap.h"
 
 namespace rk {
 namespace {
 
-__global__ void __launch_bounds__(256) w4_group_simple_kernel(W4GroupArgs a) {
-  const int n = blockIdx.x * 8 + (threadIdx.x >> 5), m = blockIdx.y, lane = threadIdx.x & 31;
-  if (n >= a.N) return;
-  const int groups = (a.K + a.group - 1) / a.group, shift = 31 - __clz(a.group);
-  const uint32_t* qw = reinterpret_cast<const uint32_t*>(a.q + static_cast<size_t>(n) * (a.K >> 1));
-  const half* x = a.x + static_cast<size_t>(m) * a.K;
-  float acc = 0.f;
-  for (int w = lane; w < (a.K >> 3); w += 32) {
-    const size_t g = static_cast<size_t>(n) * groups + ((w << 3) >> shift);
-    const float s = __half2float(a.scale[g]), z = a.zero ? __half2float(a.zero[g]) : 8.f;
-    const uint32_t u = qw[w];
-    float part = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part += (static_cast<float>((u >> (4 * i)) & 15u) - z) * __half2float(x[(w << 3) + i]);
-    acc += part * s;
-  }
-  acc = warp_sum(acc);
-  if (lane != 0) return;
-  const size_t o = static_cast<size_t>(m) * a.N + n;
-  const half hy = __float2half_rn(acc);
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kTileRows = 32;
+constexpr int kBoxWeights = 256;  // 128 bytes along a row: eight chunks of 32 weights
+constexpr int kMaxRows = 8;
+constexpr size_t kSmemLimit = 226 * 1024;
+
+struct MatvecPlan {
+  int h = 0, tiles = 0;         // rows of a tile and box, tiles per CTA
+  int boxes = 0;                // along a weight row
+  int slots = 0, slot_bytes = 0;
+  int x_pitch = 0;              // bytes from one staged row of x to the next: 64 modulo 128, two rows share no bank
+  uint32_t part_off = 0, sums_off = 0, x_off = 0;  // from the aligned start of shared memory
+  size_t smem = 0;
+  int grid = 0;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
+  if (first)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&w)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float half_of(uint32_t pair, int i) {
+  const float2 f = h2f2(pair);
+  return i ? f.y : f.x;
+}
+__device__ __forceinline__ void store_epi(const W4GroupArgs& a, size_t o, float v) {
+  const half hy = __float2half_rn(v);
   if (a.epi == kEpiF32) {
     static_cast<float*>(a.y)[o] = __half2float(hy);
   } else if (a.epi == kEpiRelu2) {
@@ -37,6 +70,233 @@ __global__ void __launch_bounds__(256) w4_group_simple_kernel(W4GroupArgs a) {
     static_cast<half*>(a.y)[o] = __float2half_rn(u * u);
   } else {
     static_cast<half*>(a.y)[o] = hy;
+  }
+}
+
+// kM: columns per chunk, the rows of x rounded up to 1, 2, 4 or 8; kShift: log2 of the group.  A box is worked off in passes of
+// kPass chunks, after each of which the sums are scaled; chunk c of a pass goes to the columns of slot c mod kSlots.
+template <int kM, int kShift>
+__global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_constant__ CUtensorMap map, const W4GroupArgs a, const MatvecPlan p, int* timeout) {
+  constexpr int kSlots = 8 / kM, kGroupChunks = 1 << (kShift - 5);
+  constexpr int kPass = kSlots > kGroupChunks ? kSlots : kGroupChunks, kPasses = 8 / kPass;
+  constexpr float kUnit = 1.0f / 16777216.0f;  // what a code of 1 stands for in the products
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t bars[kWarps][4];
+  __shared__ uint4 zeros;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint32_t dyn = smem_u32(smem_dyn), base = (dyn + 1023u) & ~1023u;
+  unsigned char* const mem = smem_dyn + (base - dyn);
+  const uint32_t ring = base + warp * p.slots * p.slot_bytes;
+  float* const part = reinterpret_cast<float*>(mem + p.part_off);
+  float* const sums = reinterpret_cast<float*>(mem + p.sums_off);
+  const int row0 = blockIdx.x * p.tiles * p.h, tiles = min(p.tiles, (a.N - row0 + p.h - 1) / p.h);
+  const int groups = (a.K + (1 << kShift) - 1) >> kShift;
+
+  if (lane == 0) {
+    for (int i = 0; i < p.slots; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) zeros = make_uint4(0u, 0u, 0u, 0u);
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
+
+  // this warp's boxes: warp, warp + 16, ... of the flattened (tile, box) sequence
+  auto advance = [&](int& tile, int& kb) {
+    kb += kWarps;
+    while (kb >= p.boxes && tile < tiles) { kb -= p.boxes; ++tile; }
+  };
+  int q_tile = 0, q_kb = warp - kWarps, q_slot = 0;
+  advance(q_tile, q_kb);
+  auto issue = [&]() {
+    if (lane == 0) {
+      const uint32_t bar = smem_u32(&bars[warp][q_slot]);
+      mbar_expect_tx(bar, p.h * 128);
+      asm volatile(
+          "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+          ::"r"(ring + q_slot * p.slot_bytes), "l"(&map), "r"(bar), "r"(q_kb << 7), "r"(row0 + q_tile * p.h)
+          : "memory");
+    }
+    if (++q_slot == p.slots) q_slot = 0;
+    advance(q_tile, q_kb);
+  };
+  for (int i = 0; i < p.slots && q_tile < tiles; ++i) issue();
+
+  // A lane's share of a box's scales and zeros, for the rows g, g + 8, g + 16, g + 24: groups of 32: the pair 2t, 2t + 1 of the
+  // box's eight; of 64: group t of four; of 128: group t / 2 of two.
+  uint32_t sc[4], ze[4];
+  const bool paired = (groups & 1) == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 3) == 0;
+  auto fetch = [&](int tile, int kb) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const size_t r = static_cast<size_t>(min(row0 + tile * p.h + g + 8 * i, a.N - 1)) * groups;
+      ze[i] = 0x48004800u;  // 8, 8
+      if (kShift == 5 && paired) {
+        const size_t o = r + min(kb * 8 + 2 * t, groups - 2);
+        sc[i] = *reinterpret_cast<const uint32_t*>(a.scale + o);
+        if (a.zero) ze[i] = *reinterpret_cast<const uint32_t*>(a.zero + o);
+      } else if (kShift == 5) {
+        const size_t o0 = r + min(kb * 8 + 2 * t, groups - 1), o1 = r + min(kb * 8 + 2 * t + 1, groups - 1);
+        const uint16_t *s = reinterpret_cast<const uint16_t*>(a.scale), *z = reinterpret_cast<const uint16_t*>(a.zero);
+        sc[i] = s[o0] | (static_cast<uint32_t>(s[o1]) << 16);
+        if (a.zero) ze[i] = z[o0] | (static_cast<uint32_t>(z[o1]) << 16);
+      } else {
+        const size_t o = r + min(kShift == 6 ? kb * 4 + t : kb * 2 + (t >> 1), groups - 1);
+        sc[i] = reinterpret_cast<const uint16_t*>(a.scale)[o];
+        if (a.zero) ze[i] = reinterpret_cast<const uint16_t*>(a.zero)[o];
+      }
+    }
+  };
+  int c_tile = 0, c_kb = warp - kWarps;
+  advance(c_tile, c_kb);
+  if (c_tile < tiles) fetch(c_tile, c_kb);
+
+  // x as halves in the order of the fragments: a block of eight as x0 x4 x2 x6 | x1 x5 x3 x7 (the operands of the low and of the high
+  // nibbles of a word); zeros behind K.  The sums of the chunks of 32 go to shared memory beside it.
+  const int blocks = p.boxes * 32, chunks = p.boxes * 8;
+  float* const chunk_sums = part;  // [M][chunks], until the first tile's partial sums
+  for (int i = threadIdx.x; i < a.M * blocks; i += kThreads) {
+    const int m = i / blocks, j = i - m * blocks;
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (j * 8 < a.K) q = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + j * 8);
+    *reinterpret_cast<uint4*>(mem + p.x_off + m * p.x_pitch + j * 16) =
+        make_uint4(__byte_perm(q.x, q.z, 0x5410), __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.x, q.z, 0x7632), __byte_perm(q.y, q.w, 0x7632));
+    const float2 f0 = h2f2(q.x), f1 = h2f2(q.y), f2 = h2f2(q.z), f3 = h2f2(q.w);
+    float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // (a.M * blocks is a multiple of 32: whole warps take part)
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    if ((j & 3) == 0) chunk_sums[m * chunks + (j >> 2)] = sum;
+  }
+  __syncthreads();
+  // -2^-24 times the sum of x that belongs to each column of each pass: [box][pass][8]
+  for (int i = threadIdx.x; i < p.boxes * kPasses * 8; i += kThreads) {
+    const int col = i & 7, c0 = (i >> 3) * kPass + col / kM, m = min(col % kM, a.M - 1);
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < kPass; c += kSlots) sum += chunk_sums[m * chunks + c0 + c];
+    sums[i] = -kUnit * sum;
+  }
+  __syncthreads();
+
+  const uint32_t w_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);  // see ldmatrix below
+  const int slot_of_lane = g / kM;
+  const uint32_t x_lane = base + p.x_off + min(g % kM, a.M - 1) * p.x_pitch + (t << 4), zero_addr = smem_u32(&zeros);
+  float acc[2][4];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
+  int cur = 0, slot = 0, phase = 0;
+  bool dead = false;  // a wait ran out: no more work, but the barriers are kept
+  const bool two = p.h > 16;
+  for (;;) {
+    // Tile boundaries: every warp leaves its sums, and one barrier later all threads add up the tile.
+    for (const int upto = min(c_tile, tiles); cur < upto; ++cur) {
+      float* const mine = part + (cur & 1) * kWarps * kTileRows * kM + warp * kTileRows * kM;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v = acc[b][i];  // row 16 b + g + 8 (i / 2), column 2 t + i % 2
+          acc[b][i] = 0.f;
+          if (kM == 1) {
+            if (i & 1) continue;
+            v += acc[b][i + 1];
+            acc[b][i + 1] = 0.f;
+          }
+          if (kM <= 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
+          if (kM <= 4) v += __shfl_xor_sync(0xffffffffu, v, 2);
+          const int m = kM == 1 ? 0 : (2 * t + (i & 1)) % kM;
+          if (2 * t < kM || (kM == 1 && t == 0)) mine[(16 * b + g + 8 * (i >> 1)) * kM + m] = v;
+        }
+      }
+      __syncthreads();
+      const int r = threadIdx.x % kTileRows, m = threadIdx.x / kTileRows, n = row0 + cur * p.h + r;
+      if (r < p.h && m < a.M && n < a.N) {
+        const float* src = part + (cur & 1) * kWarps * kTileRows * kM + r * kM + m;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += src[w * kTileRows * kM];
+        store_epi(a, static_cast<size_t>(m) * a.N + n, v * 16777216.0f);
+      }
+    }
+    if (c_tile >= tiles) break;
+
+    const int kb = c_kb;
+    uint32_t s_now[4], z_now[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { s_now[i] = sc[i]; z_now[i] = ze[i]; }
+    advance(c_tile, c_kb);
+    if (c_tile < tiles) fetch(c_tile, c_kb);
+    const uint32_t bar = smem_u32(&bars[warp][slot]);
+    if (!dead && !mbar_try_wait(bar, phase) && !mbar_wait(bar, phase)) {
+      dead = true;
+      if (lane == 0 && timeout) atomicOr(timeout, kTimeoutGemv);
+    }
+    if (!dead) {
+      const uint32_t wbase = ring + slot * p.slot_bytes;
+      float lo[2][4], hi[2][4];
+#pragma unroll
+      for (int c2 = 0; c2 < 4; ++c2) {
+        // Two chunks of 16 rows: the matrices are (rows 0-7, rows 8-15) x (chunk 2 c2, chunk 2 c2 + 1), 16 bytes a row, and a lane gets
+        // the word t of row g.  The 128-byte swizzle puts chunk c of row r at c ^ (r mod 8).
+        uint32_t w[2][4];
+        ldmatrix4(w[0], wbase + (w_lane ^ (c2 << 5)));
+        if (two) ldmatrix4(w[1], wbase + 2048 + (w_lane ^ (c2 << 5)));
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          const int c = 2 * c2 + cc;
+          const uint32_t xa = x_lane + (kb << 9) + (c << 6);
+          uint4 xv;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
+                       : "r"(kSlots == 1 || slot_of_lane == c % kSlots ? xa : zero_addr));
+          const bool first = c % kPass == 0;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && !two) break;
+            const uint32_t wa = w[b][2 * cc], wb = w[b][2 * cc + 1], va = wa >> 8, vb = wb >> 8;
+            mma16816(lo[b], wa & 0x000f000fu, wb & 0x000f000fu, va & 0x000f000fu, vb & 0x000f000fu, xv.x, xv.y, first);
+            mma16816(hi[b], wa & 0x00f000f0u, wb & 0x00f000f0u, va & 0x00f000f0u, vb & 0x00f000f0u, xv.z, xv.w, first);
+          }
+          if ((c + 1) % kPass != 0) continue;
+          // the end of a pass: scales and zeros of the groups that this lane's two columns hold
+          const int pass = c / kPass;
+          const float2 xs = *reinterpret_cast<const float2*>(sums + (kb * kPasses + pass) * 8 + 2 * t);
+          // the chunk of the column 2t, and where its group's parameters are: (lane of the quad, half of the pair)
+          const int chunk = kM == 1 ? 2 * t : pass * kPass + (kM == 8 ? 0 : 2 * t / kM);
+          const int from = kShift == 5 ? chunk >> 1 : kShift == 6 ? chunk >> 1 : (chunk >> 2) << 1;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b == 1 && !two) break;
+            float s0[2], s1[2], z0[2], z1[2];  // rows g and g + 8: of the lane's first and second column
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t sp = s_now[2 * b + i], zp = z_now[2 * b + i];
+              if (kM > 1) {
+                sp = __shfl_sync(0xffffffffu, sp, (lane & ~3) | from);
+                zp = __shfl_sync(0xffffffffu, zp, (lane & ~3) | from);
+              }
+              if (kM == 1 && kShift == 5) {
+                s0[i] = half_of(sp, 0); s1[i] = half_of(sp, 1);
+                z0[i] = half_of(zp, 0); z1[i] = half_of(zp, 1);
+              } else {
+                const int odd = kShift == 5 ? chunk & 1 : 0;
+                s0[i] = s1[i] = half_of(sp, odd);
+                z0[i] = z1[i] = half_of(zp, odd);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float u = fmaf(hi[b][i], 0.0625f, lo[b][i]);
+              acc[b][i] = fmaf(i & 1 ? s1[i >> 1] : s0[i >> 1], fmaf(i & 1 ? z1[i >> 1] : z0[i >> 1], i & 1 ? xs.y : xs.x, u), acc[b][i]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();  // every lane has read the slot: it may be overwritten
+    if (!dead && q_tile < tiles) issue();
+    if (++slot == p.slots) { slot = 0; phase ^= 1; }
   }
 }
 
@@ -100,6 +360,71 @@ int check_shape(const char* what, int N, int K, int group) {
 
 }  // namespace
 
+namespace {
+
+int columns(int M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
+
+// One tile height for all CTAs, so that a box is exactly a CTA's rows: N / SMs rows each, in equal tiles of at most 32.
+bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
+  const int kM = columns(a.M), group_chunks = a.group / 32, pass = std::max(8 / kM, group_chunks), passes = 8 / pass;
+  for (const int most : {kTileRows, 16}) {  // tiles of 16 where those of 32 leave no room for two boxes per warp
+    MatvecPlan p;
+    const int target = (a.N + sms - 1) / sms;
+    p.tiles = (target + most - 1) / most;
+    p.h = (target + p.tiles - 1) / p.tiles;
+    p.grid = (a.N + p.tiles * p.h - 1) / (p.tiles * p.h);
+    p.boxes = (a.K + kBoxWeights - 1) / kBoxWeights;
+    p.slot_bytes = (p.h * 128 + 1023) & ~1023;
+    p.x_pitch = p.boxes * kBoxWeights * 2 + 64;
+    const size_t part = std::max<size_t>(2u * kWarps * kTileRows * kM * sizeof(float), static_cast<size_t>(a.M) * p.boxes * 8 * sizeof(float));
+    const size_t sums = static_cast<size_t>(p.boxes) * passes * 8 * sizeof(float), x = static_cast<size_t>(a.M) * p.x_pitch;
+    const size_t fixed = 1024 + ((part + 127) & ~static_cast<size_t>(127)) + ((sums + 127) & ~static_cast<size_t>(127)) + x;
+    const size_t per_slot = static_cast<size_t>(kWarps) * p.slot_bytes;
+    if (fixed + 2 * per_slot > kSmemLimit) continue;
+    p.slots = static_cast<int>(std::min<size_t>(4, (kSmemLimit - fixed) / per_slot));
+    p.part_off = static_cast<uint32_t>(p.slots * per_slot);
+    p.sums_off = p.part_off + static_cast<uint32_t>((part + 127) & ~static_cast<size_t>(127));
+    p.x_off = p.sums_off + static_cast<uint32_t>((sums + 127) & ~static_cast<size_t>(127));
+    p.smem = fixed + p.slots * per_slot;
+    *out = p;
+    return true;
+  }
+  return false;
+}
+
+template <int kM, int kShift>
+int launch_matvec(cudaStream_t stream, const CUtensorMap& map, const W4GroupArgs& a, const MatvecPlan& p) {
+  RK_CUDA(cudaFuncSetAttribute(w4_matvec_kernel<kM, kShift>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit)));
+  RK_CUDA(launch_pdl(w4_matvec_kernel<kM, kShift>, dim3(p.grid), dim3(kThreads), p.smem, stream, map, a, p, timeout_word_or_null()));
+  RK_LAUNCH_CHECK("linear_w4a16_group launch");
+  return kOk;
+}
+template <int kM>
+int launch_matvec(cudaStream_t stream, const CUtensorMap& map, const W4GroupArgs& a, const MatvecPlan& p) {
+  if (a.group == 32) return launch_matvec<kM, 5>(stream, map, a, p);
+  if (a.group == 64) return launch_matvec<kM, 6>(stream, map, a, p);
+  return launch_matvec<kM, 7>(stream, map, a, p);
+}
+
+int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
+  const TensorMapEncodeFn fn = tensor_map_encode_fn();
+  RK_REQUIRE(fn, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled is not available from this driver");
+  CUtensorMap map;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.K / 2), static_cast<cuuint64_t>(a.N)}, strides[1] = {static_cast<cuuint64_t>(a.K / 2)};
+  const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(p.h)}, elem[2] = {1, 1};
+  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled failed with %d (N=%d K=%d)", static_cast<int>(r), a.N, a.K);
+  switch (columns(a.M)) {
+    case 1: return launch_matvec<1>(stream, map, a, p);
+    case 2: return launch_matvec<2>(stream, map, a, p);
+    case 4: return launch_matvec<4>(stream, map, a, p);
+    default: return launch_matvec<8>(stream, map, a, p);
+  }
+}
+
+}  // namespace
+
 int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a) {
   const int s = check_shape("linear_w4a16_group", a.N, a.K, a.group);
   if (s != kOk) return s;
@@ -107,13 +432,20 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a) {
   RK_REQUIRE(a.epi == kEpiNone || a.epi == kEpiRelu2 || a.epi == kEpiF32, kBadArg, "linear_w4a16_group: unknown epilogue %d", a.epi);
   RK_REQUIRE(((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.q)) & 15u) == 0, kBadArg,
              "linear_w4a16_group: x and q must be 16-byte aligned");
-  for (int m0 = 0; m0 < a.M; m0 += 65535) {  // (the grid's second dimension)
+  int sms = 0, status = device_sms(&sms);
+  if (status != kOk) return status;
+  for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
-    b.M = min(a.M - m0, 65535);
+    MatvecPlan p;
+    b.M = std::min(a.M - m0, kMaxRows);
+    while (!plan_matvec(b, sms, &p)) {
+      RK_REQUIRE(b.M > 1, kShape, "linear_w4a16_group: K = %d is too long", a.K);
+      b.M = (b.M + 1) / 2;
+    }
     b.x = a.x + static_cast<size_t>(m0) * a.K;
     b.y = static_cast<char*>(a.y) + static_cast<size_t>(m0) * a.N * (a.epi == kEpiF32 ? 4 : 2);
-    w4_group_simple_kernel<<<dim3((a.N + 7) / 8, b.M), 256, 0, stream>>>(b);
-    RK_LAUNCH_CHECK("linear_w4a16_group launch");
+    if ((status = matvec(stream, b, p)) != kOk) return status;
+    m0 += b.M;
   }
   return kOk;
 }

@@ -265,7 +265,7 @@ def token_logprobs(logits, tokens=None, top_k=0):
         _tensor("token_logprobs: tokens", tokens, torch.int64, dev, (rows, n) if tokens.dim() == 2 else (rows,))
         logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
     _need(type(top_k) is int and 0 <= top_k <= 32, "token_logprobs: top_k outside [0, 32]")
-    entropy, lse = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
     if top_k:
         ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
         top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
@@ -310,7 +310,7 @@ def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128)
     need = C.c_size_t()
     L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(need)))
     work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    entropy, lse = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind(0)
+    entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
     _enqueue(dev, lib.rwkv7_b200_head_logprobs, rows, K, V, x.data_ptr(), weight.data_ptr(), fmt, _address(scale) if fmt else None,
              _address(zero) if fmt == L.FMT_W4A16 else None, group_size, _address(tokens), _address(logprobs), entropy.data_ptr(), lse.data_ptr(),
              work.data_ptr(), need.value)
