@@ -12,12 +12,14 @@
 //   - mma.sync m16n8k16 has eight columns.  With fewer rows of x the columns hold different 32-weight chunks (a
 //     lane whose column is another chunk's reads zeros), so that with one row eight chunks end up in eight columns and the
 //     scales are applied once for all of them.
-// One CTA of 16 warps per SM takes a contiguous range of output channels in tiles of up to 32; a tile's K extent is cut into
-// boxes of 128 bytes per row, box b going to warp b mod 16, fetched by one 2-D tensor copy into the warp's ring.  The warps'
-// partial sums of a tile are added in warp order: results do not depend on timing.
+// One CTA of 16 warps per SM takes a contiguous range of output channels in tiles of up to 32.  The warps form 1, 2 or 4
+// teams with a tile each; the tile's K extent is cut into boxes of 128 bytes per row, dealt out to the team's warps and
+// fetched by one 2-D tensor copy each into the warp's ring.  The warps' partial sums of a tile are added in warp order:
+// results do not depend on timing.
 #include <cuda.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -32,30 +34,42 @@ constexpr int kBoxWeights = 256;  // 128 bytes along a row: eight chunks of 32 w
 constexpr int kMaxRows = 8;
 constexpr size_t kSmemLimit = 226 * 1024;
 
+struct MatvecMaps {
+  CUtensorMap q, scale, zero;
+};
+
 struct MatvecPlan {
-  int h = 0, tiles = 0;         // rows of a tile and box, tiles per CTA
+  int teams = 0;                // of 16 / teams warps
+  int h = 0, tiles = 0;         // rows of a tile and box, tiles per team
   int boxes = 0;                // along a weight row
-  int slots = 0, slot_bytes = 0;
+  int slots = 0, slot_bytes = 0;  // a slot: the box, and behind it 16 bytes of scales and of zeros per row
+  bool copied = false;            // whether tensor copies can bring those
   int x_pitch = 0;              // bytes from one staged row of x to the next: 64 modulo 128, two rows share no bank
-  uint32_t part_off = 0, sums_off = 0, x_off = 0;  // from the aligned start of shared memory
+  uint32_t part_off = 0, sums_off = 0, x_off = 0, zero_off = 0;  // from the aligned start of shared memory
   size_t smem = 0;
   int grid = 0;
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool first) {
   if (first)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&w)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
 }
 __device__ __forceinline__ float half_of(uint32_t pair, int i) {
   const float2 f = h2f2(pair);
@@ -75,47 +89,56 @@ __device__ __forceinline__ void store_epi(const W4GroupArgs& a, size_t o, float 
 
 // kM: columns per chunk, the rows of x rounded up to 1, 2, 4 or 8; kShift: log2 of the group.  A box is worked off in passes of
 // kPass chunks, after each of which the sums are scaled; chunk c of a pass goes to the columns of slot c mod kSlots.
-template <int kM, int kShift>
-__global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_constant__ CUtensorMap map, const W4GroupArgs a, const MatvecPlan p, int* timeout) {
+// kBlk: blocks of 16 rows in a tile.  kCopied: scales and zeros come with their box, by tensor copies of the eight groups
+// (16 bytes) of each row that hold the box's; otherwise (rows of groups that are not multiples of 16 bytes) through registers.
+template <int kM, int kShift, int kBlk, bool kCopied>
+__global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_constant__ MatvecMaps maps, const W4GroupArgs a, const MatvecPlan p, int* timeout) {
   constexpr int kSlots = 8 / kM, kGroupChunks = 1 << (kShift - 5);
   constexpr int kPass = kSlots > kGroupChunks ? kSlots : kGroupChunks, kPasses = 8 / kPass;
   constexpr float kUnit = 1.0f / 16777216.0f;  // what a code of 1 stands for in the products
   extern __shared__ unsigned char smem_dyn[];
   __shared__ __align__(8) uint64_t bars[kWarps][4];
-  __shared__ uint4 zeros;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t dyn = smem_u32(smem_dyn), base = (dyn + 1023u) & ~1023u;
   unsigned char* const mem = smem_dyn + (base - dyn);
   const uint32_t ring = base + warp * p.slots * p.slot_bytes;
   float* const part = reinterpret_cast<float*>(mem + p.part_off);
   float* const sums = reinterpret_cast<float*>(mem + p.sums_off);
-  const int row0 = blockIdx.x * p.tiles * p.h, tiles = min(p.tiles, (a.N - row0 + p.h - 1) / p.h);
+  const int team_warps = kWarps / p.teams, team = warp / team_warps, team_warp = warp - team * team_warps;
+  // this team's tiles: team, team + teams, ... of the CTA's
+  const int cta_row0 = blockIdx.x * p.teams * p.tiles * p.h, all_tiles = min(p.teams * p.tiles, (a.N - cta_row0 + p.h - 1) / p.h);
+  const int row0 = cta_row0 + team * p.h, row_step = p.teams * p.h, tiles = all_tiles > team ? (all_tiles - team - 1) / p.teams + 1 : 0;
   const int groups = (a.K + (1 << kShift) - 1) >> kShift;
 
   if (lane == 0) {
     for (int i = 0; i < p.slots; ++i) mbar_init(smem_u32(&bars[warp][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (warp == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.q) : "memory");
   }
-  if (threadIdx.x == 0) zeros = make_uint4(0u, 0u, 0u, 0u);
+  if (threadIdx.x < 32) *reinterpret_cast<uint4*>(mem + p.zero_off + threadIdx.x * 16) = make_uint4(0u, 0u, 0u, 0u);  // what idle columns read, at the offsets of eight chunks
   __syncwarp();
   pdl_wait();
   pdl_trigger();
 
-  // this warp's boxes: warp, warp + 16, ... of the flattened (tile, box) sequence
+  // this warp's boxes: every team_warps-th of the team's flattened (tile, box) sequence
   auto advance = [&](int& tile, int& kb) {
-    kb += kWarps;
+    kb += team_warps;
     while (kb >= p.boxes && tile < tiles) { kb -= p.boxes; ++tile; }
   };
-  int q_tile = 0, q_kb = warp - kWarps, q_slot = 0;
+  int q_tile = 0, q_kb = team_warp - team_warps, q_slot = 0;
   advance(q_tile, q_kb);
   auto issue = [&]() {
     if (lane == 0) {
       const uint32_t bar = smem_u32(&bars[warp][q_slot]);
-      mbar_expect_tx(bar, p.h * 128);
-      asm volatile(
-          "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-          ::"r"(ring + q_slot * p.slot_bytes), "l"(&map), "r"(bar), "r"(q_kb << 7), "r"(row0 + q_tile * p.h)
-          : "memory");
+      const uint32_t dst = ring + q_slot * p.slot_bytes;
+      const int n = row0 + q_tile * row_step;
+      mbar_expect_tx(bar, p.h * (128 + (kCopied ? (a.zero ? 32 : 16) : 0)));
+      tma_2d(dst, &maps.q, bar, q_kb << 7, n);
+      if (kCopied) {
+        const int first = (q_kb << (8 - kShift)) & ~7;
+        tma_2d(dst + p.slot_bytes - 1024, &maps.scale, bar, first, n);
+        if (a.zero) tma_2d(dst + p.slot_bytes - 512, &maps.zero, bar, first, n);
+      }
     }
     if (++q_slot == p.slots) q_slot = 0;
     advance(q_tile, q_kb);
@@ -124,41 +147,45 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
 
   // A lane's share of a box's scales and zeros, for the rows g, g + 8, g + 16, g + 24: groups of 32: the pair 2t, 2t + 1 of the
   // box's eight; of 64: group t of four; of 128: group t / 2 of two.
-  uint32_t sc[4], ze[4];
+  uint32_t sc[2 * kBlk], ze[2 * kBlk], row_at[2 * kBlk];  // row_at: the row's first group (the host checks that 32 bits hold it)
+  int row_tile = -1;
   const bool paired = (groups & 1) == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 3) == 0;
+  const uint16_t *const scale = reinterpret_cast<const uint16_t*>(a.scale), *const zero = reinterpret_cast<const uint16_t*>(a.zero);
   auto fetch = [&](int tile, int kb) {
+    if (tile != row_tile) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const size_t r = static_cast<size_t>(min(row0 + tile * p.h + g + 8 * i, a.N - 1)) * groups;
+      for (int i = 0; i < 2 * kBlk; ++i) row_at[i] = static_cast<uint32_t>(min(row0 + tile * row_step + g + 8 * i, a.N - 1)) * groups;
+      row_tile = tile;
+    }
+    const int at = kShift == 5 ? kb * 8 + 2 * t : kShift == 6 ? kb * 4 + t : kb * 2 + (t >> 1);
+    const uint32_t o0 = min(at, groups - (kShift == 5 && paired ? 2 : 1)), o1 = min(at + 1, groups - 1);
+#pragma unroll
+    for (int i = 0; i < 2 * kBlk; ++i) {
       ze[i] = 0x48004800u;  // 8, 8
+      const uint16_t *s = scale + (row_at[i] + o0), *z = zero + (row_at[i] + o0);
       if (kShift == 5 && paired) {
-        const size_t o = r + min(kb * 8 + 2 * t, groups - 2);
-        sc[i] = *reinterpret_cast<const uint32_t*>(a.scale + o);
-        if (a.zero) ze[i] = *reinterpret_cast<const uint32_t*>(a.zero + o);
-      } else if (kShift == 5) {
-        const size_t o0 = r + min(kb * 8 + 2 * t, groups - 1), o1 = r + min(kb * 8 + 2 * t + 1, groups - 1);
-        const uint16_t *s = reinterpret_cast<const uint16_t*>(a.scale), *z = reinterpret_cast<const uint16_t*>(a.zero);
-        sc[i] = s[o0] | (static_cast<uint32_t>(s[o1]) << 16);
-        if (a.zero) ze[i] = z[o0] | (static_cast<uint32_t>(z[o1]) << 16);
+        sc[i] = *reinterpret_cast<const uint32_t*>(s);
+        if (zero) ze[i] = *reinterpret_cast<const uint32_t*>(z);
       } else {
-        const size_t o = r + min(kShift == 6 ? kb * 4 + t : kb * 2 + (t >> 1), groups - 1);
-        sc[i] = reinterpret_cast<const uint16_t*>(a.scale)[o];
-        if (a.zero) ze[i] = reinterpret_cast<const uint16_t*>(a.zero)[o];
+        sc[i] = *s;
+        if (zero) ze[i] = *z;
+        if (kShift == 5) {
+          sc[i] |= static_cast<uint32_t>(s[o1 - o0]) << 16;
+          if (zero) ze[i] |= static_cast<uint32_t>(z[o1 - o0]) << 16;
+        }
       }
     }
   };
-  int c_tile = 0, c_kb = warp - kWarps;
+  int c_tile = 0, c_kb = team_warp - team_warps;
   advance(c_tile, c_kb);
-  if (c_tile < tiles) fetch(c_tile, c_kb);
+  if (!kCopied && c_tile < tiles) fetch(c_tile, c_kb);
 
   // x as halves in the order of the fragments: a block of eight as x0 x4 x2 x6 | x1 x5 x3 x7 (the operands of the low and of the high
   // nibbles of a word); zeros behind K.  The sums of the chunks of 32 go to shared memory beside it.
   const int blocks = p.boxes * 32, chunks = p.boxes * 8;
   float* const chunk_sums = part;  // [M][chunks], until the first tile's partial sums
-  for (int i = threadIdx.x; i < a.M * blocks; i += kThreads) {
+  auto stage = [&](int i, uint4 q) {
     const int m = i / blocks, j = i - m * blocks;
-    uint4 q = make_uint4(0u, 0u, 0u, 0u);
-    if (j * 8 < a.K) q = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + j * 8);
     *reinterpret_cast<uint4*>(mem + p.x_off + m * p.x_pitch + j * 16) =
         make_uint4(__byte_perm(q.x, q.z, 0x5410), __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.x, q.z, 0x7632), __byte_perm(q.y, q.w, 0x7632));
     const float2 f0 = h2f2(q.x), f1 = h2f2(q.y), f2 = h2f2(q.z), f3 = h2f2(q.w);
@@ -166,6 +193,19 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // (a.M * blocks is a multiple of 32: whole warps take part)
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if ((j & 3) == 0) chunk_sums[m * chunks + (j >> 2)] = sum;
+  };
+  constexpr int kDeep = 4;  // loads under way at a time
+  for (int i0 = threadIdx.x; i0 < a.M * blocks; i0 += kDeep * kThreads) {
+    uint4 q[kDeep];
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d) {
+      const int i = i0 + d * kThreads, m = i / blocks, j = i - m * blocks;
+      q[d] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < a.M * blocks && j * 8 < a.K) q[d] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + j * 8);
+    }
+#pragma unroll
+    for (int d = 0; d < kDeep; ++d)
+      if (i0 + d * kThreads < a.M * blocks) stage(i0 + d * kThreads, q[d]);
   }
   __syncthreads();
   // -2^-24 times the sum of x that belongs to each column of each pass: [box][pass][8]
@@ -180,21 +220,21 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
 
   const uint32_t w_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);  // see ldmatrix below
   const int slot_of_lane = g / kM;
-  const uint32_t x_lane = base + p.x_off + min(g % kM, a.M - 1) * p.x_pitch + (t << 4), zero_addr = smem_u32(&zeros);
-  float acc[2][4];
+  const uint32_t x_row = base + p.x_off + min(g % kM, a.M - 1) * p.x_pitch + (t << 4), zero_now = base + p.zero_off;
+  float acc[kBlk][4];
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int b = 0; b < kBlk; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
   int cur = 0, slot = 0, phase = 0;
   bool dead = false;  // a wait ran out: no more work, but the barriers are kept
-  const bool two = p.h > 16;
   for (;;) {
-    // Tile boundaries: every warp leaves its sums, and one barrier later all threads add up the tile.
+    // Tile boundaries: every warp of the team leaves its sums, and one barrier later its threads add up the tile.
     for (const int upto = min(c_tile, tiles); cur < upto; ++cur) {
-      float* const mine = part + (cur & 1) * kWarps * kTileRows * kM + warp * kTileRows * kM;
+      float* const sums_of = part + ((cur & 1) * kWarps + team * team_warps) * kTileRows * kM;
+      float* const mine = sums_of + team_warp * kTileRows * kM;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
+      for (int b = 0; b < kBlk; ++b) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = acc[b][i];  // row 16 b + g + 8 (i / 2), column 2 t + i % 2
@@ -207,27 +247,29 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
           if (kM <= 2) v += __shfl_xor_sync(0xffffffffu, v, 1);
           if (kM <= 4) v += __shfl_xor_sync(0xffffffffu, v, 2);
           const int m = kM == 1 ? 0 : (2 * t + (i & 1)) % kM;
-          if (2 * t < kM || (kM == 1 && t == 0)) mine[(16 * b + g + 8 * (i >> 1)) * kM + m] = v;
+          if (2 * t < kM) mine[(16 * b + g + 8 * (i >> 1)) * kM + m] = v;
         }
       }
-      __syncthreads();
-      const int r = threadIdx.x % kTileRows, m = threadIdx.x / kTileRows, n = row0 + cur * p.h + r;
-      if (r < p.h && m < a.M && n < a.N) {
-        const float* src = part + (cur & 1) * kWarps * kTileRows * kM + r * kM + m;
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(team_warps * 32) : "memory");
+      for (int i = team_warp * 32 + lane; i < kTileRows * kM; i += team_warps * 32) {
+        const int r = i % kTileRows, m = i / kTileRows, n = row0 + cur * row_step + r;
+        if (r >= p.h || m >= a.M || n >= a.N) continue;
         float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += src[w * kTileRows * kM];
+#pragma unroll 4
+        for (int w = 0; w < team_warps; ++w) v += sums_of[w * kTileRows * kM + r * kM + m];
         store_epi(a, static_cast<size_t>(m) * a.N + n, v * 16777216.0f);
       }
     }
     if (c_tile >= tiles) break;
 
     const int kb = c_kb;
-    uint32_t s_now[4], z_now[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { s_now[i] = sc[i]; z_now[i] = ze[i]; }
+    uint32_t s_now[2 * kBlk], z_now[2 * kBlk];
     advance(c_tile, c_kb);
-    if (c_tile < tiles) fetch(c_tile, c_kb);
+    if (!kCopied) {
+#pragma unroll
+      for (int i = 0; i < 2 * kBlk; ++i) { s_now[i] = sc[i]; z_now[i] = ze[i]; }
+      if (c_tile < tiles) fetch(c_tile, c_kb);
+    }
     const uint32_t bar = smem_u32(&bars[warp][slot]);
     if (!dead && !mbar_try_wait(bar, phase) && !mbar_wait(bar, phase)) {
       dead = true;
@@ -235,25 +277,34 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
     }
     if (!dead) {
       const uint32_t wbase = ring + slot * p.slot_bytes;
-      float lo[2][4], hi[2][4];
+      if (kCopied) {
+        const int at = (kb << (8 - kShift)) & 7;  // the box's first group among the eight
+        const unsigned char* params = mem + (wbase - base) + p.slot_bytes - 1024 + g * 16 + 2 * (at + (kShift == 5 ? 2 * t : kShift == 6 ? t : t >> 1));
+#pragma unroll
+        for (int i = 0; i < 2 * kBlk; ++i) {
+          s_now[i] = kShift == 5 ? *reinterpret_cast<const uint32_t*>(params + 128 * i) : *reinterpret_cast<const uint16_t*>(params + 128 * i);
+          z_now[i] = 0x48004800u;
+          if (a.zero) z_now[i] = kShift == 5 ? *reinterpret_cast<const uint32_t*>(params + 512 + 128 * i) : *reinterpret_cast<const uint16_t*>(params + 512 + 128 * i);
+        }
+      }
+      const uint32_t x_now = x_row + (kb << 9);
+      float lo[kBlk][4], hi[kBlk][4];
 #pragma unroll
       for (int c2 = 0; c2 < 4; ++c2) {
         // Two chunks of 16 rows: the matrices are (rows 0-7, rows 8-15) x (chunk 2 c2, chunk 2 c2 + 1), 16 bytes a row, and a lane gets
         // the word t of row g.  The 128-byte swizzle puts chunk c of row r at c ^ (r mod 8).
-        uint32_t w[2][4];
-        ldmatrix4(w[0], wbase + (w_lane ^ (c2 << 5)));
-        if (two) ldmatrix4(w[1], wbase + 2048 + (w_lane ^ (c2 << 5)));
+        uint32_t w[kBlk][4];
+#pragma unroll
+        for (int b = 0; b < kBlk; ++b) ldmatrix4(w[b], wbase + b * 2048 + (w_lane ^ (c2 << 5)));
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
           const int c = 2 * c2 + cc;
-          const uint32_t xa = x_lane + (kb << 9) + (c << 6);
           uint4 xv;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
-                       : "r"(kSlots == 1 || slot_of_lane == c % kSlots ? xa : zero_addr));
+                       : "r"((kSlots == 1 || slot_of_lane == c % kSlots ? x_now : zero_now) + (c << 6)));
           const bool first = c % kPass == 0;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && !two) break;
+          for (int b = 0; b < kBlk; ++b) {
             const uint32_t wa = w[b][2 * cc], wb = w[b][2 * cc + 1], va = wa >> 8, vb = wb >> 8;
             mma16816(lo[b], wa & 0x000f000fu, wb & 0x000f000fu, va & 0x000f000fu, vb & 0x000f000fu, xv.x, xv.y, first);
             mma16816(hi[b], wa & 0x00f000f0u, wb & 0x00f000f0u, va & 0x00f000f0u, vb & 0x00f000f0u, xv.z, xv.w, first);
@@ -266,8 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
           const int chunk = kM == 1 ? 2 * t : pass * kPass + (kM == 8 ? 0 : 2 * t / kM);
           const int from = kShift == 5 ? chunk >> 1 : kShift == 6 ? chunk >> 1 : (chunk >> 2) << 1;
 #pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            if (b == 1 && !two) break;
+          for (int b = 0; b < kBlk; ++b) {
             float s0[2], s1[2], z0[2], z1[2];  // rows g and g + 8: of the lane's first and second column
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -364,27 +414,39 @@ namespace {
 
 int columns(int M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
 
-// One tile height for all CTAs, so that a box is exactly a CTA's rows: N / SMs rows each, in equal tiles of at most 32.
+// One tile height for all CTAs, so that a box is exactly what its team works on: N / SMs rows per CTA in equal tiles of at most
+// 32.  Larger teams share a tile's K extent among more warps, smaller ones pay the end of a tile (sums through shared memory, a
+// barrier) less often per box: as many teams as keep the number of 16-row blocks within 15 % of the least.
 bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
   const int kM = columns(a.M), group_chunks = a.group / 32, pass = std::max(8 / kM, group_chunks), passes = 8 / pass;
+  const int target = (a.N + sms - 1) / sms, groups = (a.K + a.group - 1) / a.group;
+  const bool copied = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
   for (const int most : {kTileRows, 16}) {  // tiles of 16 where those of 32 leave no room for two boxes per warp
     MatvecPlan p;
-    const int target = (a.N + sms - 1) / sms;
-    p.tiles = (target + most - 1) / most;
-    p.h = (target + p.tiles - 1) / p.tiles;
-    p.grid = (a.N + p.tiles * p.h - 1) / (p.tiles * p.h);
+    auto tile = [&](int teams) {
+      p.teams = teams;
+      p.tiles = (target + most * teams - 1) / (most * teams);
+      p.h = (target + p.tiles * teams - 1) / (p.tiles * teams);
+      return p.tiles * teams * ((p.h + 15) / 16);
+    };
+    const int least = std::min(tile(1), std::min(tile(2), tile(4)));
+    if (tile(4) * 100 > least * 115 && tile(2) * 100 > least * 115) tile(1);
+    if (getenv("RK_TEAMS")) tile(atoi(getenv("RK_TEAMS")));
+    p.grid = (a.N + p.teams * p.tiles * p.h - 1) / (p.teams * p.tiles * p.h);
     p.boxes = (a.K + kBoxWeights - 1) / kBoxWeights;
-    p.slot_bytes = (p.h * 128 + 1023) & ~1023;
+    p.copied = copied;
+    p.slot_bytes = ((p.h * 128 + 1023) & ~1023) + (copied ? 1024 : 0);
     p.x_pitch = p.boxes * kBoxWeights * 2 + 64;
     const size_t part = std::max<size_t>(2u * kWarps * kTileRows * kM * sizeof(float), static_cast<size_t>(a.M) * p.boxes * 8 * sizeof(float));
     const size_t sums = static_cast<size_t>(p.boxes) * passes * 8 * sizeof(float), x = static_cast<size_t>(a.M) * p.x_pitch;
-    const size_t fixed = 1024 + ((part + 127) & ~static_cast<size_t>(127)) + ((sums + 127) & ~static_cast<size_t>(127)) + x;
+    const size_t fixed = 1024 + 512 + ((part + 127) & ~static_cast<size_t>(127)) + ((sums + 127) & ~static_cast<size_t>(127)) + x;
     const size_t per_slot = static_cast<size_t>(kWarps) * p.slot_bytes;
     if (fixed + 2 * per_slot > kSmemLimit) continue;
     p.slots = static_cast<int>(std::min<size_t>(4, (kSmemLimit - fixed) / per_slot));
     p.part_off = static_cast<uint32_t>(p.slots * per_slot);
     p.sums_off = p.part_off + static_cast<uint32_t>((part + 127) & ~static_cast<size_t>(127));
-    p.x_off = p.sums_off + static_cast<uint32_t>((sums + 127) & ~static_cast<size_t>(127));
+    p.zero_off = p.sums_off + static_cast<uint32_t>((sums + 127) & ~static_cast<size_t>(127));
+    p.x_off = p.zero_off + 512;
     p.smem = fixed + p.slots * per_slot;
     *out = p;
     return true;
@@ -392,34 +454,53 @@ bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
   return false;
 }
 
-template <int kM, int kShift>
-int launch_matvec(cudaStream_t stream, const CUtensorMap& map, const W4GroupArgs& a, const MatvecPlan& p) {
-  RK_CUDA(cudaFuncSetAttribute(w4_matvec_kernel<kM, kShift>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit)));
-  RK_CUDA(launch_pdl(w4_matvec_kernel<kM, kShift>, dim3(p.grid), dim3(kThreads), p.smem, stream, map, a, p, timeout_word_or_null()));
+template <int kM, int kShift, int kBlk, bool kCopied>
+int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
+  const auto kernel = w4_matvec_kernel<kM, kShift, kBlk, kCopied>;
+  RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit)));
+  RK_CUDA(launch_pdl(kernel, dim3(p.grid), dim3(kThreads), p.smem, stream, maps, a, p, timeout_word_or_null()));
   RK_LAUNCH_CHECK("linear_w4a16_group launch");
   return kOk;
 }
+template <int kM, int kShift>
+int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
+  if (p.copied) return p.h > 16 ? launch_matvec<kM, kShift, 2, true>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, true>(stream, maps, a, p);
+  return p.h > 16 ? launch_matvec<kM, kShift, 2, false>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, false>(stream, maps, a, p);
+}
 template <int kM>
-int launch_matvec(cudaStream_t stream, const CUtensorMap& map, const W4GroupArgs& a, const MatvecPlan& p) {
-  if (a.group == 32) return launch_matvec<kM, 5>(stream, map, a, p);
-  if (a.group == 64) return launch_matvec<kM, 6>(stream, map, a, p);
-  return launch_matvec<kM, 7>(stream, map, a, p);
+int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
+  if (a.group == 32) return launch_matvec<kM, 5>(stream, maps, a, p);
+  if (a.group == 64) return launch_matvec<kM, 6>(stream, maps, a, p);
+  return launch_matvec<kM, 7>(stream, maps, a, p);
+}
+
+int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t row_bytes, int elem_bytes, int rows, int box_cols, int box_rows,
+           CUtensorMapSwizzle swizzle) {
+  const TensorMapEncodeFn fn = tensor_map_encode_fn();
+  RK_REQUIRE(fn, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint64_t dims[2] = {row_bytes / elem_bytes, static_cast<cuuint64_t>(rows)}, strides[1] = {row_bytes};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
+  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled failed with %d (rows=%d, %zu bytes each)", static_cast<int>(r), rows, row_bytes);
+  return kOk;
 }
 
 int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
-  const TensorMapEncodeFn fn = tensor_map_encode_fn();
-  RK_REQUIRE(fn, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled is not available from this driver");
-  CUtensorMap map;
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.K / 2), static_cast<cuuint64_t>(a.N)}, strides[1] = {static_cast<cuuint64_t>(a.K / 2)};
-  const cuuint32_t box[2] = {128u, static_cast<cuuint32_t>(p.h)}, elem[2] = {1, 1};
-  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.q), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled failed with %d (N=%d K=%d)", static_cast<int>(r), a.N, a.K);
+  MatvecMaps maps;
+  int s = encode(&maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, a.K / 2, 1, a.N, 128, p.h, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (s != kOk) return s;
+  maps.scale = maps.zero = maps.q;
+  if (p.copied) {
+    const size_t row_bytes = (a.K + a.group - 1) / a.group * sizeof(half);
+    if ((s = encode(&maps.scale, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.scale, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
+    if (a.zero && (s = encode(&maps.zero, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.zero, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
+  }
   switch (columns(a.M)) {
-    case 1: return launch_matvec<1>(stream, map, a, p);
-    case 2: return launch_matvec<2>(stream, map, a, p);
-    case 4: return launch_matvec<4>(stream, map, a, p);
-    default: return launch_matvec<8>(stream, map, a, p);
+    case 1: return launch_matvec<1>(stream, maps, a, p);
+    case 2: return launch_matvec<2>(stream, maps, a, p);
+    case 4: return launch_matvec<4>(stream, maps, a, p);
+    default: return launch_matvec<8>(stream, maps, a, p);
   }
 }
 
@@ -432,6 +513,7 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a) {
   RK_REQUIRE(a.epi == kEpiNone || a.epi == kEpiRelu2 || a.epi == kEpiF32, kBadArg, "linear_w4a16_group: unknown epilogue %d", a.epi);
   RK_REQUIRE(((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.q)) & 15u) == 0, kBadArg,
              "linear_w4a16_group: x and q must be 16-byte aligned");
+  RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
   for (int m0 = 0; m0 < a.M;) {
