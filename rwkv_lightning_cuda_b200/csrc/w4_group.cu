@@ -184,28 +184,39 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
   // nibbles of a word); zeros behind K.  The sums of the chunks of 32 go to shared memory beside it.
   const int blocks = p.boxes * 32, chunks = p.boxes * 8;
   float* const chunk_sums = part;  // [M][chunks], until the first tile's partial sums
-  auto stage = [&](int i, uint4 q) {
-    const int m = i / blocks, j = i - m * blocks;
+  auto stage = [&](int m, int j, uint4 q) {
     *reinterpret_cast<uint4*>(mem + p.x_off + m * p.x_pitch + j * 16) =
         make_uint4(__byte_perm(q.x, q.z, 0x5410), __byte_perm(q.y, q.w, 0x5410), __byte_perm(q.x, q.z, 0x7632), __byte_perm(q.y, q.w, 0x7632));
     const float2 f0 = h2f2(q.x), f1 = h2f2(q.y), f2 = h2f2(q.z), f3 = h2f2(q.w);
     float sum = ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // (a.M * blocks is a multiple of 32: whole warps take part)
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);  // (blocks is a multiple of 32: whole warps take part)
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     if ((j & 3) == 0) chunk_sums[m * chunks + (j >> 2)] = sum;
   };
-  constexpr int kDeep = 4;  // loads under way at a time
-  for (int i0 = threadIdx.x; i0 < a.M * blocks; i0 += kDeep * kThreads) {
+  auto walk = [&](int& m, int& j) {  // to the block kThreads further on
+    j += kThreads;
+    while (j >= blocks) { j -= blocks; ++m; }
+  };
+  constexpr int kDeep = 8;  // loads under way at a time
+  int m_ld = 0, j_ld = static_cast<int>(threadIdx.x) - kThreads, m_st = 0, j_st = static_cast<int>(threadIdx.x) - kThreads;
+  walk(m_ld, j_ld);
+  walk(m_st, j_st);
+  while (m_st < a.M) {
     uint4 q[kDeep];
 #pragma unroll
     for (int d = 0; d < kDeep; ++d) {
-      const int i = i0 + d * kThreads, m = i / blocks, j = i - m * blocks;
       q[d] = make_uint4(0u, 0u, 0u, 0u);
-      if (i < a.M * blocks && j * 8 < a.K) q[d] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m) * a.K + j * 8);
+      if (m_ld < a.M) {
+        if (j_ld * 8 < a.K) q[d] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(m_ld) * a.K + j_ld * 8);
+        walk(m_ld, j_ld);
+      }
     }
 #pragma unroll
     for (int d = 0; d < kDeep; ++d)
-      if (i0 + d * kThreads < a.M * blocks) stage(i0 + d * kThreads, q[d]);
+      if (m_st < a.M) {
+        stage(m_st, j_st, q[d]);
+        walk(m_st, j_st);
+      }
   }
   __syncthreads();
   // -2^-24 times the sum of x that belongs to each column of each pass: [box][pass][8]

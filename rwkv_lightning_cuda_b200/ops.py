@@ -226,6 +226,11 @@ def _tensor(name, t, dtypes, device, shape=None, contiguous=True):
         _need(False, f"{name}: must be contiguous")
 
 
+# The functions below run in ten microseconds or less, so a call tests everything in one expression and looks for the argument to
+# name in the error only when that fails.
+_F16, _F32 = torch.float16, torch.float32
+
+
 def _enqueue(dev, call, *args):
     """One library call on the current stream of ``dev``, which need not be the current device; the tensors' addresses are passed as
     integers (None: NULL), the checks have been made."""
@@ -239,8 +244,21 @@ def _enqueue(dev, call, *args):
         L.check(status)
 
 
-def _address(t):
-    return None if t is None else t.data_ptr()
+def _good(t, dtype, dev, shape):
+    return t.dtype == dtype and t.device == dev and t.shape == shape and t.is_contiguous()
+
+
+def _refuse_token_logprobs(logits, tokens, top_k):
+    _need(isinstance(logits, torch.Tensor) and logits.dim() == 2, "token_logprobs: logits [rows, V] expected", 2)
+    _tensor("token_logprobs: logits", logits, (_F32, _F16), None, contiguous=False)
+    rows, V = logits.shape
+    _need(rows > 0 and V > 0, "token_logprobs: logits must not be empty")
+    _need((logits.stride(1) == 1 or V == 1) and (rows == 1 or logits.stride(0) >= V),
+          "token_logprobs: a row's logits must be contiguous, rows must not overlap")
+    if tokens is not None:
+        _need(isinstance(tokens, torch.Tensor) and tokens.dim() in (1, 2), "token_logprobs: tokens [rows] or [rows, n] expected", 2)
+        _tensor("token_logprobs: tokens", tokens, torch.int64, logits.device, (rows, tokens.shape[1]) if tokens.dim() == 2 else (rows,))
+    _need(False, "token_logprobs: top_k outside [0, 32]")
 
 
 def token_logprobs(logits, tokens=None, top_k=0):
@@ -249,88 +267,119 @@ def token_logprobs(logits, tokens=None, top_k=0):
     (at most 32) likeliest tokens, likeliest first, equal ones by index.  Returns (logprobs, entropy, lse, top_ids,
     top_logprobs): fp32 shaped like ``tokens``, fp32 [rows], fp32 [rows], int32 and fp32 [rows, top_k]; None for what was not
     asked.  -inf masks a token; a row with a NaN or +inf answers NaN."""
-    _need(isinstance(logits, torch.Tensor) and logits.dim() == 2, "token_logprobs: logits [rows, V] expected", 2)
-    _tensor("token_logprobs: logits", logits, (torch.float32, torch.float16), None, contiguous=False)
-    rows, V = logits.shape
-    _need(rows > 0 and V > 0, "token_logprobs: logits must not be empty")
-    ld, along = logits.stride()
-    if rows == 1:
-        ld = V
-    _need((along == 1 or V == 1) and ld >= V, "token_logprobs: a row's logits must be contiguous, rows must not overlap")
-    dev = logits.device
-    n, logprobs, ids, top = 0, None, None, None
+    ok = isinstance(logits, torch.Tensor) and logits.dim() == 2 and logits.is_cuda and (logits.dtype == _F32 or logits.dtype == _F16)
+    n, logprobs, ids, top, asked = 0, None, None, None, None
+    if ok:
+        (rows, V), (ld, along), dev = logits.shape, logits.stride(), logits.device
+        if rows == 1:
+            ld = V
+        ok = rows > 0 and V > 0 and (along == 1 or V == 1) and ld >= V and type(top_k) is int and 0 <= top_k <= 32
+        if ok and tokens is not None:
+            ok = isinstance(tokens, torch.Tensor) and tokens.dim() in (1, 2) and _good(tokens, torch.int64, dev, (rows, *tokens.shape[1:]))
+    if not ok:
+        _refuse_token_logprobs(logits, tokens, top_k)
     if tokens is not None:
-        _need(isinstance(tokens, torch.Tensor) and tokens.dim() in (1, 2), "token_logprobs: tokens [rows] or [rows, n] expected", 2)
-        n = tokens.shape[1] if tokens.dim() == 2 else 1
-        _tensor("token_logprobs: tokens", tokens, torch.int64, dev, (rows, n) if tokens.dim() == 2 else (rows,))
-        logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    _need(type(top_k) is int and 0 <= top_k <= 32, "token_logprobs: top_k outside [0, 32]")
-    entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
+        n, asked = tokens.numel() // rows, tokens.data_ptr()
+        logprobs = torch.empty_like(tokens, dtype=_F32)
+    entropy, lse = torch.empty(rows, dtype=_F32, device=dev), torch.empty(rows, dtype=_F32, device=dev)
     if top_k:
-        ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-        top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    _enqueue(dev, L.load_library().rwkv7_b200_token_logprobs, rows, V, logits.data_ptr(),
-             L.DT_F16 if logits.dtype == torch.float16 else L.DT_F32, ld, _address(tokens), n, top_k, _address(logprobs), entropy.data_ptr(),
-             lse.data_ptr(), _address(ids), _address(top))
+        ids, top = torch.empty(rows, top_k, dtype=torch.int32, device=dev), torch.empty(rows, top_k, dtype=_F32, device=dev)
+    _enqueue(dev, L.load_library().rwkv7_b200_token_logprobs, rows, V, logits.data_ptr(), L.DT_F16 if logits.dtype == _F16 else L.DT_F32, ld,
+             asked, n, top_k, logprobs.data_ptr() if asked else None, entropy.data_ptr(), lse.data_ptr(), ids.data_ptr() if top_k else None,
+             top.data_ptr() if top_k else None)
     return logprobs, entropy, lse, ids, top
 
 
 def _w4_group_params(what, scale, zero, rows, K, group, dev):
     _need(group in (32, 64, 128), f"{what}: groups of 32, 64 or 128", 2)
     groups = -(-K // group)
-    _tensor(f"{what}: scale", scale, torch.float16, dev, (rows, groups))
+    _tensor(f"{what}: scale", scale, _F16, dev, (rows, groups))
     if zero is not None:
-        _tensor(f"{what}: zero", zero, torch.float16, dev, (rows, groups))
+        _tensor(f"{what}: zero", zero, _F16, dev, (rows, groups))
+
+
+def _good_w4_group(scale, zero, rows, K, group, dev):
+    if group not in (32, 64, 128) or not isinstance(scale, torch.Tensor):
+        return False
+    shape = (rows, -(-K // group))
+    return _good(scale, _F16, dev, shape) and (zero is None or (isinstance(zero, torch.Tensor) and _good(zero, _F16, dev, shape)))
 
 
 _HEAD_FORMATS = {torch.float16: L.FMT_F16, torch.int8: L.FMT_W8A16, torch.uint8: L.FMT_W4A16}
+_head_workspaces = {}  # bytes of scratch by (rows, V)
+
+
+def _refuse_head_logprobs(x, weight, tokens, scale, zero, group_size):
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "head_logprobs: x [rows, K] expected", 2)
+    _tensor("head_logprobs: x", x, _F16, None)
+    rows, K = x.shape
+    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] > 0, "head_logprobs: weight [V, K] expected", 2)
+    V, fmt = weight.shape[0], _HEAD_FORMATS.get(weight.dtype, -1)
+    _tensor("head_logprobs: weight", weight, tuple(_HEAD_FORMATS), x.device, (V, K // 2 if fmt == L.FMT_W4A16 else K))
+    if fmt == L.FMT_W8A16:
+        _tensor("head_logprobs: scale", scale, _F16, x.device, (V,))
+    elif fmt == L.FMT_W4A16:
+        _w4_group_params("head_logprobs", scale, zero, V, K, group_size, x.device)
+    _tensor("head_logprobs: tokens", tokens, torch.int64, x.device, (rows,))
+    _need(False, "head_logprobs: bad argument")
 
 
 def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128):
     """``token_logprobs`` of x W^T (x fp16 [rows, K]) without writing the logits: one given token per row (int64 [rows] or
     None).  ``weight`` is fp16 [V, K], int8 [V, K] with ``scale`` fp16 [V], or uint8 [V, K/2] (two 4-bit codes a byte) with
     ``scale`` and ``zero`` (None: 8) fp16 [V, ceil(K / group_size)].  Returns (logprobs, entropy, lse), fp32 [rows]."""
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "head_logprobs: x [rows, K] expected", 2)
-    _tensor("head_logprobs: x", x, torch.float16, None)
-    rows, K = x.shape
-    dev = x.device
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == 2 and weight.shape[0] > 0, "head_logprobs: weight [V, K] expected", 2)
-    V = weight.shape[0]
-    fmt = _HEAD_FORMATS.get(weight.dtype, -1)
-    _tensor("head_logprobs: weight", weight, (torch.float16, torch.int8, torch.uint8), dev, (V, K // 2 if fmt == L.FMT_W4A16 else K))
-    if fmt == L.FMT_W8A16:
-        _tensor("head_logprobs: scale", scale, torch.float16, dev, (V,))
-    elif fmt == L.FMT_W4A16:
-        _w4_group_params("head_logprobs", scale, zero, V, K, group_size, dev)
-    logprobs = None
-    if tokens is not None:
-        _tensor("head_logprobs: tokens", tokens, torch.int64, dev, (rows,))
-        logprobs = torch.empty(rows, dtype=torch.float32, device=dev)
+    ok = isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.dim() == 2 and weight.dim() == 2 and x.is_cuda
+    if ok:
+        (rows, K), V, dev, fmt = x.shape, weight.shape[0], x.device, _HEAD_FORMATS.get(weight.dtype, -1)
+        ok = (rows > 0 and V > 0 and fmt >= 0 and x.dtype == _F16 and x.is_contiguous()
+              and _good(weight, weight.dtype, dev, (V, K // 2 if fmt == L.FMT_W4A16 else K))
+              and (tokens is None or (isinstance(tokens, torch.Tensor) and _good(tokens, torch.int64, dev, (rows,)))))
+        if ok and fmt == L.FMT_W8A16:
+            ok = isinstance(scale, torch.Tensor) and _good(scale, _F16, dev, (V,))
+        elif ok and fmt == L.FMT_W4A16:
+            ok = _good_w4_group(scale, zero, V, K, group_size, dev)
+    if not ok:
+        _refuse_head_logprobs(x, weight, tokens, scale, zero, group_size)
     lib = L.load_library()
-    need = C.c_size_t()
-    L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(need)))
-    work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    entropy, lse = torch.empty(rows, dtype=torch.float32, device=dev), torch.empty(rows, dtype=torch.float32, device=dev)
-    _enqueue(dev, lib.rwkv7_b200_head_logprobs, rows, K, V, x.data_ptr(), weight.data_ptr(), fmt, _address(scale) if fmt else None,
-             _address(zero) if fmt == L.FMT_W4A16 else None, group_size, _address(tokens), _address(logprobs), entropy.data_ptr(), lse.data_ptr(),
-             work.data_ptr(), need.value)
+    need = _head_workspaces.get((rows, V))
+    if need is None:
+        size = C.c_size_t()
+        L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(size)))
+        need = size.value
+        if len(_head_workspaces) < 4096:
+            _head_workspaces[rows, V] = need
+    work = torch.empty(need, dtype=torch.uint8, device=dev)
+    logprobs = torch.empty(rows, dtype=_F32, device=dev) if tokens is not None else None
+    entropy, lse = torch.empty(rows, dtype=_F32, device=dev), torch.empty(rows, dtype=_F32, device=dev)
+    _enqueue(dev, lib.rwkv7_b200_head_logprobs, rows, K, V, x.data_ptr(), weight.data_ptr(), fmt, scale.data_ptr() if fmt else None,
+             zero.data_ptr() if fmt == L.FMT_W4A16 and zero is not None else None, group_size, tokens.data_ptr() if tokens is not None else None,
+             logprobs.data_ptr() if tokens is not None else None, entropy.data_ptr(), lse.data_ptr(), work.data_ptr(), need)
     return logprobs, entropy, lse
+
+
+def _refuse_linear_w4a16_group(x, q, scale, zero, group_size):
+    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "linear_w4a16_group: x [M, K] expected", 2)
+    _tensor("linear_w4a16_group: x", x, _F16, None)
+    _need(isinstance(q, torch.Tensor) and q.dim() == 2 and q.shape[0] > 0, "linear_w4a16_group: q [N, K/2] expected", 2)
+    K, N = x.shape[1], q.shape[0]
+    _tensor("linear_w4a16_group: q", q, torch.uint8, x.device, (N, K // 2))
+    _w4_group_params("linear_w4a16_group", scale, zero, N, K, group_size, x.device)
+    _need(False, "linear_w4a16_group: bad argument")
 
 
 def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NONE):
     """x W^T for 4-bit weights with group scales: W = (q - zero) * scale per group of 32, 64 or 128 inputs; x fp16 [M, K], q
     uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N."""
-    _need(isinstance(x, torch.Tensor) and x.dim() == 2 and x.shape[0] > 0, "linear_w4a16_group: x [M, K] expected", 2)
-    _tensor("linear_w4a16_group: x", x, torch.float16, None)
-    M, K = x.shape
-    dev = x.device
-    _need(isinstance(q, torch.Tensor) and q.dim() == 2 and q.shape[0] > 0, "linear_w4a16_group: q [N, K/2] expected", 2)
-    N = q.shape[0]
-    _tensor("linear_w4a16_group: q", q, torch.uint8, dev, (N, K // 2))
-    _w4_group_params("linear_w4a16_group", scale, zero, N, K, group_size, dev)
-    y = torch.empty((M, N), dtype=torch.float32 if epilogue == L.EPI_F32 else torch.float16, device=dev)
-    _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(), _address(zero), group_size,
-             epilogue, y.data_ptr())
+    ok = isinstance(x, torch.Tensor) and isinstance(q, torch.Tensor) and x.dim() == 2 and q.dim() == 2 and x.is_cuda
+    if ok:
+        (M, K), N, dev = x.shape, q.shape[0], x.device
+        ok = (M > 0 and N > 0 and x.dtype == _F16 and x.is_contiguous() and _good(q, torch.uint8, dev, (N, K // 2))
+              and _good_w4_group(scale, zero, N, K, group_size, dev))
+    if not ok:
+        _refuse_linear_w4a16_group(x, q, scale, zero, group_size)
+    y = torch.empty(M, N, dtype=_F32 if epilogue == L.EPI_F32 else _F16, device=dev)
+    _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(),
+             None if zero is None else zero.data_ptr(), group_size, epilogue, y.data_ptr())
     return y
 
 
