@@ -360,10 +360,15 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
   return linear_common(stream, M, K, N, x, q, RWKV7_B200_FMT_W4A16, scale, zero, 0, epilogue, y);
 }
 int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q, const uint16_t* scale,
-                                  const uint16_t* zero, int group, int epilogue, void* y) {
+                                  const uint16_t* zero, int group, int epilogue, void* y, void* workspace, size_t workspace_bytes) {
   rk::W4GroupArgs a;
   a.M = M; a.K = K; a.N = N; a.group = group; a.x = h(x); a.q = q; a.scale = h(scale); a.zero = h(zero); a.epi = epilogue; a.y = y;
-  return rk::w4_group_linear(st(stream), a);
+  return rk::w4_group_linear(st(stream), a, workspace, workspace_bytes);
+}
+int rwkv7_b200_linear_w4a16_group_workspace(int M, int K, int N, size_t* bytes) {
+  RK_REQUIRE(M > 0 && K > 0 && N > 0 && bytes, kBadArg, "linear_w4a16_group_workspace: bad argument");
+  *bytes = rk::w4_group_workspace(M, K, N);
+  return kOk;
 }
 int rwkv7_b200_quant_pack_w4_group(void* stream, int N, int K, int group, const uint16_t* W, uint8_t* q, uint16_t* scale,
                                    uint16_t* zero) {

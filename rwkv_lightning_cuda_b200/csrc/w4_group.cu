@@ -517,16 +517,33 @@ int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
 
 }  // namespace
 
-int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a) {
+// Planes of fp32 partial sums that let the tensor-core kernel deal its 128-channel tiles out twice over to the SMs.
+size_t w4_group_workspace(int M, int K, int N) {
+  if (M <= kMaxRows || N % 4 != 0) return 0;
+  const long long tiles = static_cast<long long>((N + 127) / 128) * ((M + 255) / 256);
+  const long long planes = std::min<long long>({16, (296 + tiles - 1) / tiles, (K + 255) / 256});
+  return planes < 2 ? 0 : static_cast<size_t>(planes) * M * N * sizeof(float);
+}
+
+int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, size_t workspace_bytes) {
   const int s = check_shape("linear_w4a16_group", a.N, a.K, a.group);
   if (s != kOk) return s;
   RK_REQUIRE(a.M > 0 && a.x && a.q && a.scale && a.y, kBadArg, "linear_w4a16_group: bad argument");
   RK_REQUIRE(a.epi == kEpiNone || a.epi == kEpiRelu2 || a.epi == kEpiF32, kBadArg, "linear_w4a16_group: unknown epilogue %d", a.epi);
-  RK_REQUIRE(((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.q)) & 15u) == 0, kBadArg,
-             "linear_w4a16_group: x and q must be 16-byte aligned");
+  RK_REQUIRE(((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.y) |
+               reinterpret_cast<uintptr_t>(workspace)) & 15u) == 0, kBadArg, "linear_w4a16_group: x, q, y and the workspace must be 16-byte aligned");
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
+  const int cut = getenv("RK_CUT") ? atoi(getenv("RK_CUT")) : 16;
+  if (a.M > cut) {
+    LinearArgs l;
+    l.M = a.M; l.K = a.K; l.N = a.N; l.x = a.x; l.w = a.q; l.fmt = 2; l.scale = a.scale; l.zero = a.zero;
+    l.grouped = true; l.group = a.group; l.epi = a.epi; l.y = a.y;
+    l.scratch = static_cast<float*>(workspace); l.scratch_bytes = workspace ? workspace_bytes : 0;
+    RK_REQUIRE(gemm_tc_supported(l), kShape, "linear_w4a16_group: unsupported shape");
+    return gemm_tc(stream, l);
+  }
   for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
     MatvecPlan p;

@@ -95,7 +95,8 @@ SIGNATURES = {
     "rwkv7_b200_linear_f16_orig_static": [_vp, _i, _i, _i, _vp, _vp, _i, _vp],
     "rwkv7_b200_linear_w8a16": [_vp, _i, _i, _i, _vp, _vp, _vp, _i, _vp],
     "rwkv7_b200_linear_w4a16": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp],
-    "rwkv7_b200_linear_w4a16_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _vp],
+    "rwkv7_b200_linear_w4a16_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, C.c_size_t],
+    "rwkv7_b200_linear_w4a16_group_workspace": [_i, _i, _i, C.POINTER(C.c_size_t)],
     "rwkv7_b200_quant_pack_w4_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp],
     "rwkv7_b200_quant_unpack_w4_group": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp],
     "rwkv7_b200_quant_pack_w8": [_vp, _i, _i, _vp, _vp, _vp],

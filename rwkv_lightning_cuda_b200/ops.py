@@ -6,6 +6,7 @@ enqueued on the current torch stream; nothing here computes on the host.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import List, Optional, Sequence
 
 import torch
@@ -306,7 +307,14 @@ def _good_w4_group(scale, zero, rows, K, group, dev):
 
 
 _HEAD_FORMATS = {torch.float16: L.FMT_F16, torch.int8: L.FMT_W8A16, torch.uint8: L.FMT_W4A16}
-_head_workspaces = {}  # bytes of scratch by (rows, V)
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(query, *sizes):
+    """Bytes of scratch that the library asks for at these sizes."""
+    size = C.c_size_t()
+    L.check(getattr(L.load_library(), query)(*sizes, C.byref(size)))
+    return size.value
+
 
 
 def _refuse_head_logprobs(x, weight, tokens, scale, zero, group_size):
@@ -341,13 +349,7 @@ def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128)
     if not ok:
         _refuse_head_logprobs(x, weight, tokens, scale, zero, group_size)
     lib = L.load_library()
-    need = _head_workspaces.get((rows, V))
-    if need is None:
-        size = C.c_size_t()
-        L.check(lib.rwkv7_b200_head_logprobs_workspace(rows, V, C.byref(size)))
-        need = size.value
-        if len(_head_workspaces) < 4096:
-            _head_workspaces[rows, V] = need
+    need = _scratch_bytes("rwkv7_b200_head_logprobs_workspace", rows, V)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
     logprobs = torch.empty(rows, dtype=_F32, device=dev) if tokens is not None else None
     entropy, lse = torch.empty(rows, dtype=_F32, device=dev), torch.empty(rows, dtype=_F32, device=dev)
@@ -378,8 +380,12 @@ def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NO
     if not ok:
         _refuse_linear_w4a16_group(x, q, scale, zero, group_size)
     y = torch.empty(M, N, dtype=_F32 if epilogue == L.EPI_F32 else _F16, device=dev)
+    need, work = 0, None
+    if M > 8:
+        need = _scratch_bytes("rwkv7_b200_linear_w4a16_group_workspace", M, K, N)
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
     _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(),
-             None if zero is None else zero.data_ptr(), group_size, epilogue, y.data_ptr())
+             None if zero is None else zero.data_ptr(), group_size, epilogue, y.data_ptr(), work.data_ptr() if need else None, need)
     return y
 
 

@@ -47,7 +47,7 @@ def test_head_logprobs_refusals(lib):
 
 def test_linear_w4a16_group_refusals(lib):
     def call(M=1, K=64, N=4, x=P, q=P, scale=P, group=32, epi=0, y=P):
-        return lib.rwkv7_b200_linear_w4a16_group(None, M, K, N, x, q, scale, None, group, epi, y)
+        return lib.rwkv7_b200_linear_w4a16_group(None, M, K, N, x, q, scale, None, group, epi, y, None, 0)
     assert call(M=0) == 1 and call(N=0) == 1 and call(K=0) == 1
     assert call(K=72) == 2 and call(group=16) == 2 and call(group=256) == 2 and call(group=0) == 2
     assert call(x=None) == 1 and call(q=None) == 1 and call(scale=None) == 1 and call(y=None) == 1

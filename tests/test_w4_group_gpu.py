@@ -16,9 +16,10 @@ def ops():
 
 def check_product(y, x, weight, group, what):
     """fp32 sums of K products: at most K / 16 additions to one running sum and 64 more in the merges, each off by at most one step of what has
-    been added up, codes and zeros apart: sum |x| (q + zero) scale.  Then one rounding to half (half a step, or of the smallest subnormal)."""
+    been added up, codes and zeros apart: sum |x| (q + zero) scale.  Then one rounding to half (half a step, or of the smallest subnormal).
+    Beyond 16 rows the weights are rounded to half first."""
     x64 = x.cpu().double()
-    want = x64 @ w4_weights(*weight, group).T
+    want = x64 @ w4_weights(*weight, group, rounded=x.shape[0] > 16).T
     size = x64.abs() @ w4_weights(*weight, group, parts=True).T
     bound = size * (x.shape[1] / 16 + 64) * 2 * U32 + want.abs() * U16 * (1 + 1e-3) + 2.0 ** -25
     got = y.detach().cpu().double()
@@ -59,6 +60,16 @@ def test_pack_and_unpack(ops, N, K, group, symmetric):
 @pytest.mark.parametrize("M,N,K", [(1, 1, 32), (1, 7, 64), (1, 300, 2080), (2, 64, 256), (3, 130, 512), (4, 2561, 1056), (5, 20, 4096), (8, 1000, 416),
                                    (9, 33, 288), (16, 65, 2048), (1, 40, 16384), (7, 24, 16416), (16, 48, 10272)])
 def test_few_rows(ops, M, N, K, group, symmetric):
+    gen = torch.Generator().manual_seed(M + N + K + group)
+    q, s, z = random_w4(N, K, group, symmetric, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    check_product(ops.linear_w4a16_group(x, q, s, z, group), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(17, 128, 128), (33, 130, 416), (96, 1024, 2560), (200, 37, 1056), (256, 516, 288), (300, 40, 4128), (513, 4, 96)])
+def test_many_rows(ops, M, N, K, group, symmetric):
     gen = torch.Generator().manual_seed(M + N + K + group)
     q, s, z = random_w4(N, K, group, symmetric, gen)
     x = torch.randn(M, K, generator=gen).half().cuda()
