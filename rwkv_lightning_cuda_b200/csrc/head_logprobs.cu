@@ -5,14 +5,14 @@
 // are exact integers with the channel's scale on the sum, 4-bit weights half((q - zero) * scale).
 //
 // Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  One CTA per SM walks the units (128 rows x
-// 256 tokens), the row blocks of a token tile one after the other, so that neighbouring CTAs share a tile of weights and
-// it comes from HBM once.  The rows take the MMA's M side and the tokens its N side: a lane of tensor memory is then a row
+// up to 256 tokens), the row blocks of a token tile one after the other, so that neighbouring CTAs share a tile of weights
+// and it comes from HBM once.  The rows take the MMA's M side and the tokens its N side: a lane of tensor memory is then a row
 // of x, and an epilogue thread reduces its row's 256 logits without talking to any other.  Two accumulators, so that
 // a unit's epilogue runs under the next one's products.
 //
 // Warp roles: 0 loads (TMA, 128-byte swizzle), 1 issues tcgen05.mma, 2..5 reduce.  Quantised weights: warp 0 brings
 // packed tiles into a ring of their own, warp 6 the rows of x, and 16 more warps expand a packed tile into the swizzled
-// fp16 tile that the MMA reads (two threads to a weight row).  Every wait is bounded: one that runs out sets the device's
+// fp16 tile that the MMA reads (a thread to a weight row, the two halves of the warps taking turns).  Every wait is bounded: one that runs out sets the device's
 // failure word, every role leaves its loop, and the CTA frees its tensor memory and returns.
 #include <cuda.h>
 
@@ -27,7 +27,8 @@ namespace rk {
 namespace {
 
 constexpr int kRows = 128;   // rows of x per unit = MMA M
-constexpr int kToks = 256;   // tokens per unit = MMA N
+constexpr int kToks = 256;   // tokens per unit = MMA N, at most (HeadShape::toks)
+constexpr int kMinToks = 128;
 constexpr int kBK = 64;      // halves per K block = one 128-byte swizzle row
 constexpr uint32_t kXBytes = kRows * 128, kWBytes = kToks * 128, kStageBytes = kXBytes + kWBytes;
 constexpr int kExpandWarps = 16;
@@ -40,6 +41,12 @@ template <> struct Ring<1> { static constexpr int tiles = 3, raws = 4, raw_row =
 template <> struct Ring<2> { static constexpr int tiles = 3, raws = 8, raw_row = kBK / 2, raw = kToks * raw_row; };
 template <int kFmt> constexpr size_t smem_bytes() { return 1024 + Ring<kFmt>::tiles * kStageBytes + Ring<kFmt>::raws * Ring<kFmt>::raw; }
 template <int kFmt> constexpr int head_threads() { return kFmt == 0 ? 192 : 256 + kExpandWarps * 32; }
+
+struct HeadShape {
+  int toks, tiles;        // tokens per unit, token tiles
+  int row_blocks, units;  // blocks of 128 rows
+  int x_rows;             // rows of x that a block loads: all there are, in eights, up to 128 (the rest of the tile is not read out)
+};
 
 struct HeadMaps {
   CUtensorMap x, w;
@@ -88,8 +95,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 struct Group4 {
   __half2 scale, sub;  // (s, s) and (-(1024 + z), -(64 + z))
 };
-__device__ __forceinline__ Group4 group4(half s, float z) {
-  return {__half2half2(s), __halves2half2(__float2half_rn(-1024.f - z), __float2half_rn(-64.f - z))};
+__device__ __forceinline__ Group4 group4(uint32_t s2, uint32_t z2) {  // the group's scale and zero, twice each
+  return {*reinterpret_cast<const __half2*>(&s2), __hsub2(__floats2half2_rn(-1024.f, -64.f), *reinterpret_cast<const __half2*>(&z2))};
+}
+// Half i of eight, twice.
+__device__ __forceinline__ uint32_t pick(const uint4& v, int i) {
+  const uint32_t lo = i & 2 ? v.y : v.x, hi = i & 2 ? v.w : v.z;
+  return __byte_perm(i & 4 ? hi : lo, 0u, i & 1 ? 0x3232 : 0x1010);
 }
 __device__ __forceinline__ uint4 expand4(uint32_t w, const Group4& g) {
   const __half2 mul = __floats2half2_rn(1.0f, 0.0625f);
@@ -114,7 +126,7 @@ __device__ __forceinline__ uint2 expand8(uint32_t w) {
 
 template <int kFmt>
 __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
-    head_tc_kernel(const __grid_constant__ HeadMaps maps, const HeadLogprobsArgs a, const int row_blocks, const int units, int* timeout) {
+    head_tc_kernel(const __grid_constant__ HeadMaps maps, const HeadLogprobsArgs a, const HeadShape h, int* timeout) {
   constexpr int kTiles = Ring<kFmt>::tiles, kRaws = Ring<kFmt>::raws > 0 ? Ring<kFmt>::raws : 1;
   extern __shared__ unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kTiles], ready[kTiles], empty[kTiles], raw_full[kRaws], raw_empty[kRaws], acc_full[2], acc_empty[2];
@@ -128,12 +140,12 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kTiles; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&ready[i]), kExpandWarps);
+      mbar_init(smem_u32(&ready[i]), kExpandWarps / 2);
       mbar_init(smem_u32(&empty[i]), 1);
     }
     for (int i = 0; i < kRaws; ++i) {
       mbar_init(smem_u32(&raw_full[i]), 1);
-      mbar_init(smem_u32(&raw_empty[i]), kExpandWarps);
+      mbar_init(smem_u32(&raw_empty[i]), kExpandWarps / 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&acc_full[i]), 1);
@@ -161,17 +173,17 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
       const bool packed = kFmt != 0 && warp == 0;
       const int stages = packed ? kRaws : kTiles;
       int it = 0;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const int r0 = (u % row_blocks) * kRows, n0 = (u / row_blocks) * kToks;
+      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+        const int r0 = (u % h.row_blocks) * kRows, n0 = (u / h.row_blocks) * h.toks;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % stages;
           if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], (it / stages - 1) & 1))) break;
           const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]), dst = ring + s * kStageBytes;
           if (packed) {
-            mbar_expect_tx(bar, Ring<kFmt>::raw);
+            mbar_expect_tx(bar, h.toks * Ring<kFmt>::raw_row);
             tma_2d(raw_ring + s * Ring<kFmt>::raw, &maps.w, bar, kb * Ring<kFmt>::raw_row, n0);
           } else {
-            mbar_expect_tx(bar, kFmt == 0 ? kStageBytes : kXBytes);
+            mbar_expect_tx(bar, 128 * (h.x_rows + (kFmt == 0 ? h.toks : 0)));
             tma_2d(dst, &maps.x, bar, kb * kBK, r0);
             if (kFmt == 0) tma_2d(dst + kXBytes, &maps.w, bar, kb * kBK, n0);
           }
@@ -183,9 +195,9 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
   } else if (warp == 1) {
     // ---- products: K blocks of 64 as four instructions into the unit's accumulator
     if (lane == 0) {
-      constexpr uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(kToks >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(h.toks >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
       int it = 0, n = 0;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++n) {
+      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
         if (n >= 2 && !(ok = wait(acc_empty[n & 1], ((n >> 1) - 1) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + (n & 1) * kToks;
@@ -206,8 +218,8 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
     // ---- reduction: a thread owns a row of x, its TMEM lane, and takes the unit's tokens 32 at a time
     const int quad = warp & 3, t = threadIdx.x - 64;
     int n = 0;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++n) {
-      const int r = (u % row_blocks) * kRows + quad * 32 + lane, n0 = (u / row_blocks) * kToks, toks = min(kToks, a.V - n0);
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
+      const int r = (u % h.row_blocks) * kRows + quad * 32 + lane, n0 = (u / h.row_blocks) * h.toks, toks = min(h.toks, a.V - n0);
       const int64_t id = a.tokens && r < a.rows ? a.tokens[r] : -1;
       if (kFmt == 1) {
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the last unit's scales have been read
@@ -250,42 +262,82 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0) arrive(smem_u32(&acc_empty[n & 1]));
-      if (r < a.rows) a.part[static_cast<size_t>(u / row_blocks) * a.rows + r] = make_float4(st.m, st.s, st.t, 0.f);
+      if (r < a.rows) a.part[static_cast<size_t>(u / h.row_blocks) * a.rows + r] = make_float4(st.m, st.s, st.t, 0.f);
     }
   } else if (kFmt != 0 && warp >= 8) {
-    // ---- expansion: two threads to a weight row, 32 weights each.  Row r of the tile is 128 bytes at r * 128, its 16-byte
-    // chunk c at chunk position c ^ (r & 7).
-    const int e = threadIdx.x - 256, r = e >> 1, part = e & 1;
+    // ---- expansion: a thread owns a row of the tile, 64 weights a K block; half of the warps take the even K blocks, half the odd
+    // ones.  Row r of the tile is 128 bytes at r * 128, its 16-byte chunk c at chunk position c ^ (r & 7); a packed row of 64 (32)
+    // bytes has its chunk c at c ^ (r / 2 & 3) (c ^ (r / 4 & 1)): the swizzles of 128-, 64- and 32-byte rows, so that no two
+    // lanes of a quarter warp meet in a bank.  (No barrier's phase is
+    // missed by taking every other K block: the packed ring is even, and of the three tiles of the other ring the one waited for
+    // is at most a phase ahead of the tile this thread waited for two blocks before.)
+    const int r = threadIdx.x & 255, turn = (threadIdx.x >> 8) - 1;
     unsigned char* const base = smem + (ring - smem_u32(smem));
-    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
-    int it = 0;
-    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const int row = (u / row_blocks) * kToks + r;
-      for (int kb = 0; kb < kblocks; ++kb, ++it) {
-        const int s = it % kTiles, rs = it % kRaws;
-        Group4 g = group4(__float2half_rn(0.f), 0.f);
-        if (kFmt == 2 && row < a.V) {  // requested before the wait for the tile
-          const size_t gi = static_cast<size_t>(row) * groups + min((kb * kBK + part * 32) >> shift, groups - 1);
-          g = group4(a.scale[gi], a.zero ? __half2float(a.zero[gi]) : 8.f);
+    const unsigned char* const raw = base + kTiles * kStageBytes + r * Ring<kFmt>::raw_row;
+    unsigned char* const tile = base + kXBytes + r * 128;
+    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift, swz = (r & 7) << 4;
+    const int raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
+    // multiple of 16 bytes, group by group.
+    const bool eights = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
+    const uint16_t *sp = nullptr, *zp = nullptr;
+    constexpr uint32_t kEight = 0x48004800u;
+    uint4 sc = make_uint4(0u, 0u, 0u, 0u), ze = make_uint4(kEight, kEight, kEight, kEight), sc_next = sc, ze_next = ze;
+    auto load8 = [&](int block) {
+      if (block * 8 >= groups) return;
+      sc_next = reinterpret_cast<const uint4*>(sp)[block];
+      if (zp) ze_next = reinterpret_cast<const uint4*>(zp)[block];
+    };
+    auto load_runs = [&](int kb) {  // a K block's two runs of 32 weights into the first two halves
+      const int g0 = min((kb * kBK) >> shift, groups - 1), g1 = min((kb * kBK + 32) >> shift, groups - 1);
+      sc_next.x = sp[g0] | (static_cast<uint32_t>(sp[g1]) << 16);
+      if (zp) ze_next.x = zp[g0] | (static_cast<uint32_t>(zp[g1]) << 16);
+    };
+    int it = 0, rs = turn, raw_phase = 0, s = turn, tile_phase = 0;
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+      const int row = min((u / h.row_blocks) * h.toks + r, a.V - 1);
+      int kb = (it & 1) == turn ? 0 : 1;
+      int block = -1;
+      if (kFmt == 2 && kb < kblocks) {
+        sp = reinterpret_cast<const uint16_t*>(a.scale) + static_cast<size_t>(row) * groups;
+        if (a.zero) zp = reinterpret_cast<const uint16_t*>(a.zero) + static_cast<size_t>(row) * groups;
+        if (eights) load8((kb * kBK) >> (shift + 3));
+        else load_runs(kb);
+      }
+      for (; kb < kblocks; kb += 2) {
+        const bool first_round = it + kb < kTiles;
+        if (kFmt == 2 && (!eights || (kb * kBK) >> (shift + 3) != block)) {
+          sc = sc_next;
+          ze = ze_next;
+          block = (kb * kBK) >> (shift + 3);
+          if (eights) load8(block + 1);
         }
-        ok = __all_sync(0xffffffffu, wait(raw_full[rs], (it / kRaws) & 1) && (it < kTiles || wait(empty[s], (it / kTiles - 1) & 1)));
+        ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase) && (first_round || wait(empty[s], tile_phase ^ 1)));
         if (!ok) break;
-        const unsigned char* src = base + kTiles * kStageBytes + rs * Ring<kFmt>::raw + r * Ring<kFmt>::raw_row + part * (Ring<kFmt>::raw_row / 2);
-        uint4* dst = reinterpret_cast<uint4*>(base + s * kStageBytes + kXBytes + r * 128);
-        if (kFmt == 1) {
+        if (r < h.toks) {
+          const unsigned char* const src = raw + rs * Ring<kFmt>::raw;
+          unsigned char* const dst = tile + s * kStageBytes;
+          if (kFmt == 1) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint4 q = reinterpret_cast<const uint4*>(src)[c];
-            const uint2 h0 = expand8(q.x), h1 = expand8(q.y), h2 = expand8(q.z), h3 = expand8(q.w);
-            dst[(part * 4 + 2 * c) ^ (r & 7)] = make_uint4(h0.x, h0.y, h1.x, h1.y);
-            dst[(part * 4 + 2 * c + 1) ^ (r & 7)] = make_uint4(h2.x, h2.y, h3.x, h3.y);
+            for (int c = 0; c < 4; ++c) {
+              const uint4 q = *reinterpret_cast<const uint4*>(src + ((16 * c) ^ raw_swz));
+              const uint2 h0 = expand8(q.x), h1 = expand8(q.y), h2 = expand8(q.z), h3 = expand8(q.w);
+              *reinterpret_cast<uint4*>(dst + ((32 * c) ^ swz)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
+              *reinterpret_cast<uint4*>(dst + ((32 * c + 16) ^ swz)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
+              const Group4 g = group4(pick(sc, i), pick(ze, i));
+              const uint4 q = *reinterpret_cast<const uint4*>(src + ((16 * c) ^ raw_swz));
+              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(dst + ((64 * c + 16 * i) ^ swz)) = expand4(w[i], g);
+            }
           }
-        } else {
-          const uint4 q = *reinterpret_cast<const uint4*>(src);
-          const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[(part * 4 + i) ^ (r & 7)] = expand4(w[i], g);
         }
+        if (kFmt == 2 && !eights && kb + 2 < kblocks) load_runs(kb + 2);  // under way until this thread's next turn
         // written through the generic proxy, read by the tensor core through the async one
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -293,7 +345,12 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
           arrive(smem_u32(&ready[s]));
           arrive(smem_u32(&raw_empty[rs]));
         }
+        rs += 2;
+        if (rs >= kRaws) { rs -= kRaws; raw_phase ^= 1; }
+        s += 2;
+        if (s >= kTiles) { s -= kTiles; tile_phase ^= 1; }
       }
+      it += kblocks;
     }
   }
   if (!ok) failed = 1;
@@ -326,7 +383,7 @@ __global__ void __launch_bounds__(256) head_merge_kernel(HeadLogprobsArgs a, int
 }
 
 // A 2-D tensor [rows, row_bytes / size of an element] in boxes of box_cols x box_rows, zeros outside.
-int head_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int rows, size_t cols, int box_cols, int box_rows, bool swizzle) {
+int head_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int rows, size_t cols, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
   const TensorMapEncodeFn fn = tensor_map_encode_fn();
   RK_REQUIRE(fn, kCuda, "head_logprobs: cuTensorMapEncodeTiled is not available from this driver");
   const cuuint64_t dims[2] = {cols, static_cast<cuuint64_t>(rows)};
@@ -334,28 +391,43 @@ int head_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const v
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t elem[2] = {1, 1};
   const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "head_logprobs: cuTensorMapEncodeTiled failed with %d (rows=%d, columns=%zu)", static_cast<int>(r), rows, cols);
   return kOk;
 }
 
+// The token tile that lets the units come out in the fewest full rounds over the SMs (65536 tokens in tiles of 256 are 1.7 rounds
+// of 148, in tiles of 224 two full ones); a unit is counted as its tokens and 32 more for its beginning and end.
+HeadShape head_shape(int rows, int V, int sms) {
+  HeadShape best = {};
+  long long least = -1;
+  for (int toks = kToks; toks >= kMinToks; toks -= 16) {
+    HeadShape h;
+    h.toks = toks;
+    h.tiles = (V + toks - 1) / toks;
+    h.row_blocks = (rows + kRows - 1) / kRows;
+    h.x_rows = std::min(kRows, (rows + 7) & ~7);
+    const long long units = static_cast<long long>(h.tiles) * h.row_blocks, cost = (units + sms - 1) / sms * (toks + 32);
+    h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
+    if (least < 0 || cost < least) { least = cost; best = h; }
+  }
+  return best;
+}
+
 template <int kFmt>
-int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, int sms) {
+int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, const HeadShape& h, int sms) {
   HeadMaps maps;
-  int s = head_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, kBK, kRows, true);
+  int s = head_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, kBK, h.x_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != kOk) return s;
-  if (kFmt == 0) s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.w, a.V, a.K, kBK, kToks, true);
-  else s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.V, kFmt == 1 ? a.K : a.K / 2, Ring<kFmt>::raw_row, kToks, false);
+  if (kFmt == 0) s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.w, a.V, a.K, kBK, h.toks, CU_TENSOR_MAP_SWIZZLE_128B);
+  else s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.V, kFmt == 1 ? a.K : a.K / 2, Ring<kFmt>::raw_row, h.toks,
+                    kFmt == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
   if (s != kOk) return s;
-  const int row_blocks = (a.rows + kRows - 1) / kRows, tiles = (a.V + kToks - 1) / kToks;
-  RK_REQUIRE(static_cast<long long>(row_blocks) * tiles < (1ll << 31), kShape, "head_logprobs: too many rows");
-  const int units = row_blocks * tiles;
   RK_CUDA(cudaFuncSetAttribute(head_tc_kernel<kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<kFmt>())));
-  RK_CUDA(launch_pdl(head_tc_kernel<kFmt>, dim3(std::min(units, sms)), dim3(head_threads<kFmt>()), smem_bytes<kFmt>(), stream, maps, a, row_blocks, units,
+  RK_CUDA(launch_pdl(head_tc_kernel<kFmt>, dim3(std::min(h.units, sms)), dim3(head_threads<kFmt>()), smem_bytes<kFmt>(), stream, maps, a, h,
                      timeout_word_or_null()));
   RK_LAUNCH_CHECK("head_logprobs launch");
-  RK_CUDA(launch_pdl(head_merge_kernel, dim3((a.rows + 7) / 8), dim3(256), 0, stream, a, tiles));
+  RK_CUDA(launch_pdl(head_merge_kernel, dim3((a.rows + 7) / 8), dim3(256), 0, stream, a, h.tiles));
   RK_LAUNCH_CHECK("head_logprobs merge launch");
   return kOk;
 }
@@ -363,7 +435,7 @@ int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, int sms) {
 }  // namespace
 
 size_t head_logprobs_workspace(int rows, int V) {
-  const size_t tiles = (static_cast<size_t>(V) + kToks - 1) / kToks;
+  const size_t tiles = (static_cast<size_t>(V) + kMinToks - 1) / kMinToks;
   return static_cast<size_t>(rows) * (tiles * sizeof(float4) + sizeof(float));
 }
 
@@ -379,13 +451,15 @@ int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size
   RK_REQUIRE(workspace && workspace_bytes >= head_logprobs_workspace(a.rows, a.V), kBadArg, "head_logprobs: the workspace needs %zu bytes",
              head_logprobs_workspace(a.rows, a.V));
   a.part = static_cast<float4*>(workspace);
-  a.given = reinterpret_cast<float*>(a.part + (static_cast<size_t>(a.V) + kToks - 1) / kToks * a.rows);
   int sms = 0;
   const int status = device_sms(&sms);
   if (status != kOk) return status;
-  if (a.fmt == 1) return launch_head<1>(stream, a, sms);
-  if (a.fmt == 2) return launch_head<2>(stream, a, sms);
-  return launch_head<0>(stream, a, sms);
+  const HeadShape h = head_shape(a.rows, a.V, sms);
+  RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
+  a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
+  if (a.fmt == 1) return launch_head<1>(stream, a, h, sms);
+  if (a.fmt == 2) return launch_head<2>(stream, a, h, sms);
+  return launch_head<0>(stream, a, h, sms);
 }
 
 }  // namespace rk
