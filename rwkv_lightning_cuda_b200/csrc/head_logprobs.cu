@@ -61,6 +61,20 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
 __device__ __forceinline__ void arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Bounded wait: out of line after the first try, and over as soon as another role has given up.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, const volatile int* failed) {
+  for (uint32_t i = 0; i < kSpinLimit && !*failed; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 // Shared-memory matrix descriptor: K-major tile, 128-byte swizzle, 8-row groups 1024 bytes apart.
 __device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
   return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -165,7 +179,7 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
   pdl_wait();
   pdl_trigger();
 
-  auto wait = [&](uint64_t& bar, int parity) { return !failed && mbar_wait(smem_u32(&bar), parity); };
+  auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
   bool ok = true;
   if (warp == 0 || (kFmt != 0 && warp == 6)) {
     // ---- loads: the fp16 tiles of both operands, or the packed weights (warp 0) and the rows (warp 6) on rings of their own
@@ -235,7 +249,7 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       SoftStats st;
-      for (int c = 0; c < toks; c += 32) {
+      for (int c = 0; c < toks && r - lane < a.rows; c += 32) {  // (nothing to do for a warp beyond the last row)
         float z[32];
         tmem_ld32(tmem + (n & 1) * kToks + c + (static_cast<uint32_t>(quad * 32) << 16), z);
         const int here = min(32, toks - c);
@@ -272,11 +286,11 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
     // missed by taking every other K block: the packed ring is even, and of the three tiles of the other ring the one waited for
     // is at most a phase ahead of the tile this thread waited for two blocks before.)
     const int r = threadIdx.x & 255, turn = (threadIdx.x >> 8) - 1;
-    unsigned char* const base = smem + (ring - smem_u32(smem));
-    const unsigned char* const raw = base + kTiles * kStageBytes + r * Ring<kFmt>::raw_row;
-    unsigned char* const tile = base + kXBytes + r * 128;
-    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift, swz = (r & 7) << 4;
-    const int raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    const uint32_t raw = raw_ring + r * Ring<kFmt>::raw_row, raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
+    uint32_t at[8];  // where the chunks of this row go, in the first stage
+#pragma unroll
+    for (int c = 0; c < 8; ++c) at[c] = ring + kXBytes + r * 128 + ((16 * c) ^ ((r & 7) << 4));
     // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
     // multiple of 16 bytes, group by group.
     const bool eights = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
@@ -315,25 +329,24 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
         ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase) && (first_round || wait(empty[s], tile_phase ^ 1)));
         if (!ok) break;
         if (r < h.toks) {
-          const unsigned char* const src = raw + rs * Ring<kFmt>::raw;
-          unsigned char* const dst = tile + s * kStageBytes;
+          const uint32_t src = raw + rs * Ring<kFmt>::raw, stage = s * kStageBytes;
           if (kFmt == 1) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const uint4 q = *reinterpret_cast<const uint4*>(src + ((16 * c) ^ raw_swz));
+              const uint4 q = lds16(src + ((16 * c) ^ raw_swz));
               const uint2 h0 = expand8(q.x), h1 = expand8(q.y), h2 = expand8(q.z), h3 = expand8(q.w);
-              *reinterpret_cast<uint4*>(dst + ((32 * c) ^ swz)) = make_uint4(h0.x, h0.y, h1.x, h1.y);
-              *reinterpret_cast<uint4*>(dst + ((32 * c + 16) ^ swz)) = make_uint4(h2.x, h2.y, h3.x, h3.y);
+              sts16(at[2 * c] + stage, make_uint4(h0.x, h0.y, h1.x, h1.y));
+              sts16(at[2 * c + 1] + stage, make_uint4(h2.x, h2.y, h3.x, h3.y));
             }
           } else {
+            const uint4 q0 = lds16(src + raw_swz), q1 = lds16(src + (16 ^ raw_swz));
+            const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
               const Group4 g = group4(pick(sc, i), pick(ze, i));
-              const uint4 q = *reinterpret_cast<const uint4*>(src + ((16 * c) ^ raw_swz));
-              const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(dst + ((64 * c + 16 * i) ^ swz)) = expand4(w[i], g);
+              for (int j = 0; j < 4; ++j) sts16(at[4 * c + j] + stage, expand4(w[4 * c + j], g));
             }
           }
         }
@@ -361,21 +374,26 @@ __global__ void __launch_bounds__(head_threads<kFmt>(), 1)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// One warp per row merges the row's tiles.
-__global__ void __launch_bounds__(256) head_merge_kernel(HeadLogprobsArgs a, int tiles) {
+// One CTA per row merges the row's tiles: a load or two per thread, all under way at once.
+constexpr int kMergeThreads = 256;
+__global__ void __launch_bounds__(kMergeThreads) head_merge_kernel(HeadLogprobsArgs a, int tiles) {
+  __shared__ SoftStats warps[kMergeThreads / 32];
   pdl_wait();
   pdl_trigger();
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (r >= a.rows) return;
+  const int r = blockIdx.x, t = threadIdx.x;
   SoftStats st;
-  for (int i = lane; i < tiles; i += 32) {
+  for (int i = t; i < tiles; i += kMergeThreads) {
     const float4 p = a.part[static_cast<size_t>(i) * a.rows + r];
     SoftStats b;
     b.m = p.x; b.s = p.y; b.t = p.z;
     st = merge(st, b);
   }
   st = warp_merge(st);
-  if (lane != 0) return;
+  if ((t & 31) == 0) warps[t >> 5] = st;
+  __syncthreads();
+  if (t != 0) return;
+#pragma unroll
+  for (int w = 1; w < kMergeThreads / 32; ++w) st = merge(st, warps[w]);
   const RowResult res = finish(st);
   if (a.entropy) a.entropy[r] = res.entropy;
   if (a.lse) a.lse[r] = res.lse;
@@ -427,17 +445,60 @@ int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, const HeadShape&
   RK_CUDA(launch_pdl(head_tc_kernel<kFmt>, dim3(std::min(h.units, sms)), dim3(head_threads<kFmt>()), smem_bytes<kFmt>(), stream, maps, a, h,
                      timeout_word_or_null()));
   RK_LAUNCH_CHECK("head_logprobs launch");
-  RK_CUDA(launch_pdl(head_merge_kernel, dim3((a.rows + 7) / 8), dim3(256), 0, stream, a, h.tiles));
+  RK_CUDA(launch_pdl(head_merge_kernel, dim3(a.rows), dim3(kMergeThreads), 0, stream, a, h.tiles));
   RK_LAUNCH_CHECK("head_logprobs merge launch");
   return kOk;
 }
 
 }  // namespace
 
+// Few rows: the weight-streaming kernels read the weights once at a better rate than the kernel above with its 128-row tiles
+// and expansion through shared memory, and the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said
+// otherwise), this route against the other: 4-bit 53 against 90 us at one row, 61 against 91 at eight (31 against 48 at two
+// and K = 2048); int8 61 against 74 us at four rows; fp16 84 against 94 us at one row, but 111 against 94 at four.  In
+// small matrices of 8- and 16-bit weights the second pass costs more than it saves (32003 x 768 int8: 18.5 against 15.5 us).
+constexpr int kFewRowsF16 = 1, kFewRowsW8 = 4, kFewRowsW4 = 8;
+constexpr double kFewRowsBytes = 64e6;
+
 size_t head_logprobs_workspace(int rows, int V) {
   const size_t tiles = (static_cast<size_t>(V) + kMinToks - 1) / kMinToks;
-  return static_cast<size_t>(rows) * (tiles * sizeof(float4) + sizeof(float));
+  const size_t need = static_cast<size_t>(rows) * (tiles * sizeof(float4) + sizeof(float));
+  return rows <= kFewRowsW4 ? std::max(need, static_cast<size_t>(rows) * V * sizeof(float)) : need;
 }
+
+namespace {
+
+// (K: what the products stage of x in shared memory.)
+bool few_rows(const HeadLogprobsArgs& a, int sms) {
+  if (a.fmt == 2) {
+    W4GroupArgs w;
+    w.M = a.rows; w.K = a.K; w.N = a.V; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
+    return a.rows <= kFewRowsW4 && w4_rounded_fits(w, sms);
+  }
+  const double bytes = static_cast<double>(a.V) * a.K * (a.fmt == 0 ? 2 : 1);
+  return a.rows <= (a.fmt == 0 ? kFewRowsF16 : kFewRowsW8) && a.K <= 16384 && bytes >= kFewRowsBytes;
+}
+// Logits into the workspace, then their statistics.
+int logits_then_stats(cudaStream_t stream, const HeadLogprobsArgs& a, float* logits, int sms) {
+  int s;
+  if (a.fmt == 2) {
+    W4GroupArgs w;
+    w.M = a.rows; w.K = a.K; w.N = a.V; w.group = a.group; w.x = a.x; w.q = static_cast<const uint8_t*>(a.w); w.scale = a.scale; w.zero = a.zero;
+    w.epi = kEpiRawF32; w.y = logits;
+    s = w4_rounded_linear(stream, w, sms);
+  } else {
+    LinearArgs l;
+    l.M = a.rows; l.K = a.K; l.N = a.V; l.x = a.x; l.w = a.w; l.fmt = a.fmt; l.scale = a.scale; l.epi = kEpiRawF32; l.y = logits;
+    s = linear(stream, l);
+  }
+  if (s != kOk) return s;
+  TokenLogprobsArgs t;
+  t.rows = a.rows; t.V = a.V; t.logits = logits; t.ld = a.V; t.tokens = a.tokens; t.n_tokens = a.tokens ? 1 : 0;
+  t.logprobs = a.logprobs; t.entropy = a.entropy; t.lse = a.lse;
+  return token_logprobs(stream, t);
+}
+
+}  // namespace
 
 int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size_t workspace_bytes) {
   RK_REQUIRE(a.rows > 0 && a.K > 0 && a.V > 0 && a.x && a.w, kBadArg, "head_logprobs: bad argument");
@@ -454,6 +515,7 @@ int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size
   int sms = 0;
   const int status = device_sms(&sms);
   if (status != kOk) return status;
+  if (few_rows(a, sms)) return logits_then_stats(stream, a, static_cast<float*>(workspace), sms);
   const HeadShape h = head_shape(a.rows, a.V, sms);
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
   a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);

@@ -225,9 +225,12 @@ struct W4GroupArgs {
   const uint8_t* q = nullptr;   // [N, K/2]
   const half* scale = nullptr;  // [N, ceil(K / group)]
   const half* zero = nullptr;   // as scale, or nullptr: 8
-  int epi = kEpiNone;           // kEpiNone, kEpiRelu2 or kEpiF32
+  int epi = kEpiNone;           // kEpiNone, kEpiRelu2 or kEpiF32 (w4_rounded_linear: kEpiRawF32 too)
   void* y = nullptr;            // half [M, N], or float for kEpiF32
 };
+// The product of up to eight rows with weights rounded to half, half((q - zero) * scale), as the tensor-core kernels take them.
+bool w4_rounded_fits(const W4GroupArgs& args, int sms);
+int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& args, int sms);
 size_t w4_group_workspace(int M, int K, int N);  // scratch that lets many rows split K over more SMs; 0: none is used
 int w4_group_linear(cudaStream_t stream, const W4GroupArgs& args, void* workspace, size_t workspace_bytes);
 bool gemm_tc_supported(const LinearArgs& args);         // gemm_tcgen05.cu

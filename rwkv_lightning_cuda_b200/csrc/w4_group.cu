@@ -12,6 +12,9 @@
 //   - mma.sync m16n8k16 has eight columns.  With fewer rows of x the columns hold different 32-weight chunks (a
 //     lane whose column is another chunk's reads zeros), so that with one row eight chunks end up in eight columns and the
 //     scales are applied once for all of them.
+// kRounded: the same walk for callers whose weights are half((q - zero) * scale) (the head product of head_logprobs.cu): a word
+// becomes eight such halves (one subtraction or fused multiply-add and one product per two), the sums need no scales, and
+// the columns are up to eight rows of x.
 // One CTA of 16 warps per SM takes a contiguous range of output channels in tiles of up to 32.  The warps form 1, 2 or 4
 // teams with a tile each; the tile's K extent is cut into boxes of 128 bytes per row, dealt out to the team's warps and
 // fetched by one 2-D tensor copy each into the warp's ring.  The warps' partial sums of a tile are added in warp order:
@@ -19,7 +22,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -31,7 +33,8 @@ namespace {
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
 constexpr int kBoxWeights = 256;  // 128 bytes along a row: eight chunks of 32 weights
-constexpr int kMaxRows = 8;
+constexpr int kMaxRows = 8;      // of a launch
+constexpr int kMatvecRows = 16;  // up to which the launches of eight rows are used, see w4_group_linear
 constexpr size_t kSmemLimit = 226 * 1024;
 
 struct MatvecMaps {
@@ -71,13 +74,27 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
       ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// The eight weights of a word as pairs (0, 4), (1, 5), (2, 6), (3, 7): a nibble under the exponent of 1024 is 1024 + q, a high one
+// 1024 + 16 q; less 1024 + zero (or / 16 less 64 + zero) that is q - zero exactly, and the product rounds once.
+__device__ __forceinline__ void round4(uint32_t u, __half2 s, __half2 zlo, __half2 zhi, uint32_t (&o)[4]) {
+  const uint32_t v = u >> 8;
+  const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+  o[0] = h2u(__hmul2(__hsub2(u2h((u & 0x000f000fu) | 0x64006400u), zlo), s));
+  o[1] = h2u(__hmul2(__hfma2(u2h((u & 0x00f000f0u) | 0x64006400u), sixteenth, zhi), s));
+  o[2] = h2u(__hmul2(__hsub2(u2h((v & 0x000f000fu) | 0x64006400u), zlo), s));
+  o[3] = h2u(__hmul2(__hfma2(u2h((v & 0x00f000f0u) | 0x64006400u), sixteenth, zhi), s));
+}
 __device__ __forceinline__ float half_of(uint32_t pair, int i) {
   const float2 f = h2f2(pair);
   return i ? f.y : f.x;
 }
 __device__ __forceinline__ void store_epi(const W4GroupArgs& a, size_t o, float v) {
   const half hy = __float2half_rn(v);
-  if (a.epi == kEpiF32) {
+  if (a.epi == kEpiRawF32) {
+    static_cast<float*>(a.y)[o] = v;
+  } else if (a.epi == kEpiF32) {
     static_cast<float*>(a.y)[o] = __half2float(hy);
   } else if (a.epi == kEpiRelu2) {
     const float u = fmaxf(__half2float(hy), 0.f);
@@ -91,10 +108,11 @@ __device__ __forceinline__ void store_epi(const W4GroupArgs& a, size_t o, float 
 // kPass chunks, after each of which the sums are scaled; chunk c of a pass goes to the columns of slot c mod kSlots.
 // kBlk: blocks of 16 rows in a tile.  kCopied: scales and zeros come with their box, by tensor copies of the eight groups
 // (16 bytes) of each row that hold the box's; otherwise (rows of groups that are not multiples of 16 bytes) through registers.
-template <int kM, int kShift, int kBlk, bool kCopied>
+template <int kM, int kShift, int kBlk, bool kCopied, bool kRounded>
 __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_constant__ MatvecMaps maps, const W4GroupArgs a, const MatvecPlan p, int* timeout) {
   constexpr int kSlots = 8 / kM, kGroupChunks = 1 << (kShift - 5);
   constexpr int kPass = kSlots > kGroupChunks ? kSlots : kGroupChunks, kPasses = 8 / kPass;
+  static_assert(!kRounded || kM == 8, "");
   constexpr float kUnit = 1.0f / 16777216.0f;  // what a code of 1 stands for in the products
   extern __shared__ unsigned char smem_dyn[];
   __shared__ __align__(8) uint64_t bars[kWarps][4];
@@ -268,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
         float v = 0.f;
 #pragma unroll 4
         for (int w = 0; w < team_warps; ++w) v += sums_of[w * kTileRows * kM + r * kM + m];
-        store_epi(a, static_cast<size_t>(m) * a.N + n, v * 16777216.0f);
+        store_epi(a, static_cast<size_t>(m) * a.N + n, kRounded ? v : v * 16777216.0f);
       }
     }
     if (c_tile >= tiles) break;
@@ -300,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
       }
       const uint32_t x_now = x_row + (kb << 9);
       float lo[kBlk][4], hi[kBlk][4];
+      __half2 scale2[2 * kBlk], zero_lo[2 * kBlk], zero_hi[2 * kBlk];  // kRounded
 #pragma unroll
       for (int c2 = 0; c2 < 4; ++c2) {
         // Two chunks of 16 rows: the matrices are (rows 0-7, rows 8-15) x (chunk 2 c2, chunk 2 c2 + 1), 16 bytes a row, and a lane gets
@@ -313,6 +332,33 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
           uint4 xv;
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
                        : "r"((kSlots == 1 || slot_of_lane == c % kSlots ? x_now : zero_now) + (c << 6)));
+          if (kRounded) {
+            if (c % kGroupChunks == 0) {  // a new group: its parameters for the rows g and g + 8 of each block
+              const int from = kShift == 7 ? (c >> 2) << 1 : c >> 1;
+#pragma unroll
+              for (int i = 0; i < 2 * kBlk; ++i) {
+                const uint32_t sp = __shfl_sync(0xffffffffu, s_now[i], (lane & ~3) | from), zp = __shfl_sync(0xffffffffu, z_now[i], (lane & ~3) | from);
+                const uint32_t sel = kShift == 5 && (c & 1) ? 0x3232 : 0x1010;
+                const uint32_t s2 = __byte_perm(sp, 0u, sel), z2 = __byte_perm(zp, 0u, sel);
+                scale2[i] = u2h(s2);
+                zero_lo[i] = __hadd2(u2h(z2), __floats2half2_rn(1024.f, 1024.f));
+                zero_hi[i] = __hneg2(__hadd2(u2h(z2), __floats2half2_rn(64.f, 64.f)));
+              }
+            }
+#pragma unroll
+            for (int b = 0; b < kBlk; ++b) {
+              uint32_t ra[4], rb[4];
+              round4(w[b][2 * cc], scale2[2 * b], zero_lo[2 * b], zero_hi[2 * b], ra);
+              round4(w[b][2 * cc + 1], scale2[2 * b + 1], zero_lo[2 * b + 1], zero_hi[2 * b + 1], rb);
+              mma16816(lo[b], ra[0], rb[0], ra[2], rb[2], xv.x, xv.y, c == 0);
+              mma16816(hi[b], ra[1], rb[1], ra[3], rb[3], xv.z, xv.w, c == 0);
+              if (c == 7) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[b][i] += lo[b][i] + hi[b][i];
+              }
+            }
+            continue;
+          }
           const bool first = c % kPass == 0;
 #pragma unroll
           for (int b = 0; b < kBlk; ++b) {
@@ -428,8 +474,8 @@ int columns(int M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
 // One tile height for all CTAs, so that a box is exactly what its team works on: N / SMs rows per CTA in equal tiles of at most
 // 32.  Larger teams share a tile's K extent among more warps, smaller ones pay the end of a tile (sums through shared memory, a
 // barrier) less often per box: as many teams as keep the number of 16-row blocks within 15 % of the least.
-bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
-  const int kM = columns(a.M), group_chunks = a.group / 32, pass = std::max(8 / kM, group_chunks), passes = 8 / pass;
+bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out, bool rounded = false) {
+  const int kM = rounded ? 8 : columns(a.M), group_chunks = a.group / 32, pass = std::max(8 / kM, group_chunks), passes = 8 / pass;
   const int target = (a.N + sms - 1) / sms, groups = (a.K + a.group - 1) / a.group;
   const bool copied = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
   for (const int most : {kTileRows, 16}) {  // tiles of 16 where those of 32 leave no room for two boxes per warp
@@ -442,7 +488,6 @@ bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
     };
     const int least = std::min(tile(1), std::min(tile(2), tile(4)));
     if (tile(4) * 100 > least * 115 && tile(2) * 100 > least * 115) tile(1);
-    if (getenv("RK_TEAMS")) tile(atoi(getenv("RK_TEAMS")));
     p.grid = (a.N + p.teams * p.tiles * p.h - 1) / (p.teams * p.tiles * p.h);
     p.boxes = (a.K + kBoxWeights - 1) / kBoxWeights;
     p.copied = copied;
@@ -465,24 +510,24 @@ bool plan_matvec(const W4GroupArgs& a, int sms, MatvecPlan* out) {
   return false;
 }
 
-template <int kM, int kShift, int kBlk, bool kCopied>
+template <int kM, int kShift, int kBlk, bool kCopied, bool kRounded>
 int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
-  const auto kernel = w4_matvec_kernel<kM, kShift, kBlk, kCopied>;
+  const auto kernel = w4_matvec_kernel<kM, kShift, kBlk, kCopied, kRounded>;
   RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemLimit)));
   RK_CUDA(launch_pdl(kernel, dim3(p.grid), dim3(kThreads), p.smem, stream, maps, a, p, timeout_word_or_null()));
   RK_LAUNCH_CHECK("linear_w4a16_group launch");
   return kOk;
 }
-template <int kM, int kShift>
+template <int kM, int kShift, bool kRounded>
 int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
-  if (p.copied) return p.h > 16 ? launch_matvec<kM, kShift, 2, true>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, true>(stream, maps, a, p);
-  return p.h > 16 ? launch_matvec<kM, kShift, 2, false>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, false>(stream, maps, a, p);
+  if (p.copied) return p.h > 16 ? launch_matvec<kM, kShift, 2, true, kRounded>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, true, kRounded>(stream, maps, a, p);
+  return p.h > 16 ? launch_matvec<kM, kShift, 2, false, kRounded>(stream, maps, a, p) : launch_matvec<kM, kShift, 1, false, kRounded>(stream, maps, a, p);
 }
-template <int kM>
+template <int kM, bool kRounded = false>
 int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs& a, const MatvecPlan& p) {
-  if (a.group == 32) return launch_matvec<kM, 5>(stream, maps, a, p);
-  if (a.group == 64) return launch_matvec<kM, 6>(stream, maps, a, p);
-  return launch_matvec<kM, 7>(stream, maps, a, p);
+  if (a.group == 32) return launch_matvec<kM, 5, kRounded>(stream, maps, a, p);
+  if (a.group == 64) return launch_matvec<kM, 6, kRounded>(stream, maps, a, p);
+  return launch_matvec<kM, 7, kRounded>(stream, maps, a, p);
 }
 
 int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t row_bytes, int elem_bytes, int rows, int box_cols, int box_rows,
@@ -497,7 +542,7 @@ int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t 
   return kOk;
 }
 
-int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
+int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p, bool rounded = false) {
   MatvecMaps maps;
   int s = encode(&maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, a.K / 2, 1, a.N, 128, p.h, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != kOk) return s;
@@ -507,6 +552,7 @@ int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
     if ((s = encode(&maps.scale, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.scale, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
     if (a.zero && (s = encode(&maps.zero, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.zero, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
   }
+  if (rounded) return launch_matvec<8, true>(stream, maps, a, p);
   switch (columns(a.M)) {
     case 1: return launch_matvec<1>(stream, maps, a, p);
     case 2: return launch_matvec<2>(stream, maps, a, p);
@@ -516,6 +562,17 @@ int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p) {
 }
 
 }  // namespace
+
+bool w4_rounded_fits(const W4GroupArgs& a, int sms) {
+  MatvecPlan p;
+  return a.M <= kMaxRows && plan_matvec(a, sms, &p, true);
+}
+
+int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
+  MatvecPlan p;
+  RK_REQUIRE(a.M > 0 && a.M <= kMaxRows && plan_matvec(a, sms, &p, true), kShape, "4-bit product: unsupported shape");
+  return matvec(stream, a, p, true);
+}
 
 // Planes of fp32 partial sums that let the tensor-core kernel deal its 128-channel tiles out twice over to the SMs.
 size_t w4_group_workspace(int M, int K, int N) {
@@ -535,8 +592,7 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, 
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
-  const int cut = getenv("RK_CUT") ? atoi(getenv("RK_CUT")) : 16;
-  if (a.M > cut) {
+  if (a.M > kMatvecRows) {
     LinearArgs l;
     l.M = a.M; l.K = a.K; l.N = a.N; l.x = a.x; l.w = a.q; l.fmt = 2; l.scale = a.scale; l.zero = a.zero;
     l.grouped = true; l.group = a.group; l.epi = a.epi; l.y = a.y;
