@@ -2,15 +2,18 @@
 // likeliest alternatives of every row (definitions and corner cases: logprob.cuh).
 //
 // Bound by reading the logits once; a single row by latency.  A row goes to one CTA, or to the CTAs of a cluster when
-// there are too few rows to fill the GPU: each takes a contiguous part, and the first one merges the others' statistics
-// and alternatives out of their shared memory, so there is no scratch, no second launch and no atomic whose order could show.
-// A thread keeps 16 logits in registers and the next 16 under way, and its own running maximum (one rescaling per 16).
+// there are too few rows to fill the GPU: each takes a contiguous part and leaves its statistics and alternatives in the
+// first one's shared memory, so there is no scratch, no second launch and no atomic whose order could show.
+// A thread keeps 16 logits in registers and the next 16 under way, and its own running maximum (one rescaling per 16).  At the HBM's
+// rate an SM has 2 issue slots per fp16 logit and 4 per fp32 one, so what a logit costs counts: half a maximum and half a
+// minimum (three operands at a time), and one multiply-add, one exp2, an addition and a multiply-add for its part of the sums.
 //
-// Alternatives without a second pass: after the first 16 logits per thread the k-th largest of the maxima of disjoint groups
-// of four threads is a lower bound of the k-th largest logit; whatever reaches it goes to a list in shared memory.  The
-// bound is raised after 2, 4 and 8 steps, so some 5 k of the logits are ever listed, and the list is put in order by
-// counting, for every entry, the larger ones.  A row that fills the list (thousands of equal logits, rows sorted upwards)
-// takes k passes over its part instead.
+// Alternatives without a pass over the rest: the k-th largest of the maxima of 64 disjoint groups of threads is a lower
+// bound of the k-th largest logit, and only about k logits reach it.  Every thread has left the maxima of 16 stretches
+// of its logits in shared memory, so the few stretches that reach the bound are known; they are loaded again (out of the
+// L2, one vector per thread, all at once), what reaches the bound is listed, and the list is put in order by counting,
+// for every entry, the larger ones.  A row with too many such stretches or logits (thousands of equal ones) takes k
+// passes over its part instead.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -26,8 +29,9 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kCtasPerSm = 4;
-constexpr int kGroups = kThreads / 4;  // groups of four lanes whose maxima bound the k-th largest logit
-constexpr int kList = 1536;            // candidates a part can list
+constexpr int kGroups = 64;            // groups of neighbouring threads whose maxima bound the k-th largest logit
+constexpr int kList = 512;             // candidates a part can list
+constexpr int kStretches = 16;
 constexpr int kMaxParts = 8;           // portable cluster size
 
 using Key = unsigned long long;
@@ -77,10 +81,10 @@ __device__ __forceinline__ uint4 nothing() {  // a vector of -inf
   const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xfc00fc00u;
   return make_uint4(w, w, w, w);
 }
-__device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
+__device__ __forceinline__ void unpack(const uint4& q, float* v, float) {
   v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
 }
-__device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+__device__ __forceinline__ void unpack(const uint4& q, float* v, half) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -91,25 +95,105 @@ __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(half v) { return __half2float(v); }
 
-struct Shared {
-  SoftStats stats[kWarps];
-  float groups[kGroups];
-  float bound[2];                        // of this refresh and the one before (threads may still read that)
-  int count;
-  Key best[kWarps];
-  Key top[kMaxTopLogprobs];              // this part's alternatives, best first, 0: none
-  Key list[kList];
-  Key merged[kMaxParts * kMaxTopLogprobs];
-  RowResult result;
-};
+// Three operands, NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The largest (NaN if there is one) and the smallest of a step's logits.
+template <int kVecs>
+__device__ __forceinline__ void extremes(const uint4 (&q)[kVecs], float* hi, float* lo, float) {
+  float a = __uint_as_float(q[0].x), b = a;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const float x = __uint_as_float(q[j].x), y = __uint_as_float(q[j].y), z = __uint_as_float(q[j].z), w = __uint_as_float(q[j].w);
+    a = max3_nan(max3_nan(a, x, y), z, w);
+    b = min3(min3(b, x, y), z, w);
+  }
+  *hi = a;
+  *lo = b;
+}
+template <int kVecs>
+__device__ __forceinline__ void extremes(const uint4 (&q)[kVecs], float* hi, float* lo, half) {
+  __half2 a = *reinterpret_cast<const __half2*>(&q[0].x), b = a;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a = __hmax2_nan(a, *reinterpret_cast<const __half2*>(&w[i]));
+      b = __hmin2(b, *reinterpret_cast<const __half2*>(&w[i]));
+    }
+  }
+  const float2 x = __half22float2(a), y = __half22float2(b);
+  *hi = max_nan(x.x, x.y);
+  *lo = fminf(y.x, y.y);
+}
 
-// The k largest of n distinct keys (0: no key), in order.
-__device__ __forceinline__ void order(const Key* keys, int n, int k, Key* out) {
+// A step's 16 logits at the maximum that is in place.  2^((z - m) log2 e) as 2^(y - r) with y = z log2 e - M, M = fl(m log2 e)
+// and r = m log2 e - M, each one rounding of an exact product: r is the same for all and comes off the sums.  Needs
+// products that do not overflow; the other rows (masked tokens among them) go logit by logit.
+__device__ __forceinline__ void add_step(SoftStats& st, const float* v, float lo) {
+  if (lo >= -1e38f && fabsf(st.m) <= 1e38f) {
+    const float M = st.m * kLog2e, r = fmaf(st.m, kLog2e, -M);
+    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float y0 = fmaf(v[i], kLog2e, -M), y1 = fmaf(v[i + 1], kLog2e, -M);
+      const float e0 = exp2f(y0), e1 = exp2f(y1);
+      s0 += e0;
+      s1 += e1;
+      t0 = fmaf(e0, y0, t0);
+      t1 = fmaf(e1, y1, t1);
+    }
+    const float f = exp2f(-r), sum = s0 + s1;
+    st.s = fmaf(f, sum, st.s);
+    st.t = fmaf(f * 0.6931471805599453f, fmaf(-r, sum, t0 + t1), st.t);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) add(st, v[i]);
+  }
+}
+
+constexpr int kHits = 256;
+
+struct Stats {  // SoftStats without its initial values
+  float m, s, t;
+};
+struct Shared {
+  Stats stats[kWarps];
+  Stats parts[kMaxParts];  // of the first part: all parts' statistics and alternatives
+  alignas(16) Key part_top[kMaxParts * kMaxTopLogprobs + 2];
+  alignas(16) float groups[kGroups];
+  float bound;
+  int count, hits;
+  Key best[kWarps];
+  Key top[kMaxTopLogprobs];  // this part's alternatives, best first, 0: none
+  Key merged[kMaxTopLogprobs];
+  alignas(16) Key list[kList + 2];
+  unsigned short hit[kHits];  // stretches that reach the bound: stretch * kThreads + thread
+  float stretch[1];           // [kStretches][threads]: the largest logit of each stretch of a thread's steps
+};
+__host__ __device__ constexpr size_t shared_bytes(int threads) { return sizeof(Shared) + sizeof(float) * kStretches * threads; }
+
+// The k largest of n distinct keys (0: no key), in order; keys[n] and keys[n + 1] are overwritten.
+__device__ __forceinline__ void order(Key* keys, int n, int k, Key* out) {
+  if (threadIdx.x < 2) keys[n + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
     const Key mine = keys[i];
     int larger = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) larger += keys[j] > mine ? 1 : 0;
+    for (int j = 0; j < n; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(keys + j);
+      larger += (two.x > mine ? 1 : 0) + (two.y > mine ? 1 : 0);
+    }
     if (mine != 0 && larger < k) out[larger] = mine;
   }
 }
@@ -117,9 +201,11 @@ __device__ __forceinline__ void order(const Key* keys, int n, int k, Key* out) {
 template <typename T, bool kTop>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(const TokenLogprobsArgs a, const int parts) {
   constexpr int kVec = RowView<T>::kVec, kVecs = 16 / kVec;  // 16 logits per thread and step
-  __shared__ Shared s;
+  extern __shared__ __align__(16) unsigned char shared_mem[];
+  Shared& s = *reinterpret_cast<Shared*>(shared_mem);
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31, threads = blockDim.x;
   const int r = blockIdx.x / parts, part = blockIdx.x - r * parts;
+  if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has begun: waited for before it is written to
   pdl_wait();
   pdl_trigger();
   const RowView<T> row(static_cast<const T*>(a.logits) + static_cast<long long>(r) * a.ld, a.V);
@@ -142,68 +228,100 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(co
     if (id >= 0 && id < a.V) given = to_float(row.z[id]);
   }
   if (kTop) {
-    if (t == 0) s.count = 0;
+    if (t == 0) s.count = s.hits = 0;
     if (t < a.top_k) s.top[t] = 0;
   }
 
   SoftStats st;
-  float bound = -INFINITY;
-  int refresh = 0;
-  for (int i = 0; i < steps; ++i) {
-    uint4 q[kVecs];
+  const int stretch = (steps + kStretches - 1) / kStretches;  // in steps
+  float highest = -INFINITY;
+  uint4 q[kVecs];
+  for (int i = 0, in = 0, at = 0; i < steps; ++i) {
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) q[j] = next[j];
     if (i + 1 < steps) fetch(i + 1, next);
-    float v[kVecs][kVec];
-    float m = st.m, here = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < kVecs; ++j) {
-      unpack(q[j], v[j]);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) here = max_nan(here, v[j][e]);
-    }
-    m = max_nan(m, here);
+    float hi, lo;
+    extremes(q, &hi, &lo, T(0));
+    const float m = max_nan(st.m, hi);
     if (m != st.m) raise(st, m);
+    float v[16];
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) add(st, v[j][e]);
+    for (int j = 0; j < kVecs; ++j) unpack(q[j], v + j * kVec, T(0));
+    add_step(st, v, lo);
     if (kTop) {
-      if ((i & (i + 1)) == 0 && i < 8) {  // steps 0, 1, 3, 7: the bound
-        float g = fmaxf(st.m, __shfl_xor_sync(0xffffffffu, st.m, 1));
-        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if ((lane & 3) == 0) s.groups[t >> 2] = g;
-        refresh ^= 1;
-        if (t == 0) s.bound[refresh] = -INFINITY;
-        __syncthreads();
-        const int n = threads >> 2;
-        if (t < n) {
-          const float mine = s.groups[t];
-          int before = 0;
-          for (int j = 0; j < n; ++j) before += s.groups[j] > mine || (s.groups[j] == mine && j < t) ? 1 : 0;
-          if (before == a.top_k - 1) s.bound[refresh] = mine > -FLT_MAX ? mine : -INFINITY;  // (-FLT_MAX: a group with nothing but masked tokens)
-        }
-        __syncthreads();
-        bound = s.bound[refresh];
-      }
-      if (here >= bound && here > -INFINITY) {
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            if (v[j][e] >= bound && v[j][e] > -INFINITY) {
-              const int slot = atomicAdd(&s.count, 1);
-              if (slot < kList) s.list[slot] = rank_key(v[j][e], row.column(begin + i * step + j * threads + t) + e);
-            }
+      highest = in == 0 ? hi : fmaxf(highest, hi);
+      if (++in == stretch || i + 1 == steps) {
+        s.stretch[at++ * threads + t] = highest;
+        in = 0;
       }
     }
   }
+  const float mine = st.m;  // this thread's largest logit, -FLT_MAX if it has none that counts
   st = warp_merge(st);
-  if (lane == 0) s.stats[warp] = st;
+  if (lane == 0) s.stats[warp] = Stats{st.m, st.s, st.t};
   __syncthreads();
   if (kTop) {
+    // the bound: -inf when there are fewer groups with a logit than alternatives
+    const int share = threads > kGroups ? threads / kGroups : 1;  // threads to a group: 1, 2 or 4
+    float g = mine;
+    if (share > 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 1));
+    if (share > 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    if ((t & (share - 1)) == 0) s.groups[t / share] = g;
+    if (threads < kGroups) s.groups[t + threads] = -FLT_MAX;  // what one warp lacks
+    __syncthreads();
+    for (int j = t >> 2; j < kGroups; j += threads >> 2) {  // four threads count a quarter each of what is before group j
+      const float largest = s.groups[j];
+      int before = 0;
+#pragma unroll
+      for (int e = 0; e < kGroups / 4; ++e) {
+        const int o = 4 * e + (lane & 3);
+        const float other = s.groups[o];
+        before += other > largest || (other == largest && o < j) ? 1 : 0;
+      }
+      before += __shfl_xor_sync(0xffffffffu, before, 1);
+      before += __shfl_xor_sync(0xffffffffu, before, 2);
+      if ((lane & 3) == 0 && before == a.top_k - 1) s.bound = largest > -FLT_MAX ? largest : -INFINITY;
+    }
+    __syncthreads();
+    const float bound = s.bound;
+    auto list = [&](const float (&v)[kVec], int vec) {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (v[e] >= bound && v[e] > -INFINITY) {
+          const int slot = atomicAdd(&s.count, 1);
+          if (slot < kList) s.list[slot] = rank_key(v[e], row.column(vec) + e);
+        }
+    };
+    if (steps == 1) {  // short rows: the logits are still here
+      if (mine >= bound) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j) {
+          float v[kVec];
+          unpack(q[j], v, T(0));
+          list(v, begin + j * threads + t);
+        }
+      }
+    } else if (mine >= bound) {
+      for (int w = 0; w * stretch < steps; ++w) {
+        const float high = s.stretch[w * threads + t];
+        if (high < bound || !(high > -INFINITY)) continue;
+        const int slot = atomicAdd(&s.hits, 1);
+        if (slot < kHits) s.hit[slot] = static_cast<unsigned short>(w * kThreads + t);
+      }
+    }
+    __syncthreads();
+    const int hits = s.hits, vectors = stretch * kVecs;
+    for (int i = t; i < min(hits, kHits) * vectors; i += threads) {
+      const int hit = s.hit[i / vectors], of = i % vectors;
+      const int vec = begin + (hit / kThreads * stretch + of / kVecs) * step + of % kVecs * threads + hit % kThreads;
+      if (vec >= end) continue;
+      float v[kVec];
+      unpack(row.load(vec), v, T(0));
+      list(v, vec);
+    }
+    __syncthreads();
     const int count = s.count;
-    if (count <= kList) {
+    if (hits <= kHits && count <= kList) {
       order(s.list, count, a.top_k, s.top);
     } else {  // (the same in all threads) one pass per alternative: the largest key below the one before
       Key last = ~0ull;
@@ -211,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(co
         Key best = 0;
         for (int vec = begin + t; vec < end; vec += threads) {
           float v[kVec];
-          unpack(row.load(vec), v);
+          unpack(row.load(vec), v, T(0));
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
             const Key key = v[e] > -INFINITY ? rank_key(v[e], row.column(vec) + e) : 0;
@@ -232,37 +350,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(co
       }
     }
   }
-  const int warps = threads >> 5;
+  // Every warp merges this part's statistics; with several parts they and the alternatives go to the first one.
+  auto merged = [&](const Stats* of, int n) {
+    SoftStats b;
+    if (lane < n) { b.m = of[lane].m; b.s = of[lane].s; b.t = of[lane].t; }
+    return warp_merge(b);
+  };
+  SoftStats all = merged(s.stats, threads >> 5);
   const Key* top = s.top;
   if (parts > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    if (part == 0) {
-      if (warp == 0) {
-        SoftStats all;
-        for (int i = lane; i < parts * warps; i += 32) all = merge(all, cluster.map_shared_rank(s.stats, i / warps)[i % warps]);
-        all = warp_merge(all);
-        if (lane == 0) s.result = finish(all);
-      }
-      if (kTop) {
-        const int n = parts * a.top_k;
-        for (int i = t; i < n; i += threads) s.list[i] = cluster.map_shared_rank(s.top, i / a.top_k)[i % a.top_k];
-        if (t < a.top_k) s.merged[t] = 0;
-        __syncthreads();
-        order(s.list, n, a.top_k, s.merged);
-        top = s.merged;
-      }
+    Shared* first = cluster.map_shared_rank(&s, 0);
+    if (t == 0) first->parts[part] = Stats{all.m, all.s, all.t};
+    if (kTop) {
+      __syncthreads();
+      if (t < a.top_k) first->part_top[part * a.top_k + t] = s.top[t];
     }
-    cluster.sync();  // the others' shared memory has been read
+    cluster.sync();
     if (part != 0) return;
-  } else if (warp == 0) {
-    SoftStats all;
-    if (lane < warps) all = s.stats[lane];
-    all = warp_merge(all);
-    if (lane == 0) s.result = finish(all);
+    all = merged(s.parts, parts);
+    if (kTop) {
+      if (t < a.top_k) s.merged[t] = 0;
+      order(s.part_top, parts * a.top_k, a.top_k, s.merged);
+      top = s.merged;
+    }
   }
-  __syncthreads();
-  const RowResult res = s.result;
+  if (kTop) __syncthreads();
+  const RowResult res = finish(all);
   if (t == 0) {
     if (a.entropy) a.entropy[r] = res.entropy;
     if (a.lse) a.lse[r] = res.lse;
@@ -282,16 +397,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(co
 
 template <typename T>
 int launch(cudaStream_t stream, const TokenLogprobsArgs& a, int sms) {
-  // One CTA per row while that fills the GPU; with fewer rows, the largest cluster that leaves a thread its 16 logits and
-  // all parts resident at once.
-  const long long slots = static_cast<long long>(sms) * kCtasPerSm;
+  // Several CTAs to a row while that leaves them a thread 16 logits and about two to an SM (clusters are not placed as densely
+  // as single CTAs, and each row ends in a microsecond or two of merging).  Measured with 65536 fp32 logits and five alternatives,
+  // 1 / 2 / 4 / 8 parts: 148 rows 19.0 / 15.0 / 19.5 / 22.7 us, 64 rows 17.9 / 12.5 / 9.9 / 11.0, 32 rows 17.5 / 12.0 / 8.8 / 7.8;
+  // 256 rows and 20 alternatives 21.9 / 20.5 / 26.2 / 38.5.
   int parts = 1;
-  while (parts < kMaxParts && 2 * parts * static_cast<long long>(a.rows) <= slots && a.V >= 2 * parts * kThreads * 16) parts *= 2;
+  while (parts < kMaxParts && 2LL * parts * a.rows <= (parts == 1 ? 4 : 11 * 0.25) * sms && a.V >= 2 * parts * kThreads * 16) parts *= 2;
+  // Blocks of 256 threads, or about as many as have 16 to 32 logits each; smaller ones where there are rows for every SM several
+  // times over, because every warp of a row's block takes part in the merging (3850 rows of 2475: 29.5 us with 256 threads or what
+  // they come to, 23.6 with 64; 4096 x 65536 fp16: 116 us with 256, 110 with 128).
   const int per = (a.V + parts - 1) / parts;
-  const int threads = std::min(kThreads, (per + 16 * 32 - 1) / (16 * 32) * 32);
+  int threads = 32;
+  while (threads < kThreads && threads * 24 < per) threads *= 2;
+  if (static_cast<long long>(a.rows) * parts >= 4LL * sms) threads = std::min(threads, a.V <= 4096 ? 64 : 128);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * parts);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared_bytes(threads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
