@@ -66,9 +66,8 @@ struct Prob {
   void* y;
   const half* scale;         // optional per-output-channel factor applied to the accumulator
   int fmt;                   // weight format of this product (0 fp16, 1 W8A16, 2 W4A16)
-  const half* qscale;        // W4A16: [N, groups] group scales and zeros (no zeros: 8)
+  const half* qscale;        // W4A16: [N, K/128] group scales and zeros
   const half* qzero;
-  int gshift, groups;        // log2 of the group, groups per weight row
   const half* v;             // kEpiVres
   const half* v_first;
   const half* v0;
@@ -231,17 +230,6 @@ __device__ __forceinline__ void store4(const EpiCtx& p, int m, int n, const floa
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = epi_value(p, o + i, n + i, a[i]);
     store_half4(static_cast<half*>(p.y), o, e[0], e[1], e[2], e[3]);
-  }
-}
-
-// The same for rows that are no multiple of four channels long: one channel at a time, up to the last one.
-__device__ __forceinline__ void store_ragged(const EpiCtx& p, int m, int n, const float (&a)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= p.N) return;
-    const size_t o = static_cast<size_t>(m) * p.N + n + i;
-    if (p.epi == kEpiF32) static_cast<float*>(p.y)[o] = __half2float(__float2half_rn(a[i]));
-    else static_cast<half*>(p.y)[o] = __float2half_rn(epi_value(p, o, n + i, a[i]));
   }
 }
 
@@ -453,27 +441,18 @@ __global__ void __launch_bounds__(kThreads + (kQuant ? kDequantThreads : 0), 1)
     for (int ui = first_unit; ui < g.total_units && ok && !failed; ui += unit_stride) {
       const Unit u = decode_unit(g, ui);
       const Prob& p = g.prob[u.prob];
-      const int fmt = p.fmt, row = u.n0 + r;
+      const int fmt = p.fmt, row = u.n0 + r, groups = p.K >> 7;
       for (int kb = 0; kb < u.kblocks; ++kb, ++it) {
         const int s = it % g.stages;
         const bool mine = (it & 1) == my_parity;
-        __half2 sc2[2], add2[2];  // of the K block's two runs of 32 weights
-        sc2[0] = sc2[1] = add2[0] = add2[1] = __floats2half2_rn(0.f, 0.f);
+        __half2 sc2 = __floats2half2_rn(0.f, 0.f), add2 = sc2;
         if (mine && fmt == 2 && row < p.N) {  // this K block's group parameters, requested before the wait for the tile
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c == 1 && p.gshift > 5) {  // both runs are in one group
-              sc2[1] = sc2[0];
-              add2[1] = add2[0];
-              break;
-            }
-            const size_t gi = static_cast<size_t>(row) * p.groups + min(((u.kb_begin + kb) * kBK + 32 * c) >> p.gshift, p.groups - 1);
-            const half sc = p.qscale[gi];
-            const float z = p.qzero ? __half2float(p.qzero[gi]) : 8.f;
-            sc2[c] = __half2half2(sc);
-            // low nibble: (1024 + q) - (1024 + z); high nibble arrives as 1024 + 16 q: / 16 - (64 + z)
-            add2[c] = __halves2half2(__hneg(__float2half_rn(1024.f + z)), __hneg(__float2half_rn(64.f + z)));
-          }
+          const size_t gi = static_cast<size_t>(row) * groups + (((u.kb_begin + kb) * kBK) >> 7);
+          const half sc = p.qscale[gi];
+          const float z = __half2float(p.qzero[gi]);
+          sc2 = __half2half2(sc);
+          // low nibble: (1024 + q) - (1024 + z); high nibble arrives as 1024 + 16 q: / 16 - (64 + z)
+          add2 = __halves2half2(__hneg(__float2half_rn(1024.f + z)), __hneg(__float2half_rn(64.f + z)));
         }
         ok = mbar_wait(smem_u32(&full_bar[s]), (it / g.stages) & 1);
         // Every thread watches EVERY fill of every stage, also those the other group expands: a waiter that skipped a
@@ -523,7 +502,7 @@ __global__ void __launch_bounds__(kThreads + (kQuant ? kDequantThreads : 0), 1)
                 for (int b = 0; b < 4; ++b) {
                   const uint32_t both = __byte_perm(w[i], 0u, 0x4040u + 0x0101u * b);  // the byte in both halves
                   uint32_t pair = (both & 0x00f0000fu) | 0x64006400u;                  // (1024 + lo, 1024 + 16 hi)
-                  const __half2 v = __hmul2(__hfma2(*reinterpret_cast<__half2*>(&pair), mul, add2[c]), sc2[c]);
+                  const __half2 v = __hmul2(__hfma2(*reinterpret_cast<__half2*>(&pair), mul, add2), sc2);
                   h[b] = *reinterpret_cast<const uint32_t*>(&v);
                 }
                 dst[(4 * c + i) ^ (r & 7)] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -597,9 +576,6 @@ __global__ void __launch_bounds__(kThreads + (kQuant ? kDequantThreads : 0), 1)
             const size_t o = o_first + static_cast<size_t>((kEpiThreads / 32) * i) * p.N;
             if (p.splits > 1) {
               *reinterpret_cast<float4*>(p.partial + static_cast<size_t>(u.split) * p.M * p.N + o) = a4[i];
-            } else if (kQuant && (p.N & 3) != 0) {
-              const float a[4] = {a4[i].x, a4[i].y, a4[i].z, a4[i].w};
-              store_ragged(p, m_first + (kEpiThreads / 32) * i, n, a);
             } else if (p.epi == kEpiNone && !p.scale) {
               store_half4(static_cast<half*>(p.y), o, a4[i].x, a4[i].y, a4[i].z, a4[i].w);
             } else {
@@ -849,9 +825,8 @@ Plan make_plan_uncached(const LinearArgs* a, int n, size_t scratch_bytes, int sm
 bool problem_ok(const LinearArgs& a) {
   const int ldx = a.ldx ? a.ldx : a.K;
   if (a.fmt == 1 && (a.K % 16 != 0 || !a.scale)) return false;             // packed rows must be 16-byte multiples
-  if (a.fmt == 2 && (!a.scale || (a.grouped ? a.K % 32 != 0 : a.K % 128 != 0 || !a.zero))) return false;
-  return a.fmt >= 0 && a.fmt <= 2 && a.in_act == kActNone && a.K % 8 == 0 && ldx % 8 == 0 && a.M >= 2 &&
-         (a.N % 4 == 0 || (a.grouped && (a.epi == kEpiNone || a.epi == kEpiRelu2 || a.epi == kEpiF32))) &&
+  if (a.fmt == 2 && (a.K % 128 != 0 || !a.scale || !a.zero)) return false;
+  return a.fmt >= 0 && a.fmt <= 2 && a.in_act == kActNone && a.K % 8 == 0 && ldx % 8 == 0 && a.M >= 2 && a.N % 4 == 0 &&
          (reinterpret_cast<uintptr_t>(a.x) & 15u) == 0 && (reinterpret_cast<uintptr_t>(a.w) & 15u) == 0;
 }
 
@@ -941,8 +916,6 @@ int gemm_group(cudaStream_t stream, const LinearArgs* a, int n) {
     Prob& p = g.prob[i];
     p.M = a[i].M; p.N = a[i].N; p.K = a[i].K; p.epi = a[i].epi; p.y = a[i].y; p.scale = a[i].out_scale;
     p.fmt = a[i].fmt; p.qscale = a[i].scale; p.qzero = a[i].zero;
-    p.gshift = !a[i].grouped ? 7 : a[i].group == 32 ? 5 : a[i].group == 64 ? 6 : 7;
-    p.groups = (a[i].K + (1 << p.gshift) - 1) >> p.gshift;
     if (a[i].fmt == 1 && !p.scale) p.scale = a[i].scale;  // W8A16: one scale per output channel, applied to the accumulator
     p.v = a[i].ea.v; p.v_first = a[i].ea.v_first; p.v0 = a[i].ea.v0;
     p.tiles_n = (a[i].N + bm - 1) / bm;

@@ -4,375 +4,55 @@
 // where it is computed, and a second kernel merges a row's tiles (logprob.cuh).  fp16 operands, fp32 sums; int8 weights
 // are exact integers with the channel's scale on the sum, 4-bit weights half((q - zero) * scale).
 //
-// Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  One CTA per SM walks the units (128 rows x
-// up to 256 tokens), the row blocks of a token tile one after the other, so that neighbouring CTAs share a tile of weights
-// and it comes from HBM once.  The rows take the MMA's M side and the tokens its N side: a lane of tensor memory is then a row
-// of x, and an epilogue thread reduces its row's 256 logits without talking to any other.  Two accumulators, so that
-// a unit's epilogue runs under the next one's products.
-//
-// Warp roles: 0 loads (TMA, 128-byte swizzle), 1 issues tcgen05.mma, 2..5 reduce.  Quantised weights: warp 0 brings
-// packed tiles into a ring of their own, warp 6 the rows of x, and 16 more warps expand a packed tile into the swizzled
-// fp16 tile that the MMA reads (a thread to a weight row, the two halves of the warps taking turns).  Every wait is bounded: one that runs out sets the device's
-// failure word, every role leaves its loop, and the CTA frees its tensor memory and returns.
-#include <cuda.h>
-
+// Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  The product is tc_rows.cuh's; here are its
+// epilogue, which reduces a row's tokens in a thread's registers, the merging of the tiles, and the route for a few rows.
 #include <algorithm>
 
 #include "common.cuh"
 #include "kernels.h"
 #include "logprob.cuh"
-#include "tensormap.h"
+#include "tc_rows.cuh"
 
 namespace rk {
 namespace {
 
-constexpr int kRows = 128;   // rows of x per unit = MMA M
-constexpr int kToks = 256;   // tokens per unit = MMA N, at most (HeadShape::toks)
-constexpr int kMinToks = 128;
-constexpr int kBK = 64;      // halves per K block = one 128-byte swizzle row
-constexpr uint32_t kXBytes = kRows * 128, kWBytes = kToks * 128, kStageBytes = kXBytes + kWBytes;
-constexpr int kExpandWarps = 16;
-constexpr uint32_t kTmemCols = 512;
+constexpr int kMinToks = 128;  // the narrowest token tile
 
-// Stages of the tile ring and of the ring of packed tiles, bytes of a packed row and tile.
-template <int kFmt> struct Ring;
-template <> struct Ring<0> { static constexpr int tiles = 4, raws = 0, raw_row = 0, raw = 0; };
-template <> struct Ring<1> { static constexpr int tiles = 3, raws = 4, raw_row = kBK, raw = kToks * raw_row; };
-template <> struct Ring<2> { static constexpr int tiles = 3, raws = 8, raw_row = kBK / 2, raw = kToks * raw_row; };
-template <int kFmt> constexpr size_t smem_bytes() { return 1024 + Ring<kFmt>::tiles * kStageBytes + Ring<kFmt>::raws * Ring<kFmt>::raw; }
-template <int kFmt> constexpr int head_threads() { return kFmt == 0 ? 192 : 256 + kExpandWarps * 32; }
-
-struct HeadShape {
-  int toks, tiles;        // tokens per unit, token tiles
-  int row_blocks, units;  // blocks of 128 rows
-  int x_rows;             // rows of x that a block loads: all there are, in eights, up to 128 (the rest of the tile is not read out)
+// A row's tokens of a unit: m, s and t over them, and the given token's logit where it is among them.
+struct StatsEpilogue {
+  float4* part;   // [tiles][rows]
+  float* given;   // [rows]
+  const int64_t* tokens;
+  int n_rows, toks;
+  int r, n0;
+  int64_t id;
+  SoftStats st;
+  __device__ __forceinline__ int rows() const { return n_rows; }
+  __device__ __forceinline__ void begin(int row, int first, int, int) {
+    r = row;
+    n0 = first;
+    id = tokens ? tokens[row] : -1;
+    st = SoftStats();
+  }
+  __device__ __forceinline__ void chunk(int c, float (&z)[32], int here) {
+    if (here < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) z[i] = i < here ? z[i] : -INFINITY;
+    }
+    if (id >= n0 + c && id < n0 + c + here) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (id == n0 + c + i) given[r] = z[i];
+    }
+    float m = st.m;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) m = max_nan(m, z[i]);
+    raise(st, m);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) add(st, z[i]);
+  }
+  __device__ __forceinline__ void end() { part[static_cast<size_t>(n0 / toks) * n_rows + r] = make_float4(st.m, st.s, st.t, 0.f); }
 };
-
-struct HeadMaps {
-  CUtensorMap x, w;
-};
-
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
-}
-__device__ __forceinline__ void arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bounded wait: out of line after the first try, and over as soon as another role has given up.
-__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, const volatile int* failed) {
-  for (uint32_t i = 0; i < kSpinLimit && !*failed; ++i)
-    if (mbar_try_wait(bar, parity)) return true;
-  return false;
-}
-__device__ __forceinline__ uint4 lds16(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-// Shared-memory matrix descriptor: K-major tile, 128-byte swizzle, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Eight 4-bit codes to eight halves half((q - zero) * scale): a nibble under the exponent of 1024 is 1024 + q (the high ones
-// arrive as 1024 + 16 q), so one subtraction or fused multiply-add leaves q - zero exactly and the product rounds once.
-struct Group4 {
-  __half2 scale, sub;  // (s, s) and (-(1024 + z), -(64 + z))
-};
-__device__ __forceinline__ Group4 group4(uint32_t s2, uint32_t z2) {  // the group's scale and zero, twice each
-  return {*reinterpret_cast<const __half2*>(&s2), __hsub2(__floats2half2_rn(-1024.f, -64.f), *reinterpret_cast<const __half2*>(&z2))};
-}
-// Half i of eight, twice.
-__device__ __forceinline__ uint32_t pick(const uint4& v, int i) {
-  const uint32_t lo = i & 2 ? v.y : v.x, hi = i & 2 ? v.w : v.z;
-  return __byte_perm(i & 4 ? hi : lo, 0u, i & 1 ? 0x3232 : 0x1010);
-}
-__device__ __forceinline__ uint4 expand4(uint32_t w, const Group4& g) {
-  const __half2 mul = __floats2half2_rn(1.0f, 0.0625f);
-  uint32_t h[4];
-#pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    const uint32_t both = __byte_perm(w, 0u, 0x4040u + 0x0101u * b);  // the byte in both halves
-    uint32_t pair = (both & 0x00f0000fu) | 0x64006400u;
-    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<__half2*>(&pair), mul, g.sub), g.scale);
-    h[b] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-  return make_uint4(h[0], h[1], h[2], h[3]);
-}
-// Four int8 codes to four halves, exactly: code + 128 under the exponent of 1024, less 1152.
-__device__ __forceinline__ uint2 expand8(uint32_t w) {
-  const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
-  const uint32_t t = w ^ 0x80808080u;
-  uint32_t lo = __byte_perm(t, 0x64646464u, 0x4140), hi = __byte_perm(t, 0x64646464u, 0x4342);
-  const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), bias), b = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
-
-template <int kFmt>
-__global__ void __launch_bounds__(head_threads<kFmt>(), 1)
-    head_tc_kernel(const __grid_constant__ HeadMaps maps, const HeadLogprobsArgs a, const HeadShape h, int* timeout) {
-  constexpr int kTiles = Ring<kFmt>::tiles, kRaws = Ring<kFmt>::raws > 0 ? Ring<kFmt>::raws : 1;
-  extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kTiles], ready[kTiles], empty[kTiles], raw_full[kRaws], raw_empty[kRaws], acc_full[2], acc_empty[2];
-  __shared__ float scales[kToks];
-  __shared__ uint32_t tmem_slot;
-  __shared__ volatile int failed;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + kTiles * kStageBytes;
-  const int kblocks = (a.K + kBK - 1) / kBK;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kTiles; ++i) {
-      mbar_init(smem_u32(&full[i]), 1);
-      mbar_init(smem_u32(&ready[i]), kExpandWarps / 2);
-      mbar_init(smem_u32(&empty[i]), 1);
-    }
-    for (int i = 0; i < kRaws; ++i) {
-      mbar_init(smem_u32(&raw_full[i]), 1);
-      mbar_init(smem_u32(&raw_empty[i]), kExpandWarps / 2);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&acc_full[i]), 1);
-      mbar_init(smem_u32(&acc_empty[i]), 4);
-    }
-    failed = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_slot;
-  pdl_wait();
-  pdl_trigger();
-
-  auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
-  bool ok = true;
-  if (warp == 0 || (kFmt != 0 && warp == 6)) {
-    // ---- loads: the fp16 tiles of both operands, or the packed weights (warp 0) and the rows (warp 6) on rings of their own
-    if (lane == 0) {
-      const bool packed = kFmt != 0 && warp == 0;
-      const int stages = packed ? kRaws : kTiles;
-      int it = 0;
-      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
-        const int r0 = (u % h.row_blocks) * kRows, n0 = (u / h.row_blocks) * h.toks;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % stages;
-          if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], (it / stages - 1) & 1))) break;
-          const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]), dst = ring + s * kStageBytes;
-          if (packed) {
-            mbar_expect_tx(bar, h.toks * Ring<kFmt>::raw_row);
-            tma_2d(raw_ring + s * Ring<kFmt>::raw, &maps.w, bar, kb * Ring<kFmt>::raw_row, n0);
-          } else {
-            mbar_expect_tx(bar, 128 * (h.x_rows + (kFmt == 0 ? h.toks : 0)));
-            tma_2d(dst, &maps.x, bar, kb * kBK, r0);
-            if (kFmt == 0) tma_2d(dst + kXBytes, &maps.w, bar, kb * kBK, n0);
-          }
-        }
-      }
-      if (!ok)  // leave no copy in flight behind
-        for (int i = it > stages ? it - stages : 0; i < it; ++i) mbar_wait(smem_u32(packed ? &raw_full[i % stages] : &full[i % stages]), (i / stages) & 1);
-    }
-  } else if (warp == 1) {
-    // ---- products: K blocks of 64 as four instructions into the unit's accumulator
-    if (lane == 0) {
-      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(h.toks >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
-      int it = 0, n = 0;
-      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
-        if (n >= 2 && !(ok = wait(acc_empty[n & 1], ((n >> 1) - 1) & 1))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t acc = tmem + (n & 1) * kToks;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % kTiles;
-          ok = wait(full[s], (it / kTiles) & 1) && (kFmt == 0 || wait(ready[s], (it / kTiles) & 1));
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t dx = tile_desc(ring + s * kStageBytes), dw = tile_desc(ring + s * kStageBytes + kXBytes);
-#pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4) mma(acc, dx + 2 * k4, dw + 2 * k4, idesc, (kb | k4) != 0);
-          commit(smem_u32(&empty[s]));
-        }
-        if (ok) commit(smem_u32(&acc_full[n & 1]));
-      }
-    }
-  } else if (warp < 6) {
-    // ---- reduction: a thread owns a row of x, its TMEM lane, and takes the unit's tokens 32 at a time
-    const int quad = warp & 3, t = threadIdx.x - 64;
-    int n = 0;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
-      const int r = (u % h.row_blocks) * kRows + quad * 32 + lane, n0 = (u / h.row_blocks) * h.toks, toks = min(h.toks, a.V - n0);
-      const int64_t id = a.tokens && r < a.rows ? a.tokens[r] : -1;
-      if (kFmt == 1) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the last unit's scales have been read
-        for (int i = t; i < kToks; i += 128) scales[i] = i < toks ? __half2float(a.scale[n0 + i]) : 0.f;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
-      ok = __all_sync(0xffffffffu, wait(acc_full[n & 1], (n >> 1) & 1));
-      if (kFmt == 1) {  // all four warps stay or leave together: they meet at the barriers above
-        uint32_t all;
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.and.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
-        ok = all != 0;
-      }
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      SoftStats st;
-      for (int c = 0; c < toks && r - lane < a.rows; c += 32) {  // (nothing to do for a warp beyond the last row)
-        float z[32];
-        tmem_ld32(tmem + (n & 1) * kToks + c + (static_cast<uint32_t>(quad * 32) << 16), z);
-        const int here = min(32, toks - c);
-        if (kFmt == 1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] *= scales[c + i];
-        }
-        if (here < 32) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = i < here ? z[i] : -INFINITY;
-        }
-        if (id >= n0 + c && id < n0 + c + here) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (id == n0 + c + i) a.given[r] = z[i];
-        }
-        float m = st.m;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) m = max_nan(m, z[i]);
-        raise(st, m);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) add(st, z[i]);
-      }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive(smem_u32(&acc_empty[n & 1]));
-      if (r < a.rows) a.part[static_cast<size_t>(u / h.row_blocks) * a.rows + r] = make_float4(st.m, st.s, st.t, 0.f);
-    }
-  } else if (kFmt != 0 && warp >= 8) {
-    // ---- expansion: a thread owns a row of the tile, 64 weights a K block; half of the warps take the even K blocks, half the odd
-    // ones.  Row r of the tile is 128 bytes at r * 128, its 16-byte chunk c at chunk position c ^ (r & 7); a packed row of 64 (32)
-    // bytes has its chunk c at c ^ (r / 2 & 3) (c ^ (r / 4 & 1)): the swizzles of 128-, 64- and 32-byte rows, so that no two
-    // lanes of a quarter warp meet in a bank.  (No barrier's phase is
-    // missed by taking every other K block: the packed ring is even, and of the three tiles of the other ring the one waited for
-    // is at most a phase ahead of the tile this thread waited for two blocks before.)
-    const int r = threadIdx.x & 255, turn = (threadIdx.x >> 8) - 1;
-    const uint32_t raw = raw_ring + r * Ring<kFmt>::raw_row, raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
-    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
-    uint32_t at[8];  // where the chunks of this row go, in the first stage
-#pragma unroll
-    for (int c = 0; c < 8; ++c) at[c] = ring + kXBytes + r * 128 + ((16 * c) ^ ((r & 7) << 4));
-    // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
-    // multiple of 16 bytes, group by group.
-    const bool eights = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
-    const uint16_t *sp = nullptr, *zp = nullptr;
-    constexpr uint32_t kEight = 0x48004800u;
-    uint4 sc = make_uint4(0u, 0u, 0u, 0u), ze = make_uint4(kEight, kEight, kEight, kEight), sc_next = sc, ze_next = ze;
-    auto load8 = [&](int block) {
-      if (block * 8 >= groups) return;
-      sc_next = reinterpret_cast<const uint4*>(sp)[block];
-      if (zp) ze_next = reinterpret_cast<const uint4*>(zp)[block];
-    };
-    auto load_runs = [&](int kb) {  // a K block's two runs of 32 weights into the first two halves
-      const int g0 = min((kb * kBK) >> shift, groups - 1), g1 = min((kb * kBK + 32) >> shift, groups - 1);
-      sc_next.x = sp[g0] | (static_cast<uint32_t>(sp[g1]) << 16);
-      if (zp) ze_next.x = zp[g0] | (static_cast<uint32_t>(zp[g1]) << 16);
-    };
-    int it = 0, rs = turn, raw_phase = 0, s = turn, tile_phase = 0;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
-      const int row = min((u / h.row_blocks) * h.toks + r, a.V - 1);
-      int kb = (it & 1) == turn ? 0 : 1;
-      int block = -1;
-      if (kFmt == 2 && kb < kblocks) {
-        sp = reinterpret_cast<const uint16_t*>(a.scale) + static_cast<size_t>(row) * groups;
-        if (a.zero) zp = reinterpret_cast<const uint16_t*>(a.zero) + static_cast<size_t>(row) * groups;
-        if (eights) load8((kb * kBK) >> (shift + 3));
-        else load_runs(kb);
-      }
-      for (; kb < kblocks; kb += 2) {
-        const bool first_round = it + kb < kTiles;
-        if (kFmt == 2 && (!eights || (kb * kBK) >> (shift + 3) != block)) {
-          sc = sc_next;
-          ze = ze_next;
-          block = (kb * kBK) >> (shift + 3);
-          if (eights) load8(block + 1);
-        }
-        ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase) && (first_round || wait(empty[s], tile_phase ^ 1)));
-        if (!ok) break;
-        if (r < h.toks) {
-          const uint32_t src = raw + rs * Ring<kFmt>::raw, stage = s * kStageBytes;
-          if (kFmt == 1) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint4 q = lds16(src + ((16 * c) ^ raw_swz));
-              const uint2 h0 = expand8(q.x), h1 = expand8(q.y), h2 = expand8(q.z), h3 = expand8(q.w);
-              sts16(at[2 * c] + stage, make_uint4(h0.x, h0.y, h1.x, h1.y));
-              sts16(at[2 * c + 1] + stage, make_uint4(h2.x, h2.y, h3.x, h3.y));
-            }
-          } else {
-            const uint4 q0 = lds16(src + raw_swz), q1 = lds16(src + (16 ^ raw_swz));
-            const uint32_t w[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
-              const Group4 g = group4(pick(sc, i), pick(ze, i));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sts16(at[4 * c + j] + stage, expand4(w[4 * c + j], g));
-            }
-          }
-        }
-        if (kFmt == 2 && !eights && kb + 2 < kblocks) load_runs(kb + 2);  // under way until this thread's next turn
-        // written through the generic proxy, read by the tensor core through the async one
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          arrive(smem_u32(&ready[s]));
-          arrive(smem_u32(&raw_empty[rs]));
-        }
-        rs += 2;
-        if (rs >= kRaws) { rs -= kRaws; raw_phase ^= 1; }
-        s += 2;
-        if (s >= kTiles) { s -= kTiles; tile_phase ^= 1; }
-      }
-      it += kblocks;
-    }
-  }
-  if (!ok) failed = 1;
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (threadIdx.x == 0 && failed && timeout) atomicOr(timeout, kTimeoutGemm);
-  __syncwarp();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-}
 
 // One CTA per row merges the row's tiles: a load or two per thread, all under way at once.
 constexpr int kMergeThreads = 256;
@@ -400,31 +80,19 @@ __global__ void __launch_bounds__(kMergeThreads) head_merge_kernel(HeadLogprobsA
   if (a.tokens) a.logprobs[r] = given_logprob(res, a.tokens[r], a.V, [&](int64_t) { return a.given[r]; });
 }
 
-// A 2-D tensor [rows, row_bytes / size of an element] in boxes of box_cols x box_rows, zeros outside.
-int head_map(CUtensorMap* map, CUtensorMapDataType type, int elem_bytes, const void* base, int rows, size_t cols, int box_cols, int box_rows, CUtensorMapSwizzle swizzle) {
-  const TensorMapEncodeFn fn = tensor_map_encode_fn();
-  RK_REQUIRE(fn, kCuda, "head_logprobs: cuTensorMapEncodeTiled is not available from this driver");
-  const cuuint64_t dims[2] = {cols, static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {cols * elem_bytes};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t elem[2] = {1, 1};
-  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "head_logprobs: cuTensorMapEncodeTiled failed with %d (rows=%d, columns=%zu)", static_cast<int>(r), rows, cols);
-  return kOk;
-}
-
 // The token tile that lets the units come out in the fewest full rounds over the SMs (65536 tokens in tiles of 256 are 1.7 rounds
 // of 148, in tiles of 224 two full ones); a unit is counted as its tokens and 32 more for its beginning and end.
-HeadShape head_shape(int rows, int V, int sms) {
-  HeadShape best = {};
+tc::Shape head_shape(int rows, int V, int K, int sms) {
+  tc::Shape best = {};
   long long least = -1;
-  for (int toks = kToks; toks >= kMinToks; toks -= 16) {
-    HeadShape h;
+  for (int toks = tc::kToks; toks >= kMinToks; toks -= 16) {
+    tc::Shape h;
     h.toks = toks;
     h.tiles = (V + toks - 1) / toks;
-    h.row_blocks = (rows + kRows - 1) / kRows;
-    h.x_rows = std::min(kRows, (rows + 7) & ~7);
+    h.row_blocks = (rows + tc::kRows - 1) / tc::kRows;
+    h.splits = 1;
+    h.kb_per_split = (K + tc::kBK - 1) / tc::kBK;
+    h.x_rows = std::min(tc::kRows, (rows + 7) & ~7);
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks, cost = (units + sms - 1) / sms * (toks + 32);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
     if (least < 0 || cost < least) { least = cost; best = h; }
@@ -433,18 +101,13 @@ HeadShape head_shape(int rows, int V, int sms) {
 }
 
 template <int kFmt>
-int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, const HeadShape& h, int sms) {
-  HeadMaps maps;
-  int s = head_map(&maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.x, a.rows, a.K, kBK, h.x_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, const tc::Shape& h, int sms) {
+  tc::Weights w;
+  w.V = a.V; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
+  StatsEpilogue epi;
+  epi.part = a.part; epi.given = a.given; epi.tokens = a.tokens; epi.n_rows = a.rows; epi.toks = h.toks;
+  const int s = tc::launch_rows<kFmt>(stream, "head_logprobs", a.x, a.rows, a.w, w, h, epi, sms);
   if (s != kOk) return s;
-  if (kFmt == 0) s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.w, a.V, a.K, kBK, h.toks, CU_TENSOR_MAP_SWIZZLE_128B);
-  else s = head_map(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.w, a.V, kFmt == 1 ? a.K : a.K / 2, Ring<kFmt>::raw_row, h.toks,
-                    kFmt == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
-  if (s != kOk) return s;
-  RK_CUDA(cudaFuncSetAttribute(head_tc_kernel<kFmt>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<kFmt>())));
-  RK_CUDA(launch_pdl(head_tc_kernel<kFmt>, dim3(std::min(h.units, sms)), dim3(head_threads<kFmt>()), smem_bytes<kFmt>(), stream, maps, a, h,
-                     timeout_word_or_null()));
-  RK_LAUNCH_CHECK("head_logprobs launch");
   RK_CUDA(launch_pdl(head_merge_kernel, dim3(a.rows), dim3(kMergeThreads), 0, stream, a, h.tiles));
   RK_LAUNCH_CHECK("head_logprobs merge launch");
   return kOk;
@@ -516,7 +179,7 @@ int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size
   const int status = device_sms(&sms);
   if (status != kOk) return status;
   if (few_rows(a, sms)) return logits_then_stats(stream, a, static_cast<float*>(workspace), sms);
-  const HeadShape h = head_shape(a.rows, a.V, sms);
+  const tc::Shape h = head_shape(a.rows, a.V, a.K, sms);
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
   a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
   if (a.fmt == 1) return launch_head<1>(stream, a, h, sms);

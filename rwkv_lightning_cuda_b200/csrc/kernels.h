@@ -155,8 +155,6 @@ struct LinearArgs {
   int fmt = 0;               // 0 fp16, 1 W8A16, 2 W4A16 (group 128)
   const half* scale = nullptr;  // W8: [N]; W4: [N,K/128]
   const half* zero = nullptr;   // W4: [N,K/128]
-  bool grouped = false;         // W4, tensor-core path: groups of `group` (32, 64, 128), any K % 32 == 0, zero may be nullptr (8)
-  int group = 128;
   int in_act = kActNone;
   int epi = kEpiNone;
   EpiArgs ea;
@@ -233,8 +231,6 @@ bool w4_rounded_fits(const W4GroupArgs& args, int sms);
 int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& args, int sms);
 size_t w4_group_workspace(int M, int K, int N);  // scratch that lets many rows split K over more SMs; 0: none is used
 int w4_group_linear(cudaStream_t stream, const W4GroupArgs& args, void* workspace, size_t workspace_bytes);
-bool gemm_tc_supported(const LinearArgs& args);         // gemm_tcgen05.cu
-int gemm_tc(cudaStream_t stream, const LinearArgs& args);
 int quant_pack_w4_group(cudaStream_t stream, int N, int K, int group, const half* W, uint8_t* q, half* scale, half* zero);
 int quant_unpack_w4_group(cudaStream_t stream, int N, int K, int group, const uint8_t* q, const half* scale, const half* zero, half* W);
 

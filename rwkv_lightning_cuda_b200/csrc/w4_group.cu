@@ -22,9 +22,11 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tc_rows.cuh"
 #include "tensormap.h"
 
 namespace rk {
@@ -90,18 +92,18 @@ __device__ __forceinline__ float half_of(uint32_t pair, int i) {
   const float2 f = h2f2(pair);
   return i ? f.y : f.x;
 }
+// What becomes of an fp32 sum; the store rounds to half where y is half.
+__device__ __forceinline__ float w4_epilogue(float v, int epi) {
+  if (epi == kEpiRawF32) return v;
+  const float h = __half2float(__float2half_rn(v));
+  if (epi != kEpiRelu2) return h;
+  const float u = fmaxf(h, 0.f);
+  return u * u;
+}
 __device__ __forceinline__ void store_epi(const W4GroupArgs& a, size_t o, float v) {
-  const half hy = __float2half_rn(v);
-  if (a.epi == kEpiRawF32) {
-    static_cast<float*>(a.y)[o] = v;
-  } else if (a.epi == kEpiF32) {
-    static_cast<float*>(a.y)[o] = __half2float(hy);
-  } else if (a.epi == kEpiRelu2) {
-    const float u = fmaxf(__half2float(hy), 0.f);
-    static_cast<half*>(a.y)[o] = __float2half_rn(u * u);
-  } else {
-    static_cast<half*>(a.y)[o] = hy;
-  }
+  const float e = w4_epilogue(v, a.epi);
+  if (a.epi == kEpiF32 || a.epi == kEpiRawF32) static_cast<float*>(a.y)[o] = e;
+  else static_cast<half*>(a.y)[o] = __float2half_rn(e);
 }
 
 // kM: columns per chunk, the rows of x rounded up to 1, 2, 4 or 8; kShift: log2 of the group.  A box is worked off in passes of
@@ -574,12 +576,127 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
   return matvec(stream, a, p, true);
 }
 
-// Planes of fp32 partial sums that let the tensor-core kernel deal its 128-channel tiles out twice over to the SMs.
+// ---- more rows: the tensor-core skeleton of tc_rows.cuh, weights rounded to half
+namespace {
+
+// A row's results of a unit to y, or to the unit's plane of partial sums.
+struct ProductEpilogue {
+  void* y;
+  float* partial;  // [splits][rows][N], or nullptr
+  int n_rows, N, epi;
+  size_t at;  // of the row's first result of the unit
+  float* plane;
+  __device__ __forceinline__ int rows() const { return n_rows; }
+  __device__ __forceinline__ void begin(int row, int n0, int, int split) {
+    at = static_cast<size_t>(row) * N + n0;
+    plane = partial ? partial + static_cast<size_t>(split) * n_rows * N : nullptr;
+  }
+  __device__ __forceinline__ void chunk(int c, float (&z)[32], int here) {
+    const size_t o = at + c;
+    if (plane) {  // (N is a multiple of four)
+#pragma unroll
+      for (int i = 0; i < 32; i += 4)
+        if (i < here) *reinterpret_cast<float4*>(plane + o + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) z[i] = w4_epilogue(z[i], epi);
+    if (epi == kEpiF32) {
+      float* y32 = static_cast<float*>(y) + o;
+      if (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          if (i < here) *reinterpret_cast<float4*>(y32 + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < here) y32[i] = z[i];
+      }
+      return;
+    }
+    half* y16 = static_cast<half*>(y) + o;
+    if (N % 8 == 0) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        if (i < here)
+          *reinterpret_cast<uint4*>(y16 + i) = make_uint4(h2u(__floats2half2_rn(z[i], z[i + 1])), h2u(__floats2half2_rn(z[i + 2], z[i + 3])),
+                                                          h2u(__floats2half2_rn(z[i + 4], z[i + 5])), h2u(__floats2half2_rn(z[i + 6], z[i + 7])));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (i < here) y16[i] = __float2half_rn(z[i]);
+    }
+  }
+  __device__ __forceinline__ void end() {}
+};
+
+// Adds the planes in order (the result does not depend on timing) and applies the epilogue: four channels per thread.
+__global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p, int splits) {
+  pdl_wait();
+  pdl_trigger();
+  const size_t total = static_cast<size_t>(p.n_rows) * p.N, i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (i >= total) return;
+  float4 v = *reinterpret_cast<const float4*>(p.partial + i);
+  for (int s = 1; s < splits; ++s) {
+    const float4 w = *reinterpret_cast<const float4*>(p.partial + s * total + i);
+    v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+  }
+  const float e[4] = {w4_epilogue(v.x, p.epi), w4_epilogue(v.y, p.epi), w4_epilogue(v.z, p.epi), w4_epilogue(v.w, p.epi)};
+  if (p.epi == kEpiF32)
+    *reinterpret_cast<float4*>(static_cast<float*>(p.y) + i) = make_float4(e[0], e[1], e[2], e[3]);
+  else
+    *reinterpret_cast<uint2*>(static_cast<half*>(p.y) + i) = make_uint2(h2u(__floats2half2_rn(e[0], e[1])), h2u(__floats2half2_rn(e[2], e[3])));
+}
+
+// Token tiles and K ranges with the least time by this account, in clocks of an SM: a K block of t tokens takes COST, a unit
+// 2500 to begin and end, the second kernel 6000 and its traffic.
+tc::Shape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
+  tc::Shape best = {};
+  double least = 0;
+  const int kblocks = (K + tc::kBK - 1) / tc::kBK;
+  const size_t plane = static_cast<size_t>(M) * N;
+  for (int toks = tc::kToks; toks >= 64; toks -= 16)
+    for (int want = 1; want <= 16 && want <= kblocks; ++want) {
+      tc::Shape h;
+      h.toks = toks;
+      h.tiles = (N + toks - 1) / toks;
+      h.row_blocks = (M + tc::kRows - 1) / tc::kRows;
+      h.x_rows = std::min(tc::kRows, (M + 7) & ~7);
+      h.kb_per_split = (kblocks + want - 1) / want;
+      h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
+      if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
+      const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
+      double cost = static_cast<double>((units + sms - 1) / sms) * (h.kb_per_split * (200.0 + 4.0 * toks) + 2500);
+      if (h.splits > 1) cost += 6000 + 4.0 * (h.splits + 1) * plane / (24.0 * sms);
+      h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
+      if (best.toks == 0 || cost < least) { least = cost; best = h; }
+    }
+  return best;
+}
+
+int many_rows(cudaStream_t stream, const W4GroupArgs& a, float* scratch, size_t scratch_bytes, int sms) {
+  const tc::Shape h = many_rows_shape(a.M, a.K, a.N, scratch ? scratch_bytes / sizeof(float) : 0, sms);
+  RK_REQUIRE(h.units < 0x7fffffff, kShape, "linear_w4a16_group: too many rows");
+  tc::Weights w;
+  w.V = a.N; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
+  ProductEpilogue epi;
+  epi.y = a.y; epi.partial = h.splits > 1 ? scratch : nullptr; epi.n_rows = a.M; epi.N = a.N; epi.epi = a.epi;
+  const int s = tc::launch_rows<2>(stream, "linear_w4a16_group", a.x, a.M, a.q, w, h, epi, sms);
+  if (s != kOk || h.splits == 1) return s;
+  const size_t quads = static_cast<size_t>(a.M) * a.N / 4;
+  RK_CUDA(launch_pdl(w4_reduce_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, epi, h.splits));
+  RK_LAUNCH_CHECK("linear_w4a16_group reduction launch");
+  return kOk;
+}
+
+}  // namespace
+
 size_t w4_group_workspace(int M, int K, int N) {
-  if (M <= kMaxRows || N % 4 != 0) return 0;
-  const long long tiles = static_cast<long long>((N + 127) / 128) * ((M + 255) / 256);
-  const long long planes = std::min<long long>({16, (296 + tiles - 1) / tiles, (K + 255) / 256});
-  return planes < 2 ? 0 : static_cast<size_t>(planes) * M * N * sizeof(float);
+  if (M <= kMatvecRows || N % 4 != 0) return 0;
+  int sms = 148;
+  if (device_sms(&sms) != kOk) sms = 148;
+  const tc::Shape h = many_rows_shape(M, K, N, ~static_cast<size_t>(0) / 8, sms);
+  return h.splits > 1 ? static_cast<size_t>(h.splits) * M * N * sizeof(float) : 0;
 }
 
 int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, size_t workspace_bytes) {
@@ -592,14 +709,7 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, 
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
-  if (a.M > kMatvecRows) {
-    LinearArgs l;
-    l.M = a.M; l.K = a.K; l.N = a.N; l.x = a.x; l.w = a.q; l.fmt = 2; l.scale = a.scale; l.zero = a.zero;
-    l.grouped = true; l.group = a.group; l.epi = a.epi; l.y = a.y;
-    l.scratch = static_cast<float*>(workspace); l.scratch_bytes = workspace ? workspace_bytes : 0;
-    RK_REQUIRE(gemm_tc_supported(l), kShape, "linear_w4a16_group: unsupported shape");
-    return gemm_tc(stream, l);
-  }
+  if (a.M > (getenv("RK_CUT") ? atoi(getenv("RK_CUT")) : kMatvecRows)) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
   for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
     MatvecPlan p;
