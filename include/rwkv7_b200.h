@@ -142,6 +142,17 @@ int rwkv7_b200_forward(rwkv7_b200_model* m, const int64_t* tokens_host, int B, i
 int rwkv7_b200_forward_to_host(rwkv7_b200_model* m, const int64_t* tokens_host, int B, int T, void* shift,
                                void* wkv, int* elapsed, float* logits, float* logits_host, void* stream);
 
+/* rwkv7_b200_forward for scoring a prompt (no counterpart in the reference, whose forward keeps the last token's logits
+ * only): the state is advanced as by rwkv7_b200_forward, and for every position logprobs [B][T] receives the log probability
+ * of the given token targets_host[b][t] after the tokens up to and including position t (for a prompt's own likelihood:
+ * the tokens one position on, and -1 behind the last), 0 where the id is below 0; ids of vocab or more are BAD_ARG.
+ * entropy [B][T] may be NULL, and so may logits (fp32 [B][vocab] of the last position).  The log probabilities are those of
+ * rwkv7_b200_head_logprobs, over logits that are not rounded to half.  Asynchronous; both host arrays may be reused on
+ * return.  A call that has to grow its scratch synchronises the device first.  Not available for tensor-parallel models. */
+int rwkv7_b200_forward_score(rwkv7_b200_model* m, const int64_t* tokens_host, const int64_t* targets_host, int B, int T,
+                             void* shift, void* wkv, int* elapsed, float* logits, float* logprobs, float* entropy,
+                             void* stream);
+
 /* The step after the path, kept on the device: `steps` decode steps in a row, each followed by a greedy choice of
  * every sequence's next token, with no host round trip between them.  Replaces, for top_p == 0 (the sampler's greedy
  * case, src/utils/sampling.cu:507-512), the engine's loop forward_decode -> sampler -> copy to the host -> next

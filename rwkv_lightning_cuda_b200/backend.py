@@ -213,6 +213,38 @@ class ModelBackend:
             raise L.Rwkv7B200Error(1, "token_batches must not be empty")
         self._forward(t.reshape(-1, 1), state, logits, sync)
 
+    def forward_score(self, token_batches: Sequence[Sequence[int]], state: GenerationState, targets=None,
+                      logits: Optional[DeviceLogits] = None):
+        """Advances ``state`` as forward_prefill does and scores every position: the log probability of ``targets[b][t]`` (an id
+        below 0 asks for nothing and gets 0) after the tokens up to position t, and the entropy there.  ``targets`` None: the
+        prompt's own tokens one position on, nothing behind the last.  ``logits``, if given, receives the last position's.  Returns
+        (logprobs, entropy), fp32 [B, T] on the device; not synchronised.  Not for tensor-parallel models."""
+        t = self._as_tokens(token_batches)
+        B, T = t.shape
+        if targets is None:
+            want = torch.full_like(t, -1)
+            want[:, :-1] = t[:, 1:]
+        else:
+            want = self._as_tokens(targets)
+        if tuple(want.shape) != (B, T):
+            raise L.Rwkv7B200Error(1, "targets must have the shape of the tokens")
+        if state.batch_size != B:
+            raise L.Rwkv7B200Error(1, "state batch size mismatch")
+        if state.wkv32 != self.use_wkv32:
+            raise L.Rwkv7B200Error(3, "state wkv precision mismatch")
+        dev = torch.device("cuda", self.device)
+        if logits is not None:
+            if logits.values is None or logits.values.numel() < B * self.dims.vocab:
+                logits.values = torch.empty((B, self.dims.vocab), dtype=torch.float32, device=dev)
+            logits.rows, logits.vocab_size = B, self.dims.vocab
+        logprobs = torch.empty((B, T), dtype=torch.float32, device=dev)
+        entropy = torch.empty((B, T), dtype=torch.float32, device=dev)
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        L.check(self._lib.rwkv7_b200_forward_score(
+            self._h, C.c_void_p(t.data_ptr()), C.c_void_p(want.data_ptr()), B, T, _ptr(state.shift), _ptr(state.wkv_state), _ptr(state.elapsed),
+            _ptr(logits.values) if logits is not None else None, _ptr(logprobs), _ptr(entropy), C.c_void_p(stream)))
+        return logprobs, entropy
+
     def forward_to_host(self, tokens: torch.Tensor, state: GenerationState, logits: DeviceLogits, out_host: torch.Tensor) -> None:
         """Host-buffer call: token ids from host memory in, fp32 logits in (pinned) host memory out."""
         B, T = tokens.shape

@@ -104,6 +104,12 @@ int rwkv7_b200_forward_to_host(rwkv7_b200_model* m, const int64_t* tokens_host, 
   return m->impl.timeout_result();
 }
 
+int rwkv7_b200_forward_score(rwkv7_b200_model* m, const int64_t* tokens_host, const int64_t* targets_host, int B, int T, void* shift,
+                             void* wkv, int* elapsed, float* logits, float* logprobs, float* entropy, void* stream) {
+  RK_REQUIRE(m, kBadArg, "null model");
+  return m->impl.forward_score(tokens_host, targets_host, B, T, shift, wkv, elapsed, logits, logprobs, entropy, st(stream));
+}
+
 int rwkv7_b200_decode_greedy(rwkv7_b200_model* m, const int64_t* first_tokens_host, int B, int steps, void* shift, void* wkv,
                              int* elapsed, float* logits, float* penalties, float presence_penalty, float repetition_penalty,
                              float penalty_decay, int* out_tokens, int* out_tokens_host, void* stream) {

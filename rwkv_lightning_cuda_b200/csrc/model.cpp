@@ -61,6 +61,8 @@ Model::~Model() {
     if (tokens_copied_[i]) cudaEventDestroy(tokens_copied_[i]);
   }
   if (last_done_) cudaEventDestroy(last_done_);
+  if (targets_pinned_) cudaFreeHost(targets_pinned_);
+  if (targets_copied_) cudaEventDestroy(targets_copied_);
   if (timeout_host_) cudaFreeHost(timeout_host_);
 }
 
@@ -603,7 +605,8 @@ int Model::enqueue_decode(Workspace& ws, int B, half* shift, void* wkv, int* ela
   return kOk;
 }
 
-int Model::enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* elapsed, float* logits, cudaStream_t st) {
+int Model::enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* elapsed, float* logits, cudaStream_t st,
+                   const Score* score) {
   const int C = cfg_.channels, L = cfg_.layers, rows = B * T;
   const int G = tp_size_, Cl = C / G, Hl = H_ / G;  // this rank's share of channels / heads
   const EpiArgs none;
@@ -628,7 +631,7 @@ int Model::enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* ela
     const bool gemv_rows = rows == 1 || (cfg_.weight_format != RWKV7_B200_FMT_F16 && !quant_tc) ||
                            (cfg_.weight_format == RWKV7_B200_FMT_F16 && rows < fp16_tc_rows);
     // (the fused path stages a step's activations in shared memory: B rows of ffn inputs must fit)
-    if (G == 1 && T == 1 && rows <= 4 && gemv_rows && tmix_decode_supported(probe) && C <= 4096 && rows_ok &&
+    if (!score && G == 1 && T == 1 && rows <= 4 && gemv_rows && tmix_decode_supported(probe) && C <= 4096 && rows_ok &&
         ((mma_fp16 || mma_quant) ? gemv_mma_fits(rows, std::max(C, cfg_.ffn))
                                  : (linear_batch_fused_fits(rows, cfg_.ffn) && linear_batch_fused_fits(rows, C))))
       return enqueue_decode(ws, B, shift, wkv, elapsed, logits, st);
@@ -825,11 +828,31 @@ int Model::enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* ela
       a.shift = shift + static_cast<size_t>(li + 1) * 2 * B * C; a.n_mix = 6;
       for (int i = 0; i < 6; ++i) { a.mix[i] = Nx.mix[i].as<half>(); a.mix_out[i] = ws.xm[i]; }
     } else {
-      a.ln_w = ln_out_w_.as<half>(); a.ln_b = ln_out_b_.as<half>(); a.n_out = ws.xf; a.last_only = true;
+      a.ln_w = ln_out_w_.as<half>(); a.ln_b = ln_out_b_.as<half>();
+      if (score) {  // every position's row (n1 is the fused decode path's)
+        a.B = rows; a.T = 1; a.n_out = ws.n1;
+      } else {
+        a.n_out = ws.xf; a.last_only = true;
+      }
     }
     RK_TRY(row_op(st, a));
   }
   RK_TRY(advance_i32(st, elapsed, T, B));
+  if (score) {
+    HeadLogprobsArgs h;
+    h.rows = rows; h.K = C; h.V = cfg_.vocab; h.x = ws.n1; h.w = head_.w.p; h.fmt = head_.fmt; h.group = 128;
+    h.scale = head_.scale.as<half>(); h.zero = head_.zero.as<half>(); h.tokens = score->targets;
+    h.logprobs = score->logprobs; h.entropy = score->entropy;
+    const size_t at = (static_cast<size_t>(rows) * sizeof(int64_t) + 15) & ~static_cast<size_t>(15);  // behind the given tokens
+    RK_TRY(head_logprobs(st, h, score_.as<char>() + at, score_.bytes - at));
+    if (!logits) return kOk;
+    LinearArgs a;  // the last position's rows, T rows apart
+    a.M = B; a.K = C; a.N = cfg_.vocab; a.x = ws.n1 + static_cast<size_t>(T - 1) * C; a.ldx = T * C; a.w = head_.w.p; a.fmt = head_.fmt;
+    a.scale = head_.scale.as<half>(); a.zero = head_.zero.as<half>(); a.epi = kEpiF32; a.y = logits; a.w_dynamic = false;
+    a.prefer_tc = head_.fmt == RWKV7_B200_FMT_F16 ? options().gemv_mma < 2 : B >= quant_tc_rows(head_.fmt);
+    a.scratch = ws.gemm_scratch; a.scratch_bytes = ws.gemm_scratch_bytes;
+    return linear(st, a);
+  }
   if (G == 1) {
     RK_TRY(lin(st, B, head_, ws.xf, logits, kEpiF32));
   } else {
@@ -859,6 +882,16 @@ int Model::forward(const int64_t* tokens_host, int B, int T, void* shift, void* 
   return step(tokens_host, B, T, shift, wkv, elapsed, logits, stream);
 }
 
+int Model::stage_tokens(const int64_t* tokens_host, long long rows, cudaStream_t stream) {
+  const int slot = slot_;
+  slot_ = (slot + 1) % kSlots;
+  RK_CUDA(cudaEventSynchronize(tokens_copied_[slot]));  // the copy that last read this slot is done
+  std::memcpy(tokens_pinned_[slot], tokens_host, static_cast<size_t>(rows) * sizeof(int64_t));
+  RK_CUDA(cudaMemcpyAsync(ws_.tokens, tokens_pinned_[slot], static_cast<size_t>(rows) * sizeof(int64_t), cudaMemcpyHostToDevice, stream));
+  RK_CUDA(cudaEventRecord(tokens_copied_[slot], stream));
+  return kOk;
+}
+
 // One forward with mu_ held.  tokens_host == nullptr: the ids are in the workspace's device buffer already (written
 // by the greedy pick of the previous step).
 int Model::step(const int64_t* tokens_host, int B, int T, void* shift, void* wkv, int* elapsed, float* logits,
@@ -867,14 +900,7 @@ int Model::step(const int64_t* tokens_host, int B, int T, void* shift, void* wkv
   int s = kOk;
   if ((s = prepare(B, T, stream)) != kOk) return s;
   Workspace* ws = &ws_;
-  if (tokens_host) {
-    const int slot = slot_;
-    slot_ = (slot + 1) % kSlots;
-    RK_CUDA(cudaEventSynchronize(tokens_copied_[slot]));  // the copy that last read this slot is done
-    std::memcpy(tokens_pinned_[slot], tokens_host, static_cast<size_t>(rows) * sizeof(int64_t));
-    RK_CUDA(cudaMemcpyAsync(ws->tokens, tokens_pinned_[slot], static_cast<size_t>(rows) * sizeof(int64_t), cudaMemcpyHostToDevice, stream));
-    RK_CUDA(cudaEventRecord(tokens_copied_[slot], stream));
-  }
+  if (tokens_host && (s = stage_tokens(tokens_host, rows, stream)) != kOk) return s;
   s = run(*ws, B, T, shift, wkv, elapsed, logits, stream);
   if (s != kOk) return s;
   RK_CUDA(cudaEventRecord(last_done_, stream));
@@ -939,6 +965,54 @@ int Model::run(Workspace& wsr, int B, int T, void* shift, void* wkv, int* elapse
   }
   RK_CUDA(cudaGraphLaunch(e.exec, stream));
   launches_ += e.launches;
+  return kOk;
+}
+
+// The layers as in a forward, but the final LayerNorm over every position and the head product reduced to log probabilities where
+// it is computed (head_logprobs.cu): the logits of B * T positions exist nowhere.  Enqueued kernel by kernel, no graph.
+int Model::forward_score(const int64_t* tokens_host, const int64_t* targets_host, int B, int T, void* shift, void* wkv, int* elapsed,
+                         float* logits, float* logprobs, float* entropy, cudaStream_t stream) {
+  RK_REQUIRE(finalized_, kNotReady, "forward_score: model not finalised");
+  RK_REQUIRE(B > 0, kBadArg, "token_batches must not be empty");
+  RK_REQUIRE(T > 0, kBadArg, "token batch length must be positive");
+  RK_REQUIRE(tokens_host && targets_host && shift && wkv && elapsed && logprobs, kBadArg, "forward_score: null pointer");
+  RK_REQUIRE(tp_size_ == 1, kBadArg, "forward_score: not available for a tensor-parallel model");
+  const long long rows = static_cast<long long>(B) * T;
+  RK_REQUIRE(rows < (1ll << 31), kShape, "forward_score: too many tokens");
+  for (long long i = 0; i < rows; ++i) {
+    RK_REQUIRE(tokens_host[i] >= 0 && tokens_host[i] < cfg_.vocab, kBadArg, "token id out of range");
+    RK_REQUIRE(targets_host[i] < cfg_.vocab, kBadArg, "given token id out of range");
+  }
+  int s = use_device();
+  if (s != kOk) return s;
+  std::lock_guard<std::mutex> lock(mu_);
+  if ((s = prepare(B, T, stream)) != kOk) return s;
+  const size_t need = static_cast<size_t>(rows) * sizeof(int64_t) + 16 + head_logprobs_workspace(static_cast<int>(rows), cfg_.vocab);
+  if (need > score_.bytes || static_cast<size_t>(rows) > targets_rows_) {
+    RK_CUDA(cudaDeviceSynchronize());
+    if (need > score_.bytes && (s = score_.alloc(need)) != kOk) return s;
+    if (!targets_copied_) RK_CUDA(cudaEventCreateWithFlags(&targets_copied_, cudaEventDisableTiming));
+    if (static_cast<size_t>(rows) > targets_rows_) {
+      if (targets_pinned_) cudaFreeHost(targets_pinned_);
+      targets_pinned_ = nullptr;
+      targets_rows_ = 0;
+      RK_CUDA(cudaMallocHost(reinterpret_cast<void**>(&targets_pinned_), static_cast<size_t>(rows) * sizeof(int64_t)));
+      targets_rows_ = static_cast<size_t>(rows);
+    }
+  }
+  if ((s = stage_tokens(tokens_host, rows, stream)) != kOk) return s;
+  RK_CUDA(cudaEventSynchronize(targets_copied_));
+  std::memcpy(targets_pinned_, targets_host, static_cast<size_t>(rows) * sizeof(int64_t));
+  RK_CUDA(cudaMemcpyAsync(score_.p, targets_pinned_, static_cast<size_t>(rows) * sizeof(int64_t), cudaMemcpyHostToDevice, stream));
+  RK_CUDA(cudaEventRecord(targets_copied_, stream));
+  const Score score{score_.as<int64_t>(), logprobs, entropy};
+  const long long before = launch_counter();
+  s = enqueue(ws_, B, T, static_cast<half*>(shift), wkv, elapsed, logits, stream, &score);
+  launches_ += launch_counter() - before;
+  if (s != kOk) return s;
+  RK_CUDA(cudaEventRecord(last_done_, stream));
+  last_stream_ = stream;
+  have_last_ = true;
   return kOk;
 }
 

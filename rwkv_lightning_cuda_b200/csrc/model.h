@@ -73,6 +73,9 @@ class Model {
   int decode_greedy(const int64_t* first_tokens_host, int B, int steps, void* shift, void* wkv, int* elapsed, float* logits,
                     float* penalties, float presence, float repetition, float decay, int* out_tokens, cudaStream_t stream,
                     const rwkv7_b200_sampling* sampling = nullptr);
+  // A forward that answers for every position: log probability of a given next token, entropy; logits of the last tokens if wanted
+  int forward_score(const int64_t* tokens_host, const int64_t* targets_host, int B, int T, void* shift, void* wkv, int* elapsed,
+                    float* logits, float* logprobs, float* entropy, cudaStream_t stream);
   int state_sizes(int B, size_t* shift_elems, size_t* wkv_elems, size_t* elapsed_elems) const;
   int state_init(int B, void* shift, void* wkv, int* elapsed, cudaStream_t stream) const;
   int copy_state_slice(const void* src_shift, const void* src_wkv, const int* src_elapsed, int src_B, int src_off,
@@ -89,7 +92,7 @@ class Model {
   // given the copy by enqueue_timeout_read and be synchronised by the caller in between.
   int enqueue_timeout_read(cudaStream_t stream);
   int timeout_result();
-  size_t workspace_bytes() const { return arena_.bytes + gemm_scratch_.bytes + part32_.bytes; }
+  size_t workspace_bytes() const { return arena_.bytes + gemm_scratch_.bytes + part32_.bytes + score_.bytes; }
 
   const rwkv7_b200_config& cfg() const { return cfg_; }
   long long launches() const { return launches_; }
@@ -118,9 +121,14 @@ class Model {
   int quantize(Matrix& m);
   int prepare(int B, int T, cudaStream_t stream);
   void drop_graphs();
+  struct Score {
+    const int64_t* targets;  // [B * T], device
+    float *logprobs, *entropy;
+  };
+  int stage_tokens(const int64_t* tokens_host, long long rows, cudaStream_t stream);
   int step(const int64_t* tokens_host, int B, int T, void* shift, void* wkv, int* elapsed, float* logits, cudaStream_t stream);
   int run(Workspace& ws, int B, int T, void* shift, void* wkv, int* elapsed, float* logits, cudaStream_t stream);
-  int enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* elapsed, float* logits, cudaStream_t s);
+  int enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* elapsed, float* logits, cudaStream_t s, const Score* score = nullptr);
   int enqueue_decode(Workspace& ws, int B, half* shift, void* wkv, int* elapsed, float* logits, cudaStream_t s);
   int lin(cudaStream_t s, int M, const Matrix& W, const half* x, void* y, int epi);
   int lin16(cudaStream_t s, int M, int K, int N, const half* x, const half* w, half* y, int in_act, int epi,
@@ -145,6 +153,10 @@ class Model {
   // first waits for that one's work (last_done_), because both would use these buffers.
   std::mutex mu_;
   DevBuf arena_, gemm_scratch_, part32_, probs_;  // probs_: the sampler's scratch, [B, vocab] fp32
+  DevBuf score_;                                  // forward_score: the given tokens and the head's scratch
+  int64_t* targets_pinned_ = nullptr;             // their staging, reused once targets_copied_ has passed
+  size_t targets_rows_ = 0;
+  cudaEvent_t targets_copied_ = nullptr;
   Workspace ws_;
   // ring of pinned host staging slots for the token ids; a slot is reused only after the copy that read it has
   // completed, so callers may overwrite their token array as soon as forward returns

@@ -22,7 +22,6 @@
 #include <cuda.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -648,8 +647,9 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
     *reinterpret_cast<uint2*>(static_cast<half*>(p.y) + i) = make_uint2(h2u(__floats2half2_rn(e[0], e[1])), h2u(__floats2half2_rn(e[2], e[3])));
 }
 
-// Token tiles and K ranges with the least time by this account, in clocks of an SM: a K block of t tokens takes COST, a unit
-// 2500 to begin and end, the second kernel 6000 and its traffic.
+// Token tiles and K ranges with the least time by this account, in clocks of an SM: a K block takes some 1000 whatever its width
+// (measured 1000 at 80 tokens, 1060 at 224: the issuing thread's waits and the shared-memory traffic of the expansion), a
+// unit 2500 to begin and end, the second kernel 6000 and its traffic.
 tc::Shape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
   tc::Shape best = {};
   double least = 0;
@@ -666,7 +666,7 @@ tc::Shape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
       h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
       if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
       const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
-      double cost = static_cast<double>((units + sms - 1) / sms) * (h.kb_per_split * (200.0 + 4.0 * toks) + 2500);
+      double cost = static_cast<double>((units + sms - 1) / sms) * (h.kb_per_split * (950.0 + 0.5 * toks) + 2500);
       if (h.splits > 1) cost += 6000 + 4.0 * (h.splits + 1) * plane / (24.0 * sms);
       h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
       if (best.toks == 0 || cost < least) { least = cost; best = h; }
@@ -709,7 +709,7 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, 
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
-  if (a.M > (getenv("RK_CUT") ? atoi(getenv("RK_CUT")) : kMatvecRows)) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
+  if (a.M > kMatvecRows) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
   for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
     MatvecPlan p;

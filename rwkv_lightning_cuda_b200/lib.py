@@ -55,6 +55,7 @@ SIGNATURES = {
     "rwkv7_b200_state_init": [_vp, _i, _vp, _vp, _vp, _vp],
     "rwkv7_b200_forward": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp],
     "rwkv7_b200_forward_to_host": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp],
+    "rwkv7_b200_forward_score": [_vp, _vp, _vp, _i, _i] + [_vp] * 7,
     "rwkv7_b200_decode_greedy": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _vp, _vp, _vp],
     "rwkv7_b200_greedy_pick": [_vp, _i, _i, _vp, _vp, _f, _f, _f, _vp, _vp],
     "rwkv7_b200_decode_sample": [_vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, C.POINTER(Sampling), _vp, _vp, _vp],
