@@ -26,17 +26,13 @@ namespace tc {
 constexpr int kRows = 128;   // rows of x per unit = MMA M
 constexpr int kToks = 256;   // tokens per unit = MMA N, at most (Shape::toks)
 constexpr int kBK = 64;      // halves per K block = one 128-byte swizzle row
-constexpr uint32_t kXBytes = kRows * 128, kWBytes = kToks * 128, kStageBytes = kXBytes + kWBytes;
 constexpr int kExpandWarps = 16;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kMaxTiles = 8, kMaxRaws = 8;
+constexpr size_t kSmemBytes = 225 * 1024;  // of 227 KB, beside the static part
 
-// Stages of the tile ring and of the ring of packed tiles, bytes of a packed row and tile.
-template <int kFmt> struct Ring;
-template <> struct Ring<0> { static constexpr int tiles = 4, raws = 0, raw_row = 0, raw = 0; };
-template <> struct Ring<1> { static constexpr int tiles = 3, raws = 4, raw_row = kBK, raw = kToks * raw_row; };
-template <> struct Ring<2> { static constexpr int tiles = 3, raws = 8, raw_row = kBK / 2, raw = kToks * raw_row; };
-template <int kFmt> constexpr size_t smem_bytes() { return 1024 + Ring<kFmt>::tiles * kStageBytes + Ring<kFmt>::raws * Ring<kFmt>::raw; }
 template <int kFmt> constexpr int tc_threads() { return kFmt == 0 ? 192 : 256 + kExpandWarps * 32; }
+template <int kFmt> __host__ __device__ constexpr int raw_row() { return kFmt == 0 ? 0 : kFmt == 1 ? kBK : kBK / 2; }  // bytes of a packed row of a K block
 
 // The weights: fp16, int8 with a scale per row (applied to the sums), or 4 bits with scales and zeros per group (half((q - zero) * scale)).
 struct Weights {
@@ -50,6 +46,9 @@ struct Shape {
   int splits, kb_per_split; // ranges of K and their K blocks (the last one may have fewer)
   int units;
   int x_rows;  // rows of x that a block loads: all there are, in eights, up to 128 (the rest of the tile is not read out)
+  // shared memory, set by launch_rows: the rings of tiles (x, then weights) and of packed tiles
+  int ring_tiles, ring_raws;
+  uint32_t x_bytes, tile_bytes, raw_bytes;
 };
 struct Unit {
   int r0, n0, split, kb0, kblocks;
@@ -160,23 +159,22 @@ __device__ __forceinline__ uint2 expand8(uint32_t w) {
 template <int kFmt, class Epi>
 __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
     tc_rows_kernel(const __grid_constant__ Maps maps, const Weights a, const Shape h, const Epi epilogue, int* timeout) {
-  constexpr int kTiles = Ring<kFmt>::tiles, kRaws = Ring<kFmt>::raws > 0 ? Ring<kFmt>::raws : 1;
   extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kTiles], ready[kTiles], empty[kTiles], raw_full[kRaws], raw_empty[kRaws], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[kMaxTiles], ready[kMaxTiles], empty[kMaxTiles], raw_full[kMaxRaws], raw_empty[kMaxRaws], acc_full[2], acc_empty[2];
   __shared__ float scales[kToks];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + kTiles * kStageBytes;
+  const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring_tiles * h.tile_bytes;
   const int kblocks = (a.K + kBK - 1) / kBK;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kTiles; ++i) {
+    for (int i = 0; i < h.ring_tiles; ++i) {
       mbar_init(smem_u32(&full[i]), 1);
       mbar_init(smem_u32(&ready[i]), kExpandWarps / 2);
       mbar_init(smem_u32(&empty[i]), 1);
     }
-    for (int i = 0; i < kRaws; ++i) {
+    for (int i = 0; i < h.ring_raws; ++i) {
       mbar_init(smem_u32(&raw_full[i]), 1);
       mbar_init(smem_u32(&raw_empty[i]), kExpandWarps / 2);
     }
@@ -204,22 +202,22 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
     // ---- loads: the fp16 tiles of both operands, or the packed weights (warp 0) and the rows (warp 6) on rings of their own
     if (lane == 0) {
       const bool packed = kFmt != 0 && warp == 0;
-      const int stages = packed ? kRaws : kTiles;
-      int it = 0;
+      const int stages = packed ? h.ring_raws : h.ring_tiles;
+      int it = 0, s = 0, phase = 0;
       for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
         const Unit un = unit_of(h, u, kblocks);
         for (int kb = un.kb0; kb < un.kb0 + un.kblocks; ++kb, ++it) {
-          const int s = it % stages;
-          if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], (it / stages - 1) & 1))) break;
-          const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]), dst = ring + s * kStageBytes;
+          if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], phase ^ 1))) break;
+          const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]), dst = ring + s * h.tile_bytes;
           if (packed) {
-            mbar_expect_tx(bar, h.toks * Ring<kFmt>::raw_row);
-            tma_2d(raw_ring + s * Ring<kFmt>::raw, &maps.w, bar, kb * Ring<kFmt>::raw_row, un.n0);
+            mbar_expect_tx(bar, h.toks * raw_row<kFmt>());
+            tma_2d(raw_ring + s * h.raw_bytes, &maps.w, bar, kb * raw_row<kFmt>(), un.n0);
           } else {
             mbar_expect_tx(bar, 128 * (h.x_rows + (kFmt == 0 ? h.toks : 0)));
             tma_2d(dst, &maps.x, bar, kb * kBK, un.r0);
-            if (kFmt == 0) tma_2d(dst + kXBytes, &maps.w, bar, kb * kBK, un.n0);
+            if (kFmt == 0) tma_2d(dst + h.x_bytes, &maps.w, bar, kb * kBK, un.n0);
           }
+          if (++s == stages) { s = 0; phase ^= 1; }
         }
       }
       if (!ok)  // leave no copy in flight behind
@@ -229,21 +227,21 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
     // ---- products: K blocks of 64 as four instructions into the unit's accumulator
     if (lane == 0) {
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(h.toks >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);
-      int it = 0, n = 0;
+      int n = 0, s = 0, phase = 0;
       for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
         if (n >= 2 && !(ok = wait(acc_empty[n & 1], ((n >> 1) - 1) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t acc = tmem + (n & 1) * kToks;
         const int here = unit_of(h, u, kblocks).kblocks;
-        for (int kb = 0; kb < here; ++kb, ++it) {
-          const int s = it % kTiles;
-          ok = wait(full[s], (it / kTiles) & 1) && (kFmt == 0 || wait(ready[s], (it / kTiles) & 1));
+        for (int kb = 0; kb < here; ++kb) {
+          ok = wait(full[s], phase) && (kFmt == 0 || wait(ready[s], phase));
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t dx = tile_desc(ring + s * kStageBytes), dw = tile_desc(ring + s * kStageBytes + kXBytes);
+          const uint64_t dx = tile_desc(ring + s * h.tile_bytes), dw = tile_desc(ring + s * h.tile_bytes + h.x_bytes);
 #pragma unroll
           for (int k4 = 0; k4 < kBK / 16; ++k4) mma(acc, dx + 2 * k4, dw + 2 * k4, idesc, (kb | k4) != 0);
           commit(smem_u32(&empty[s]));
+          if (++s == h.ring_tiles) { s = 0; phase ^= 1; }
         }
         if (ok) commit(smem_u32(&acc_full[n & 1]));
       }
@@ -290,14 +288,14 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
     // ones.  Row r of the tile is 128 bytes at r * 128, its 16-byte chunk c at chunk position c ^ (r & 7); a packed row of 64 (32)
     // bytes has its chunk c at c ^ (r / 2 & 3) (c ^ (r / 4 & 1)): the swizzles of 128-, 64- and 32-byte rows, so that no two
     // lanes of a quarter warp meet in a bank.  (No barrier's phase is
-    // missed by taking every other K block: the packed ring is even, and of the three tiles of the other ring the one waited for
-    // is at most a phase ahead of the tile this thread waited for two blocks before.)
+    // missed by taking every other K block: the packed ring is even; and in the other ring of T >= 2 tiles block i waits until block
+    // i - T is used, when block i - 2 has shown that i - 2 - T is, so the fill of this tile before that one, i - 2 T, is too.)
     const int r = threadIdx.x & 255, turn = (threadIdx.x >> 8) - 1;
-    const uint32_t raw = raw_ring + r * Ring<kFmt>::raw_row, raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    const uint32_t raw = raw_ring + r * raw_row<kFmt>(), raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
     const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
     uint32_t at[8];  // where the chunks of this row go, in the first stage
 #pragma unroll
-    for (int c = 0; c < 8; ++c) at[c] = ring + kXBytes + r * 128 + ((16 * c) ^ ((r & 7) << 4));
+    for (int c = 0; c < 8; ++c) at[c] = ring + h.x_bytes + r * 128 + ((16 * c) ^ ((r & 7) << 4));
     // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
     // multiple of 16 bytes, group by group.
     const bool eights = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
@@ -327,7 +325,7 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
         else load_runs(kb);
       }
       for (; kb < kb_end; kb += 2) {
-        const bool first_round = it + kb - un.kb0 < kTiles;
+        const bool first_round = it + kb - un.kb0 < h.ring_tiles;
         if (kFmt == 2 && (!eights || (kb * kBK) >> (shift + 3) != block)) {
           sc = sc_next;
           ze = ze_next;
@@ -337,7 +335,7 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
         ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase) && (first_round || wait(empty[s], tile_phase ^ 1)));
         if (!ok) break;
         if (r < h.toks) {
-          const uint32_t src = raw + rs * Ring<kFmt>::raw, stage = s * kStageBytes;
+          const uint32_t src = raw + rs * h.raw_bytes, stage = s * h.tile_bytes;
           if (kFmt == 1) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -367,9 +365,9 @@ __global__ void __launch_bounds__(tc_threads<kFmt>(), 1)
           arrive(smem_u32(&raw_empty[rs]));
         }
         rs += 2;
-        if (rs >= kRaws) { rs -= kRaws; raw_phase ^= 1; }
+        if (rs >= h.ring_raws) { rs -= h.ring_raws; raw_phase ^= 1; }
         s += 2;
-        if (s >= kTiles) { s -= kTiles; tile_phase ^= 1; }
+        if (s >= h.ring_tiles) { s -= h.ring_tiles; tile_phase ^= 1; }
       }
       it += un.kblocks;
     }
@@ -398,17 +396,31 @@ inline int encode_map(const char* what, CUtensorMap* map, CUtensorMapDataType ty
 }
 
 template <int kFmt, class Epi>
-int launch_rows(cudaStream_t stream, const char* what, const half* x, int rows, const void* w, const Weights& a, const Shape& h, const Epi& epi, int sms) {
+int launch_rows(cudaStream_t stream, const char* what, const half* x, int rows, const void* w, const Weights& a, Shape h, const Epi& epi, int sms) {
   Maps maps;
   int s = encode_map(what, &maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, rows, a.K, kBK, h.x_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != kOk) return s;
   if (kFmt == 0) s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, w, a.V, a.K, kBK, h.toks, CU_TENSOR_MAP_SWIZZLE_128B);
-  else s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.V, kFmt == 1 ? a.K : a.K / 2, Ring<kFmt>::raw_row, h.toks,
+  else s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.V, kFmt == 1 ? a.K : a.K / 2, raw_row<kFmt>(), h.toks,
                       kFmt == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
   if (s != kOk) return s;
+  // The rings: packed tiles want enough in flight for the HBM (64 KB or so), fp16 tiles one more than the expansion and the MMA hold
+  // at a time: four where the packed ring keeps four, otherwise three.
+  h.x_bytes = (h.x_rows * 128 + 1023) & ~1023;
+  h.tile_bytes = std::max<uint32_t>(h.x_bytes + h.toks * 128, kRows * 128);  // (the MMA reads 128 rows of x, whatever is there)
+  h.raw_bytes = (h.toks * raw_row<kFmt>() + 1023) & ~1023;
+  const int budget = static_cast<int>(kSmemBytes) - 1024;
+  if (kFmt == 0) {
+    h.ring_tiles = std::min(kMaxTiles, budget / static_cast<int>(h.tile_bytes));
+    h.ring_raws = 0;
+  } else {
+    h.ring_tiles = budget - 4 * static_cast<int>(h.tile_bytes) >= 4 * static_cast<int>(h.raw_bytes) ? 4 : 3;
+    h.ring_raws = std::min(kMaxRaws, (budget - h.ring_tiles * static_cast<int>(h.tile_bytes)) / static_cast<int>(h.raw_bytes)) & ~1;
+  }
+  const size_t smem = 1024 + h.ring_tiles * static_cast<size_t>(h.tile_bytes) + h.ring_raws * static_cast<size_t>(h.raw_bytes);
   const auto kernel = tc_rows_kernel<kFmt, Epi>;
-  RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes<kFmt>())));
-  RK_CUDA(launch_pdl(kernel, dim3(std::min(h.units, sms)), dim3(tc_threads<kFmt>()), smem_bytes<kFmt>(), stream, maps, a, h, epi, timeout_word_or_null()));
+  RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
+  RK_CUDA(launch_pdl(kernel, dim3(std::min(h.units, sms)), dim3(tc_threads<kFmt>()), smem, stream, maps, a, h, epi, timeout_word_or_null()));
   RK_LAUNCH_CHECK(what);
   return kOk;
 }
