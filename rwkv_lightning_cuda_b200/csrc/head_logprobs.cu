@@ -4,21 +4,24 @@
 // where it is computed, and a second kernel merges a row's tiles (logprob.cuh).  fp16 operands, fp32 sums; int8 weights
 // are exact integers with the channel's scale on the sum, 4-bit weights half((q - zero) * scale).
 //
-// Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  The product is tc_rows.cuh's; here are its
-// epilogue, which reduces a row's tokens in a thread's registers, the merging of the tiles, and the route for a few rows.
+// Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  The products are tc_rows.cuh's (fp16 weights) and
+// tc_packed.cuh's (quantised ones); here are their epilogues, which reduce a tile of logits to (m, s, t) per row, the merging of the
+// tiles, and the route for a few rows.
 #include <algorithm>
 
 #include "common.cuh"
 #include "kernels.h"
 #include "logprob.cuh"
+#include "tc_packed.cuh"
 #include "tc_rows.cuh"
 
 namespace rk {
 namespace {
 
 constexpr int kMinToks = 128;  // the narrowest token tile
+static_assert(kMinToks <= tc::kTileToks, "");
 
-// A row's tokens of a unit: m, s and t over them, and the given token's logit where it is among them.
+// A row's tokens of a unit: m, s and t over them, and the given token's logit where it is among them.  A thread has one row.
 struct StatsEpilogue {
   float4* part;   // [tiles][rows]
   float* given;   // [rows]
@@ -28,7 +31,7 @@ struct StatsEpilogue {
   int64_t id;
   SoftStats st;
   __device__ __forceinline__ int rows() const { return n_rows; }
-  __device__ __forceinline__ void begin(int row, int first, int, int) {
+  __device__ __forceinline__ void begin(int row, int first, int) {
     r = row;
     n0 = first;
     id = tokens ? tokens[row] : -1;
@@ -52,6 +55,63 @@ struct StatsEpilogue {
     for (int i = 0; i < 32; ++i) add(st, z[i]);
   }
   __device__ __forceinline__ void end() { part[static_cast<size_t>(n0 / toks) * n_rows + r] = make_float4(st.m, st.s, st.t, 0.f); }
+};
+
+// The same where a thread has one token and all rows: 32 tokens x 32 rows at a time go through shared memory, after which a lane has
+// one row's 32 tokens; the four warps' parts of a row are merged at the end of the unit.
+struct PackedStatsEpilogue {
+  static constexpr int kPitch = 33, kWarpFloats = 32 * kPitch, kParts = 4 * tc::kMaxBlockRows;
+  static constexpr int kScratch = 4 * kWarpFloats * 4 + kParts * 16;
+  float4* part;   // [tiles][rows]
+  float* given;   // [rows]
+  const int64_t* tokens;
+  int n_rows, V;
+  int token, r0, rows, lane, quad;
+  float* box;       // this warp's [row][token]
+  float4* parts;    // [warp][row of the block]
+  __device__ __forceinline__ void begin(int tok, int first, int rows_here, int, unsigned char* scratch) {
+    token = tok;
+    r0 = first;
+    rows = rows_here;
+    lane = threadIdx.x & 31;
+    quad = (threadIdx.x >> 5) & 3;
+    box = reinterpret_cast<float*>(scratch) + quad * kWarpFloats;
+    parts = reinterpret_cast<float4*>(scratch + 4 * kWarpFloats * 4);
+  }
+  __device__ __forceinline__ void chunk(int c, float (&z)[32], int here) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) box[i * kPitch + lane] = token < V ? z[i] : -INFINITY;
+    __syncwarp();
+    if (lane < here) {
+      const int64_t id = tokens ? tokens[r0 + c + lane] - (token - lane) : -1;  // relative to the warp's first token
+      if (id >= 0 && id < 32 && token - lane + id < V) given[r0 + c + lane] = box[lane * kPitch + id];
+      SoftStats st;
+      float m = st.m;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) m = max_nan(m, box[lane * kPitch + i]);
+      st.m = m;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) add(st, box[lane * kPitch + i]);
+      parts[quad * tc::kMaxBlockRows + c + lane] = make_float4(st.m, st.s, st.t, 0.f);
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void end() {
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int tile = (token - lane) / tc::kTileToks;
+    for (int r = threadIdx.x & 127; r < rows; r += 128) {
+      SoftStats all;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float4 p = parts[w * tc::kMaxBlockRows + r];
+        SoftStats b;
+        b.m = p.x; b.s = p.y; b.t = p.z;
+        all = merge(all, b);
+      }
+      part[static_cast<size_t>(tile) * n_rows + r0 + r] = make_float4(all.m, all.s, all.t, 0.f);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the parts have been read
+  }
 };
 
 // One CTA per row merges the row's tiles: a load or two per thread, all under way at once.
@@ -82,7 +142,7 @@ __global__ void __launch_bounds__(kMergeThreads) head_merge_kernel(HeadLogprobsA
 
 // The token tile that lets the units come out in the fewest full rounds over the SMs (65536 tokens in tiles of 256 are 1.7 rounds
 // of 148, in tiles of 224 two full ones); a unit is counted as its tokens and 32 more for its beginning and end.
-tc::Shape head_shape(int rows, int V, int K, int sms) {
+tc::Shape head_shape(int rows, int V, int sms) {
   tc::Shape best = {};
   long long least = -1;
   for (int toks = tc::kToks; toks >= kMinToks; toks -= 16) {
@@ -90,8 +150,6 @@ tc::Shape head_shape(int rows, int V, int K, int sms) {
     h.toks = toks;
     h.tiles = (V + toks - 1) / toks;
     h.row_blocks = (rows + tc::kRows - 1) / tc::kRows;
-    h.splits = 1;
-    h.kb_per_split = (K + tc::kBK - 1) / tc::kBK;
     h.x_rows = std::min(tc::kRows, (rows + 7) & ~7);
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks, cost = (units + sms - 1) / sms * (toks + 32);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
@@ -100,17 +158,39 @@ tc::Shape head_shape(int rows, int V, int K, int sms) {
   return best;
 }
 
-template <int kFmt>
-int launch_head(cudaStream_t stream, const HeadLogprobsArgs& a, const tc::Shape& h, int sms) {
-  tc::Weights w;
-  w.V = a.V; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
-  StatsEpilogue epi;
-  epi.part = a.part; epi.given = a.given; epi.tokens = a.tokens; epi.n_rows = a.rows; epi.toks = h.toks;
-  const int s = tc::launch_rows<kFmt>(stream, "head_logprobs", a.x, a.rows, a.w, w, h, epi, sms);
-  if (s != kOk) return s;
-  RK_CUDA(launch_pdl(head_merge_kernel, dim3(a.rows), dim3(kMergeThreads), 0, stream, a, h.tiles));
+int merge_tiles(cudaStream_t stream, const HeadLogprobsArgs& a, int tiles) {
+  RK_CUDA(launch_pdl(head_merge_kernel, dim3(a.rows), dim3(kMergeThreads), 0, stream, a, tiles));
   RK_LAUNCH_CHECK("head_logprobs merge launch");
   return kOk;
+}
+
+int head_f16(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
+  const tc::Shape h = head_shape(a.rows, a.V, sms);
+  RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
+  a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
+  StatsEpilogue epi;
+  epi.part = a.part; epi.given = a.given; epi.tokens = a.tokens; epi.n_rows = a.rows; epi.toks = h.toks;
+  const int s = tc::launch_rows(stream, "head_logprobs", a.x, a.rows, static_cast<const half*>(a.w), a.K, a.V, h, epi, sms);
+  return s != kOk ? s : merge_tiles(stream, a, h.tiles);
+}
+
+template <int kFmt>
+int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
+  tc::PackedShape h = {};
+  tc::set_row_blocks(&h, a.rows);
+  h.tiles = (a.V + tc::kTileToks - 1) / tc::kTileToks;
+  h.splits = 1;
+  h.kb_per_split = (a.K + tc::kBK - 1) / tc::kBK;
+  const long long units = static_cast<long long>(h.tiles) * h.row_blocks;
+  RK_REQUIRE(units < 0x7fffffff, kShape, "head_logprobs: too many rows");
+  h.units = static_cast<int>(units);
+  a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
+  tc::Packed w;
+  w.V = a.V; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
+  PackedStatsEpilogue epi;
+  epi.part = a.part; epi.given = a.given; epi.tokens = a.tokens; epi.n_rows = a.rows; epi.V = a.V;
+  const int s = tc::launch_packed<kFmt>(stream, "head_logprobs", a.x, a.w, w, h, epi, sms);
+  return s != kOk ? s : merge_tiles(stream, a, h.tiles);
 }
 
 }  // namespace
@@ -179,12 +259,9 @@ int head_logprobs(cudaStream_t stream, HeadLogprobsArgs a, void* workspace, size
   const int status = device_sms(&sms);
   if (status != kOk) return status;
   if (few_rows(a, sms)) return logits_then_stats(stream, a, static_cast<float*>(workspace), sms);
-  const tc::Shape h = head_shape(a.rows, a.V, a.K, sms);
-  RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
-  a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
-  if (a.fmt == 1) return launch_head<1>(stream, a, h, sms);
-  if (a.fmt == 2) return launch_head<2>(stream, a, h, sms);
-  return launch_head<0>(stream, a, h, sms);
+  if (a.fmt == 1) return head_packed<1>(stream, a, sms);
+  if (a.fmt == 2) return head_packed<2>(stream, a, sms);
+  return head_f16(stream, a, sms);
 }
 
 }  // namespace rk

@@ -1,0 +1,385 @@
+// x W^T for rows of x and quantised weights on the tensor cores, with whatever is done with the products left to the caller: the skeleton
+// of the 4-bit products of many rows (w4_group.cu) and of the quantised head product that keeps no logits (head_logprobs.cu).
+//
+// The weights take the MMA's M side, 128 tokens (output channels) per unit, as an operand in tensor memory: a thread expands a
+// token's packed weights in registers and stores them to its lane, so that the fp16 weights never pass through shared
+// memory.  (Expanded into shared memory, as the operand of the N side, a K block of 224 tokens took some 1000 clocks, of which
+// its stores, the MMA's reads of both operands and the copies filled shared memory for 900.)  The N side are up to 256 rows of x.
+// Units: 128 tokens x a block of rows x a range of K, the row blocks of a token tile one after the other.  A lane of tensor
+// memory is a token, a column a row of x.  Up to 128 rows in a block there are two accumulators, and a unit's epilogue runs
+// under the next one's products; with more there is one.
+//
+// Warp roles: 0 loads packed tiles, 1 issues tcgen05.mma, 2..5 run the epilogue, 6 loads rows of x, 8..23 expand, four warps to a
+// K block in turn.  Every wait is bounded: one that runs out sets the device's failure word, every role leaves its loop, and the
+// CTA frees its tensor memory and returns.
+#pragma once
+
+#include "tc_common.cuh"
+
+namespace rk {
+namespace tc {
+
+constexpr int kTileToks = 128;    // tokens per unit = MMA M
+constexpr int kMaxBlockRows = 256;
+constexpr int kTurns = 4;         // groups of four warps that expand K blocks in turn
+constexpr int kMaxRing = 8;
+constexpr int kPackedThreads = 256 + kTurns * 128;
+constexpr int kOperandCols = kBK / 2;  // of tensor memory that a K block of weights takes
+constexpr int kOperandAt = 256;        // behind the accumulators
+
+template <int kFmt> __host__ __device__ constexpr int raw_row() { return kFmt == 1 ? kBK : kBK / 2; }  // bytes of a packed row of a K block
+
+// int8 with a scale per token (applied to the sums), or 4 bits with scales and zeros per group (half((q - zero) * scale)).
+struct Packed {
+  int V, K;
+  int group;                 // 4 bits: 32, 64 or 128
+  const half *scale, *zero;  // zero nullptr: 8
+};
+struct PackedShape {
+  int tiles;                 // of 128 tokens
+  int rows, row_blocks, block_rows;  // rows of x; block_rows: a multiple of 16, at most kMaxBlockRows
+  int splits, kb_per_split;  // ranges of K and their K blocks (the last one may have fewer)
+  int units;
+  int ring, raws;            // stages of x and weights, and of packed tiles (set by launch_packed)
+};
+struct PackedMaps {
+  CUtensorMap x, w;
+};
+struct PackedUnit {
+  int r0, n0, split, kb0, kblocks;
+};
+__device__ __forceinline__ PackedUnit unit_of(const PackedShape& h, int u, int kblocks) {
+  PackedUnit r;
+  r.r0 = u % h.row_blocks * h.block_rows;
+  u /= h.row_blocks;
+  r.split = u % h.splits;
+  r.n0 = u / h.splits * kTileToks;
+  r.kb0 = r.split * h.kb_per_split;
+  r.kblocks = min(h.kb_per_split, kblocks - r.kb0);
+  return r;
+}
+
+// Eight 4-bit codes to eight halves half((q - zero) * scale): a nibble under the exponent of 1024 is 1024 + q (the high ones
+// arrive as 1024 + 16 q), so one subtraction or fused multiply-add leaves q - zero exactly and the product rounds once.
+struct Group4 {
+  __half2 scale, sub;  // (s, s) and (-(1024 + z), -(64 + z))
+};
+__device__ __forceinline__ Group4 group4(uint32_t s2, uint32_t z2) {  // the group's scale and zero, twice each
+  return {*reinterpret_cast<const __half2*>(&s2), __hsub2(__floats2half2_rn(-1024.f, -64.f), *reinterpret_cast<const __half2*>(&z2))};
+}
+// Half i of eight, twice.
+__device__ __forceinline__ uint32_t pick(const uint4& v, int i) {
+  const uint32_t lo = i & 2 ? v.y : v.x, hi = i & 2 ? v.w : v.z;
+  return __byte_perm(i & 4 ? hi : lo, 0u, i & 1 ? 0x3232 : 0x1010);
+}
+// The constants are the caller's registers: as literals, mask and bias of the AND-OR would not fit into one instruction.
+struct Expand4 {
+  uint32_t nibbles, bias;  // 0x00f0000f, 0x64006400
+  __half2 mul;             // 1, 1/16
+};
+__device__ __forceinline__ uint4 expand4(uint32_t w, const Group4& g, const Expand4& e) {
+  uint32_t h[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint32_t both = __byte_perm(w, 0u, 0x4040u + 0x0101u * b);  // the byte in both halves
+    uint32_t pair;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(pair) : "r"(both), "r"(e.nibbles), "r"(e.bias));
+    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<__half2*>(&pair), e.mul, g.sub), g.scale);
+    h[b] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(h[0], h[1], h[2], h[3]);
+}
+// Four int8 codes to four halves, exactly: code + 128 under the exponent of 1024, less 1152.
+__device__ __forceinline__ uint2 expand8(uint32_t w) {
+  const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
+  const uint32_t t = w ^ 0x80808080u;
+  uint32_t lo = __byte_perm(t, 0x64646464u, 0x4140), hi = __byte_perm(t, 0x64646464u, 0x4342);
+  const __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), bias), b = __hsub2(*reinterpret_cast<__half2*>(&hi), bias);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Epi: a copy per epilogue thread and unit, all 128 of which are asked; begin(token, r0, rows, split, scratch), then chunk(c, z, here) for every
+// 32 rows r0 + c .. (here of them valid), where z[i] is the result of row r0 + c + i, then end(); scratch: Epi::kScratch bytes of shared
+// memory.  The threads may meet at barrier 1.
+template <int kFmt, class Epi>
+__global__ void __launch_bounds__(kPackedThreads, 1)
+    tc_packed_kernel(const __grid_constant__ PackedMaps maps, const Packed a, const PackedShape h, const Epi epilogue, int* timeout) {
+  extern __shared__ unsigned char smem[];
+  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing], raw_full[kMaxRing], raw_empty[kMaxRing], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int failed;
+  constexpr uint32_t kRawBytes = kTileToks * raw_row<kFmt>();
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const uint32_t x_bytes = h.block_rows * 128, ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring * x_bytes;
+  const int kblocks = (a.K + kBK - 1) / kBK;
+  const int accs = h.block_rows <= 128 ? 2 : 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < h.ring; ++i) {
+      mbar_init(smem_u32(&full[i]), 1 + 4);  // the rows of x, and the four warps' parts of the weights
+      mbar_init(smem_u32(&empty[i]), 1);
+    }
+    for (int i = 0; i < h.raws; ++i) {
+      mbar_init(smem_u32(&raw_full[i]), 1);
+      mbar_init(smem_u32(&raw_empty[i]), 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&acc_full[i]), 1);
+      mbar_init(smem_u32(&acc_empty[i]), 4);
+    }
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = uniform(tmem_slot);
+  pdl_wait();
+  pdl_trigger();
+
+  auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
+  bool ok = true;
+  if (warp == 0 || warp == 6) {
+    if (lane == 0) {
+      const bool packed = warp == 0;
+      const int stages = packed ? h.raws : h.ring;
+      int it = 0, s = 0, phase = 0;
+      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+        const PackedUnit un = unit_of(h, u, kblocks);
+        for (int kb = un.kb0; kb < un.kb0 + un.kblocks; ++kb, ++it) {
+          if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], phase ^ 1))) break;
+          const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]);
+          mbar_expect_tx(bar, packed ? kRawBytes : x_bytes);
+          if (packed) tma_2d(raw_ring + s * kRawBytes, &maps.w, bar, kb * raw_row<kFmt>(), un.n0);
+          else tma_2d(ring + s * x_bytes, &maps.x, bar, kb * kBK, un.r0);
+          if (++s == stages) { s = 0; phase ^= 1; }
+        }
+      }
+      if (!ok)  // leave no copy in flight behind
+        for (int i = it > stages ? it - stages : 0; i < it; ++i) mbar_wait(smem_u32(packed ? &raw_full[i % stages] : &full[i % stages]), (i / stages) & 1);
+    }
+  } else if (warp == 1) {
+    // ---- products: K blocks of 64 as four instructions into the unit's accumulator.  The whole warp goes through the loop, so that the
+    // operands are computed in uniform registers, and one lane issues (700 clocks a K block when one lane did all of it, between
+    // the instructions of 16 other warps); the next stage's barrier is asked, without waiting, before this one's products are issued.
+    const uint32_t idesc = instruction_desc(h.block_rows);
+    const bool issuer = elect_one();
+    int n = 0, s = 0, phase = 0;
+    bool ready = false;
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
+      const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
+      if (use >= 1 && !(ok = __all_sync(0xffffffffu, wait(acc_empty[acc], (use - 1) & 1)))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const int here = unit_of(h, u, kblocks).kblocks;
+      for (int kb = 0; kb < here; ++kb) {
+        if (!__all_sync(0xffffffffu, ready) && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t dx = tile_desc(ring + s * x_bytes);
+        const uint32_t dw = tmem + kOperandAt + s * kOperandCols, done = smem_u32(&empty[s]);
+        if (++s == h.ring) { s = 0; phase ^= 1; }
+        ready = mbar_test(smem_u32(&full[s]), phase);
+        if (issuer) {
+#pragma unroll
+          for (int k4 = 0; k4 < kBK / 16; ++k4) mma_from_tmem(tmem + acc * 128, dw + 8 * k4, dx + 2 * k4, idesc, (kb | k4) != 0);
+          commit(done);
+        }
+        __syncwarp();
+      }
+      if (ok && issuer) commit(smem_u32(&acc_full[acc]));
+      __syncwarp();
+    }
+  } else if (warp >= 2 && warp < 6) {
+    // ---- epilogue: a thread owns a token, its TMEM lane, and takes the unit's rows 32 at a time
+    const int quad = warp & 3;
+    unsigned char* const scratch = smem + (raw_ring - smem_u32(smem)) + h.raws * kRawBytes;
+    int n = 0;
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
+      const PackedUnit un = unit_of(h, u, kblocks);
+      const int token = un.n0 + quad * 32 + lane, rows = min(h.block_rows, h.rows - un.r0);
+      const float scale = kFmt == 1 && token < a.V ? __half2float(a.scale[token]) : 1.f;
+      const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
+      // (asleep: these four warps' polling of a wait this long cost the expansion a quarter of its time)
+      for (uint32_t i = 0; i < kSpinLimit && !(ok = mbar_test(smem_u32(&acc_full[acc]), use & 1)) && !failed; ++i) __nanosleep(100);
+      {  // all four warps stay or leave together: an epilogue may have them meet at a barrier
+        uint32_t all;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.and.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
+        ok = all != 0;
+      }
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      Epi epi = epilogue;
+      epi.begin(token, un.r0, rows, un.split, scratch);
+      for (int c = 0; c < rows; c += 32) {
+        float z[32];
+        tmem_ld32(tmem + acc * 128 + c + (static_cast<uint32_t>(quad * 32) << 16), z);
+        if (kFmt == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] *= scale;
+        }
+        epi.chunk(c, z, min(32, rows - c));
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(smem_u32(&acc_empty[acc]));
+      epi.end();
+    }
+  } else if (warp >= 8) {
+    // ---- expansion: a thread owns a token of the tile, 64 weights a K block; four warps take every fourth K block.  A packed row of 64
+    // (32) bytes has its 16-byte chunk c at c ^ (r / 2 & 3) (c ^ (r / 4 & 1)), the swizzles of 64- and 32-byte rows, so that no two
+    // lanes of a quarter warp meet in a bank.  (No barrier's phase is missed by taking every fourth K block: the packed ring is a multiple of four; and
+    // in the other ring of T >= 4 stages block i waits until block i - T is used, when block i - 4 has shown that i - 4 - T is, so
+    // the fill of this stage before that one, i - 2 T, is too.)
+    const int r = threadIdx.x & 127, turn = (static_cast<int>(threadIdx.x) - 256) >> 7;
+    const uint32_t raw = raw_ring + r * raw_row<kFmt>(), raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    const uint32_t operand = tmem + kOperandAt + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
+    const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
+    // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
+    // multiple of 16 bytes, group by group.
+    const bool eights = groups % 8 == 0 && ((reinterpret_cast<uintptr_t>(a.scale) | reinterpret_cast<uintptr_t>(a.zero)) & 15u) == 0;
+    const uint16_t *sp = nullptr, *zp = nullptr;
+    constexpr uint32_t kEight = 0x48004800u;
+    uint4 sc = make_uint4(0u, 0u, 0u, 0u), ze = make_uint4(kEight, kEight, kEight, kEight), sc_next = sc, ze_next = ze;
+    auto load8 = [&](int block) {
+      if (block * 8 >= groups) return;
+      sc_next = reinterpret_cast<const uint4*>(sp)[block];
+      if (zp) ze_next = reinterpret_cast<const uint4*>(zp)[block];
+    };
+    auto load_runs = [&](int kb) {  // a K block's two runs of 32 weights into the first two halves
+      const int g0 = min((kb * kBK) >> shift, groups - 1), g1 = min((kb * kBK + 32) >> shift, groups - 1);
+      sc_next.x = sp[g0] | (static_cast<uint32_t>(sp[g1]) << 16);
+      if (zp) ze_next.x = zp[g0] | (static_cast<uint32_t>(zp[g1]) << 16);
+    };
+    const uint32_t none = ring >> 30;  // 0, which the compiler does not know, so that the constants stay in registers
+    const uint32_t mul = 0x2c003c00u + none;
+    const Expand4 e4 = {0x00f0000fu + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
+    int it = 0, rs = turn, raw_phase = 0, s = turn, phase = 0;
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+      const PackedUnit un = unit_of(h, u, kblocks);
+      const int row = min(un.n0 + r, a.V - 1), kb_end = un.kb0 + un.kblocks;
+      int kb = un.kb0 + ((turn - it) & (kTurns - 1));
+      int block = -1;
+      if (kFmt == 2 && kb < kb_end) {
+        sp = reinterpret_cast<const uint16_t*>(a.scale) + static_cast<size_t>(row) * groups;
+        if (a.zero) zp = reinterpret_cast<const uint16_t*>(a.zero) + static_cast<size_t>(row) * groups;
+        if (eights) load8((kb * kBK) >> (shift + 3));
+        else load_runs(kb);
+      }
+      for (; kb < kb_end; kb += kTurns) {
+        const bool first_round = it + kb - un.kb0 < h.ring;
+        if (kFmt == 2 && (!eights || (kb * kBK) >> (shift + 3) != block)) {
+          sc = sc_next;
+          ze = ze_next;
+          block = (kb * kBK) >> (shift + 3);
+          if (eights) load8(block + 1);
+        }
+        ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase));
+        if (!ok) break;
+        const uint32_t src = raw + rs * kRawBytes;
+        uint4 q[kFmt == 1 ? 4 : 2];
+#pragma unroll
+        for (int c = 0; c < (kFmt == 1 ? 4 : 2); ++c) q[c] = lds16(src + ((16 * c) ^ raw_swz));
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
+        ok = __all_sync(0xffffffffu, first_round || wait(empty[s], phase ^ 1));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        Group4 g;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 32 weights at a time: the whole K block's would take too many registers
+          uint32_t o[16];
+          if (kFmt == 1) {
+            const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint2 p = expand8(w[i]);
+              o[2 * i] = p.x;
+              o[2 * i + 1] = p.y;
+            }
+          } else {
+            if (c == 0 || shift == 5) {
+              const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
+              g = group4(pick(sc, i), pick(ze, i));
+            }
+            const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 p = expand4(w[j], g, e4);
+              o[4 * j] = p.x;
+              o[4 * j + 1] = p.y;
+              o[4 * j + 2] = p.z;
+              o[4 * j + 3] = p.w;
+            }
+          }
+          tmem_st16(operand + s * kOperandCols + 16 * c, o);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        if (kFmt == 2 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&full[s]));
+        rs += kTurns;
+        if (rs >= h.raws) { rs -= h.raws; raw_phase ^= 1; }
+        s += kTurns;
+        if (s >= h.ring) { s -= h.ring; phase ^= 1; }
+      }
+      it += un.kblocks;
+    }
+  }
+  if (!ok) failed = 1;
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0 && failed && timeout) atomicOr(timeout, kTimeoutGemm);
+  __syncwarp();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+// Blocks of rows as equal as sixteens allow, at most kMaxBlockRows each.
+inline void set_row_blocks(PackedShape* h, int rows) {
+  h->rows = rows;
+  h->row_blocks = (rows + kMaxBlockRows - 1) / kMaxBlockRows;
+  h->block_rows = ((rows + h->row_blocks - 1) / h->row_blocks + 15) & ~15;
+}
+
+template <int kFmt, class Epi>
+int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, PackedShape h, const Epi& epi, int sms) {
+  PackedMaps maps;
+  int s = encode_map(what, &maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, h.rows, a.K, kBK, h.block_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (s == kOk)
+    s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.V, kFmt == 1 ? a.K : a.K / 2, raw_row<kFmt>(), kTileToks,
+                   kFmt == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  if (s != kOk) return s;
+  constexpr int kRawBytes = kTileToks * raw_row<kFmt>();
+  const int budget = static_cast<int>(kSmemBytes) - 1024 - Epi::kScratch;
+  for (h.raws = kMaxRing;; h.raws = kTurns) {  // the rows of x go first: four stages of them at least
+    h.ring = std::min(kMaxRing, (budget - h.raws * kRawBytes) / (h.block_rows * 128));
+    if (h.ring >= kTurns || h.raws == kTurns) break;
+  }
+  const size_t smem = 1024 + Epi::kScratch + static_cast<size_t>(h.ring) * h.block_rows * 128 + static_cast<size_t>(h.raws) * kRawBytes;
+  RK_REQUIRE(h.ring >= kTurns, kShape, "%s: no room for four stages", what);
+  const auto kernel = tc_packed_kernel<kFmt, Epi>;
+  RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
+  RK_CUDA(launch_pdl(kernel, dim3(std::min(h.units, sms)), dim3(kPackedThreads), smem, stream, maps, a, h, epi, timeout_word_or_null()));
+  RK_LAUNCH_CHECK(what);
+  return kOk;
+}
+
+}  // namespace tc
+}  // namespace rk

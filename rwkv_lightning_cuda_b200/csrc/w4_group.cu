@@ -25,7 +25,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
-#include "tc_rows.cuh"
+#include "tc_packed.cuh"
 #include "tensormap.h"
 
 namespace rk {
@@ -575,55 +575,69 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
   return matvec(stream, a, p, true);
 }
 
-// ---- more rows: the tensor-core skeleton of tc_rows.cuh, weights rounded to half
+// ---- more rows: the tensor-core skeleton of tc_packed.cuh, weights rounded to half
 namespace {
 
-// A row's results of a unit to y, or to the unit's plane of partial sums.
+__device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void sts2(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
+
+// A token's (channel's) results for the unit's rows to y, or to the unit's plane of partial sums; a warp's 32 channels are neighbours.
 struct ProductEpilogue {
+  static constexpr int kScratch = 4 * 2048;
   void* y;
   float* partial;  // [splits][rows][N], or nullptr
   int n_rows, N, epi;
-  size_t at;  // of the row's first result of the unit
+  int n;
+  size_t at;  // of the first row's result
   float* plane;
-  __device__ __forceinline__ int rows() const { return n_rows; }
-  __device__ __forceinline__ void begin(int row, int n0, int, int split) {
-    at = static_cast<size_t>(row) * N + n0;
+  uint32_t tile;  // this warp's part of the scratch
+  __device__ __forceinline__ void begin(int channel, int r0, int, int split, unsigned char* scratch) {
+    n = channel;
+    at = static_cast<size_t>(r0) * N + n;
     plane = partial ? partial + static_cast<size_t>(split) * n_rows * N : nullptr;
+    tile = smem_u32(scratch) + (threadIdx.x >> 5 & 3) * 2048;
   }
+  // A lane has a channel of 32 rows; a warp's stores of one row each, 64 or 128 bytes, took 90 to 110 clocks apiece (11,000 of a
+  // unit of 96 rows), so the rows change places in shared memory and leave 16 bytes a lane.
   __device__ __forceinline__ void chunk(int c, float (&z)[32], int here) {
-    const size_t o = at + c;
-    if (plane) {  // (N is a multiple of four)
-#pragma unroll
-      for (int i = 0; i < 32; i += 4)
-        if (i < here) *reinterpret_cast<float4*>(plane + o + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) z[i] = w4_epilogue(z[i], epi);
-    if (epi == kEpiF32) {
-      float* y32 = static_cast<float*>(y) + o;
+    const int lane = threadIdx.x & 31;
+    const size_t o = at + static_cast<size_t>(c) * N;
+    if (plane || epi == kEpiF32) {
+      float* const to = plane ? plane : static_cast<float*>(y);
       if (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          if (i < here) *reinterpret_cast<float4*>(y32 + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
-      } else {
+        for (int h = 0; h < 2; ++h) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sts4(tile + 128 * i + 4 * lane, __float_as_uint(plane ? z[16 * h + i] : w4_epilogue(z[16 * h + i], epi)));
+          __syncwarp();
+          const int col = n - lane + 4 * (lane & 7);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int i = 4 * j + (lane >> 3);
+            if (16 * h + i < here && col < N) *reinterpret_cast<uint4*>(to + o - n + col + static_cast<size_t>(16 * h + i) * N) = tc::lds16(tile + 512 * j + 16 * lane);
+          }
+        }
+      } else if (n < N) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (i < here) y32[i] = z[i];
+          if (i < here) to[o + static_cast<size_t>(i) * N] = plane ? z[i] : w4_epilogue(z[i], epi);
       }
-      return;
-    }
-    half* y16 = static_cast<half*>(y) + o;
-    if (N % 8 == 0) {
+    } else if (N % 8 == 0) {
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 32; i += 8)
-        if (i < here)
-          *reinterpret_cast<uint4*>(y16 + i) = make_uint4(h2u(__floats2half2_rn(z[i], z[i + 1])), h2u(__floats2half2_rn(z[i + 2], z[i + 3])),
-                                                          h2u(__floats2half2_rn(z[i + 4], z[i + 5])), h2u(__floats2half2_rn(z[i + 6], z[i + 7])));
-    } else {
+      for (int i = 0; i < 32; ++i) sts2(tile + 64 * i + 2 * lane, __half_as_ushort(__float2half_rn(w4_epilogue(z[i], epi))));
+      __syncwarp();
+      const int col = n - lane + 8 * (lane & 3);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 8 * j + (lane >> 2);
+        if (i < here && col < N) *reinterpret_cast<uint4*>(static_cast<half*>(y) + o - n + col + static_cast<size_t>(i) * N) = tc::lds16(tile + 512 * j + 16 * lane);
+      }
+    } else if (n < N) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i < here) y16[i] = __float2half_rn(z[i]);
+        if (i < here) static_cast<half*>(y)[o + static_cast<size_t>(i) * N] = __float2half_rn(w4_epilogue(z[i], epi));
     }
   }
   __device__ __forceinline__ void end() {}
@@ -647,41 +661,40 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
     *reinterpret_cast<uint2*>(static_cast<half*>(p.y) + i) = make_uint2(h2u(__floats2half2_rn(e[0], e[1])), h2u(__floats2half2_rn(e[2], e[3])));
 }
 
-// Token tiles and K ranges with the least time by this account, in clocks of an SM: a K block takes some 1000 whatever its width
-// (measured 1000 at 80 tokens, 1060 at 224: the issuing thread's waits and the shared-memory traffic of the expansion), a
-// unit 2500 to begin and end, the second kernel 6000 and its traffic.
-tc::Shape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
-  tc::Shape best = {};
+// K ranges with the least time by this account, in clocks of an SM: a K block takes the expansion 420, or the tensor cores 2.35 a
+// row; a unit's results take 50 a row, hidden under the next unit's products where there are two accumulators; the second
+// kernel 3000 and its traffic.  (24 rows of 2048 x 8192: 36.1 us whole, 11.4 in eight ranges; 96 rows of 10240 x 2560: 17.1 whole,
+// 19.4 in two, 16.1 in three; 256 rows of 2560 x 10240: 58 whole, 22.0 in six, 32.3 in eight, which is a second wave.)
+tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
+  tc::PackedShape best = {};
   double least = 0;
   const int kblocks = (K + tc::kBK - 1) / tc::kBK;
   const size_t plane = static_cast<size_t>(M) * N;
-  for (int toks = tc::kToks; toks >= 64; toks -= 16)
-    for (int want = 1; want <= 16 && want <= kblocks; ++want) {
-      tc::Shape h;
-      h.toks = toks;
-      h.tiles = (N + toks - 1) / toks;
-      h.row_blocks = (M + tc::kRows - 1) / tc::kRows;
-      h.x_rows = std::min(tc::kRows, (M + 7) & ~7);
-      h.kb_per_split = (kblocks + want - 1) / want;
-      h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
-      if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
-      const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
-      double cost = static_cast<double>((units + sms - 1) / sms) * (h.kb_per_split * (950.0 + 0.5 * toks) + 2500);
-      if (h.splits > 1) cost += 6000 + 4.0 * (h.splits + 1) * plane / (24.0 * sms);
-      h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
-      if (best.toks == 0 || cost < least) { least = cost; best = h; }
-    }
+  for (int want = 1; want <= 16 && want <= kblocks; ++want) {
+    tc::PackedShape h = {};
+    tc::set_row_blocks(&h, M);
+    h.tiles = (N + tc::kTileToks - 1) / tc::kTileToks;
+    h.kb_per_split = (kblocks + want - 1) / want;
+    h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
+    if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
+    const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
+    const double waves = static_cast<double>((units + sms - 1) / sms), results = 50.0 * h.block_rows;
+    double cost = waves * (h.kb_per_split * std::max(420.0, 2.35 * h.block_rows)) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
+    if (h.splits > 1) cost += 3000 + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
+    h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
+    if (best.units == 0 || cost < least) { least = cost; best = h; }
+  }
   return best;
 }
 
 int many_rows(cudaStream_t stream, const W4GroupArgs& a, float* scratch, size_t scratch_bytes, int sms) {
-  const tc::Shape h = many_rows_shape(a.M, a.K, a.N, scratch ? scratch_bytes / sizeof(float) : 0, sms);
+  const tc::PackedShape h = many_rows_shape(a.M, a.K, a.N, scratch ? scratch_bytes / sizeof(float) : 0, sms);
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "linear_w4a16_group: too many rows");
-  tc::Weights w;
+  tc::Packed w;
   w.V = a.N; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
   ProductEpilogue epi;
   epi.y = a.y; epi.partial = h.splits > 1 ? scratch : nullptr; epi.n_rows = a.M; epi.N = a.N; epi.epi = a.epi;
-  const int s = tc::launch_rows<2>(stream, "linear_w4a16_group", a.x, a.M, a.q, w, h, epi, sms);
+  const int s = tc::launch_packed<2>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms);
   if (s != kOk || h.splits == 1) return s;
   const size_t quads = static_cast<size_t>(a.M) * a.N / 4;
   RK_CUDA(launch_pdl(w4_reduce_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, epi, h.splits));
@@ -695,7 +708,7 @@ size_t w4_group_workspace(int M, int K, int N) {
   if (M <= kMatvecRows || N % 4 != 0) return 0;
   int sms = 148;
   if (device_sms(&sms) != kOk) sms = 148;
-  const tc::Shape h = many_rows_shape(M, K, N, ~static_cast<size_t>(0) / 8, sms);
+  const tc::PackedShape h = many_rows_shape(M, K, N, ~static_cast<size_t>(0) / 8, sms);
   return h.splits > 1 ? static_cast<size_t>(h.splits) * M * N * sizeof(float) : 0;
 }
 
