@@ -60,15 +60,17 @@ struct StatsEpilogue {
 // The same where a thread has one token and all rows: 32 tokens x 32 rows at a time go through shared memory, after which a lane has
 // one row's 32 tokens; the four warps' parts of a row are merged at the end of the unit.
 struct PackedStatsEpilogue {
-  static constexpr int kPitch = 33, kWarpFloats = 32 * kPitch, kParts = 4 * tc::kMaxBlockRows;
+  static constexpr int kPitch = 36, kWarpFloats = 32 * kPitch, kParts = 4 * tc::kMaxBlockRows;
   static constexpr int kScratch = 4 * kWarpFloats * 4 + kParts * 16;
   float4* part;   // [tiles][rows]
   float* given;   // [rows]
   const int64_t* tokens;
   int n_rows, V;
   int token, r0, rows, lane, quad;
-  float* box;       // this warp's [row][token]
+  int64_t id;       // asked of the next chunk's row, on its way since the chunk before
+  float* box;       // this warp's [row][token]: written by columns, read by 16 bytes, neither with a conflict
   float4* parts;    // [warp][row of the block]
+  __device__ __forceinline__ int64_t asked(int c) const { return tokens && c + lane < rows ? tokens[r0 + c + lane] : -1; }
   __device__ __forceinline__ void begin(int tok, int first, int rows_here, int, unsigned char* scratch) {
     token = tok;
     r0 = first;
@@ -77,22 +79,37 @@ struct PackedStatsEpilogue {
     quad = (threadIdx.x >> 5) & 3;
     box = reinterpret_cast<float*>(scratch) + quad * kWarpFloats;
     parts = reinterpret_cast<float4*>(scratch + 4 * kWarpFloats * 4);
+    id = asked(0);
   }
   __device__ __forceinline__ void chunk(int c, float (&z)[32], int here) {
+    const int64_t at = id - (token - lane);  // relative to the warp's first token
+    const bool mine = id >= 0 && at >= 0 && at < 32 && id < V;
+    id = asked(c + 32);
 #pragma unroll
     for (int i = 0; i < 32; ++i) box[i * kPitch + lane] = token < V ? z[i] : -INFINITY;
     __syncwarp();
     if (lane < here) {
-      const int64_t id = tokens ? tokens[r0 + c + lane] - (token - lane) : -1;  // relative to the warp's first token
-      if (id >= 0 && id < 32 && token - lane + id < V) given[r0 + c + lane] = box[lane * kPitch + id];
-      SoftStats st;
-      float m = st.m;
+      const float4* row = reinterpret_cast<const float4*>(box + lane * kPitch);
+      float v[32];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) m = max_nan(m, box[lane * kPitch + i]);
-      st.m = m;
+      for (int i = 0; i < 8; ++i) {
+        const float4 q = row[i];
+        v[4 * i] = q.x;
+        v[4 * i + 1] = q.y;
+        v[4 * i + 2] = q.z;
+        v[4 * i + 3] = q.w;
+      }
+      if (mine) given[r0 + c + lane] = box[lane * kPitch + at];
+      SoftStats st[4];  // chains of their own
 #pragma unroll
-      for (int i = 0; i < 32; ++i) add(st, box[lane * kPitch + i]);
-      parts[quad * tc::kMaxBlockRows + c + lane] = make_float4(st.m, st.s, st.t, 0.f);
+      for (int i = 0; i < 32; ++i) st[i & 3].m = max_nan(st[i & 3].m, v[i]);
+      const float m = max_nan(max_nan(st[0].m, st[1].m), max_nan(st[2].m, st[3].m));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) st[i].m = m;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) add(st[i & 3], v[i]);
+      parts[quad * tc::kMaxBlockRows + c + lane] =
+          make_float4(m, (st[0].s + st[1].s) + (st[2].s + st[3].s), (st[0].t + st[1].t) + (st[2].t + st[3].t), 0.f);
     }
     __syncwarp();
   }

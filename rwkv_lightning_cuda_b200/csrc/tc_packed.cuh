@@ -112,9 +112,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       : "memory");
 }
 
-// Epi: a copy per epilogue thread and unit, all 128 of which are asked; begin(token, r0, rows, split, scratch), then chunk(c, z, here) for every
-// 32 rows r0 + c .. (here of them valid), where z[i] is the result of row r0 + c + i, then end(); scratch: Epi::kScratch bytes of shared
-// memory.  The threads may meet at barrier 1.
+// Epi: a copy per epilogue thread and unit, all 128 of which are asked; begin(token, r0, rows, split, scratch) while the products are under
+// way, then chunk(c, z, here) for every 32 rows r0 + c .. (here of them valid), where z[i] is the result of row r0 + c + i, then end();
+// scratch: Epi::kScratch bytes of shared memory.  The threads may meet at barrier 1.
 template <int kFmt, class Epi>
 __global__ void __launch_bounds__(kPackedThreads, 1)
     tc_packed_kernel(const __grid_constant__ PackedMaps maps, const Packed a, const PackedShape h, const Epi epilogue, int* timeout) {
@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.w) : "memory");
+  if (warp == 6 && lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.x) : "memory");
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -216,6 +218,8 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       const int token = un.n0 + quad * 32 + lane, rows = min(h.block_rows, h.rows - un.r0);
       const float scale = kFmt == 1 && token < a.V ? __half2float(a.scale[token]) : 1.f;
       const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
+      Epi epi = epilogue;
+      epi.begin(token, un.r0, rows, un.split, scratch);
       // (asleep: these four warps' polling of a wait this long cost the expansion a quarter of its time)
       for (uint32_t i = 0; i < kSpinLimit && !(ok = mbar_test(smem_u32(&acc_full[acc]), use & 1)) && !failed; ++i) __nanosleep(100);
       {  // all four warps stay or leave together: an epilogue may have them meet at a barrier
@@ -225,8 +229,6 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       }
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      Epi epi = epilogue;
-      epi.begin(token, un.r0, rows, un.split, scratch);
       for (int c = 0; c < rows; c += 32) {
         float z[32];
         tmem_ld32(tmem + acc * 128 + c + (static_cast<uint32_t>(quad * 32) << 16), z);

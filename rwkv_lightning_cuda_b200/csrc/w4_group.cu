@@ -579,7 +579,6 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
 namespace {
 
 __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ void sts2(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
 
 // A token's (channel's) results for the unit's rows to y, or to the unit's plane of partial sums; a warp's 32 channels are neighbours.
 struct ProductEpilogue {
@@ -623,16 +622,25 @@ struct ProductEpilogue {
         for (int i = 0; i < 32; ++i)
           if (i < here) to[o + static_cast<size_t>(i) * N] = plane ? z[i] : w4_epilogue(z[i], epi);
       }
-    } else if (N % 8 == 0) {
+    } else if (N % 8 == 0) {  // two rows of a channel share a word: 8 words are 8 channels of both
+      if (epi == kEpiRelu2) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = w4_epilogue(z[i], kEpiRelu2);
+      }
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sts2(tile + 64 * i + 2 * lane, __half_as_ushort(__float2half_rn(w4_epilogue(z[i], epi))));
+      for (int i = 0; i < 16; ++i) sts4(tile + 128 * i + 4 * lane, h2u(__floats2half2_rn(z[2 * i], z[2 * i + 1])));
       __syncwarp();
       const int col = n - lane + 8 * (lane & 3);
+      half* const to = static_cast<half*>(y) + o - n + col;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 8 * j + (lane >> 2);
-        if (i < here && col < N) *reinterpret_cast<uint4*>(static_cast<half*>(y) + o - n + col + static_cast<size_t>(i) * N) = tc::lds16(tile + 512 * j + 16 * lane);
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * (8 * j + (lane >> 2));
+        const uint4 a = tc::lds16(tile + 1024 * j + 32 * lane), b = tc::lds16(tile + 1024 * j + 32 * lane + 16);
+        const uint4 even = {__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.z, a.w, 0x5410), __byte_perm(b.x, b.y, 0x5410), __byte_perm(b.z, b.w, 0x5410)};
+        const uint4 odd = {__byte_perm(a.x, a.y, 0x7632), __byte_perm(a.z, a.w, 0x7632), __byte_perm(b.x, b.y, 0x7632), __byte_perm(b.z, b.w, 0x7632)};
+        if (i < here && col < N) *reinterpret_cast<uint4*>(to + static_cast<size_t>(i) * N) = even;
+        if (i + 1 < here && col < N) *reinterpret_cast<uint4*>(to + static_cast<size_t>(i + 1) * N) = odd;
       }
     } else if (n < N) {
 #pragma unroll
@@ -662,9 +670,10 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
 }
 
 // K ranges with the least time by this account, in clocks of an SM: a K block takes the expansion 420, or the tensor cores 2.35 a
-// row; a unit's results take 50 a row, hidden under the next unit's products where there are two accumulators; the second
-// kernel 3000 and its traffic.  (24 rows of 2048 x 8192: 36.1 us whole, 11.4 in eight ranges; 96 rows of 10240 x 2560: 17.1 whole,
-// 19.4 in two, 16.1 in three; 256 rows of 2560 x 10240: 58 whole, 22.0 in six, 32.3 in eight, which is a second wave.)
+// row; a unit's results take 25 a row, hidden under the next unit's products where there are two accumulators; the second
+// kernel 3000, 200 a range and its traffic.  (64 rows of 1024 x 1024: 7.5 us whole, 6.5 in eight ranges, 7.9 in sixteen; 96 rows
+// of 10240 x 2560: 15.7 whole, 19.0 in two, 16.2 in three; 96 rows of 2560 x 10240: 43.7 whole, 15.7 in seven, 19.6 in nine, which
+// is a second wave.)
 tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
   tc::PackedShape best = {};
   double least = 0;
@@ -678,9 +687,9 @@ tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int 
     h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
-    const double waves = static_cast<double>((units + sms - 1) / sms), results = 50.0 * h.block_rows;
+    const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;
     double cost = waves * (h.kb_per_split * std::max(420.0, 2.35 * h.block_rows)) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
-    if (h.splits > 1) cost += 3000 + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
+    if (h.splits > 1) cost += 3000 + 200 * h.splits + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
     if (best.units == 0 || cost < least) { least = cost; best = h; }
   }
