@@ -78,14 +78,20 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // The eight weights of a word as pairs (0, 4), (1, 5), (2, 6), (3, 7): a nibble under the exponent of 1024 is 1024 + q, a high one
-// 1024 + 16 q; less 1024 + zero (or / 16 less 64 + zero) that is q - zero exactly, and the product rounds once.
-__device__ __forceinline__ void round4(uint32_t u, __half2 s, __half2 zlo, __half2 zhi, uint32_t (&o)[4]) {
+// 1024 + 16 q; less 1024 + zero (or / 16 less 64 + zero) that is q - zero exactly, and the product rounds once.  one: 0x64006400 in a
+// register of the caller's (as a literal beside the mask it would take an instruction of its own).
+template <uint32_t kMask> __device__ __forceinline__ __half2 under_1024(uint32_t u, uint32_t one) {
+  uint32_t v;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(u), "n"(kMask), "r"(one));  // (u & mask) | one
+  return u2h(v);
+}
+__device__ __forceinline__ void round4(uint32_t u, uint32_t one, __half2 s, __half2 zlo, __half2 zhi, uint32_t (&o)[4]) {
   const uint32_t v = u >> 8;
   const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
-  o[0] = h2u(__hmul2(__hsub2(u2h((u & 0x000f000fu) | 0x64006400u), zlo), s));
-  o[1] = h2u(__hmul2(__hfma2(u2h((u & 0x00f000f0u) | 0x64006400u), sixteenth, zhi), s));
-  o[2] = h2u(__hmul2(__hsub2(u2h((v & 0x000f000fu) | 0x64006400u), zlo), s));
-  o[3] = h2u(__hmul2(__hfma2(u2h((v & 0x00f000f0u) | 0x64006400u), sixteenth, zhi), s));
+  o[0] = h2u(__hmul2(__hsub2(under_1024<0x000f000fu>(u, one), zlo), s));
+  o[1] = h2u(__hmul2(__hfma2(under_1024<0x00f000f0u>(u, one), sixteenth, zhi), s));
+  o[2] = h2u(__hmul2(__hsub2(under_1024<0x000f000fu>(v, one), zlo), s));
+  o[3] = h2u(__hmul2(__hfma2(under_1024<0x00f000f0u>(v, one), sixteenth, zhi), s));
 }
 __device__ __forceinline__ float half_of(uint32_t pair, int i) {
   const float2 f = h2f2(pair);
@@ -256,6 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
   for (int b = 0; b < kBlk; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
+  const uint32_t one = 0x64006400u + (base >> 30);  // (a shared-memory address is below 2^30, which the compiler does not know)
   int cur = 0, slot = 0, phase = 0;
   bool dead = false;  // a wait ran out: no more work, but the barriers are kept
   for (;;) {
@@ -343,14 +350,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
                 const uint32_t s2 = __byte_perm(sp, 0u, sel), z2 = __byte_perm(zp, 0u, sel);
                 scale2[i] = u2h(s2);
                 zero_lo[i] = __hadd2(u2h(z2), __floats2half2_rn(1024.f, 1024.f));
-                zero_hi[i] = __hneg2(__hadd2(u2h(z2), __floats2half2_rn(64.f, 64.f)));
+                zero_hi[i] = __hfma2(u2h(z2), __floats2half2_rn(-1.f, -1.f), __floats2half2_rn(-64.f, -64.f));
               }
             }
 #pragma unroll
             for (int b = 0; b < kBlk; ++b) {
               uint32_t ra[4], rb[4];
-              round4(w[b][2 * cc], scale2[2 * b], zero_lo[2 * b], zero_hi[2 * b], ra);
-              round4(w[b][2 * cc + 1], scale2[2 * b + 1], zero_lo[2 * b + 1], zero_hi[2 * b + 1], rb);
+              round4(w[b][2 * cc], one, scale2[2 * b], zero_lo[2 * b], zero_hi[2 * b], ra);
+              round4(w[b][2 * cc + 1], one, scale2[2 * b + 1], zero_lo[2 * b + 1], zero_hi[2 * b + 1], rb);
               mma16816(lo[b], ra[0], rb[0], ra[2], rb[2], xv.x, xv.y, c == 0);
               mma16816(hi[b], ra[1], rb[1], ra[3], rb[3], xv.z, xv.w, c == 0);
               if (c == 7) {
