@@ -4,9 +4,10 @@
 // Bound by reading the logits once; a single row by latency.  A row goes to one CTA, or to the CTAs of a cluster when
 // there are too few rows to fill the GPU: each takes a contiguous part and leaves its statistics and alternatives in the
 // first one's shared memory, so there is no scratch, no second launch and no atomic whose order could show.
-// A thread keeps 16 logits in registers and the next 16 under way, and its own running maximum (one rescaling per 16).  At the HBM's
-// rate an SM has 2 issue slots per fp16 logit and 4 per fp32 one, so what a logit costs counts: half a maximum and half a
-// minimum (three operands at a time), and one multiply-add, one exp2, an addition and a multiply-add for its part of the sums.
+// A thread keeps 16 logits in registers and the next 16 under way, and its own running maximum (one rescaling per 16).  What a
+// logit costs counts: half a maximum (a third with fp32), an exp2, and the multiply-adds and additions of its sums two logits at a
+// time.  4096 rows of 65536: fp32 164 us, what the HBM takes (6.5 TB/s); fp16 105 us (5.1 TB/s), the exp2 units busy for 72 of them
+// and the issue slots for 73.  (Two steps of fp16 under way instead of one: 114 us.)
 //
 // Alternatives without a pass over the rest: the k-th largest of the maxima of 64 disjoint groups of threads is a lower
 // bound of the k-th largest logit, and only about k logits reach it.  Every thread has left the maxima of 16 stretches
@@ -101,60 +102,74 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float min3(float a, float b, float c) {
-  float r;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-// The largest (NaN if there is one) and the smallest of a step's logits.
+// The largest of a step's logits, NaN if there is one.
 template <int kVecs>
-__device__ __forceinline__ void extremes(const uint4 (&q)[kVecs], float* hi, float* lo, float) {
-  float a = __uint_as_float(q[0].x), b = a;
+__device__ __forceinline__ float largest_of(const uint4 (&q)[kVecs], float) {
+  float a = __uint_as_float(q[0].x);
 #pragma unroll
   for (int j = 0; j < kVecs; ++j) {
     const float x = __uint_as_float(q[j].x), y = __uint_as_float(q[j].y), z = __uint_as_float(q[j].z), w = __uint_as_float(q[j].w);
     a = max3_nan(max3_nan(a, x, y), z, w);
-    b = min3(min3(b, x, y), z, w);
   }
-  *hi = a;
-  *lo = b;
+  return a;
 }
 template <int kVecs>
-__device__ __forceinline__ void extremes(const uint4 (&q)[kVecs], float* hi, float* lo, half) {
-  __half2 a = *reinterpret_cast<const __half2*>(&q[0].x), b = a;
+__device__ __forceinline__ float largest_of(const uint4 (&q)[kVecs], half) {
+  __half2 a = *reinterpret_cast<const __half2*>(&q[0].x);
 #pragma unroll
   for (int j = 0; j < kVecs; ++j) {
     const uint32_t w[4] = {q[j].x, q[j].y, q[j].z, q[j].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a = __hmax2_nan(a, *reinterpret_cast<const __half2*>(&w[i]));
-      b = __hmin2(b, *reinterpret_cast<const __half2*>(&w[i]));
-    }
+    for (int i = 0; i < 4; ++i) a = __hmax2_nan(a, *reinterpret_cast<const __half2*>(&w[i]));
   }
-  const float2 x = __half22float2(a), y = __half22float2(b);
-  *hi = max_nan(x.x, x.y);
-  *lo = fminf(y.x, y.y);
+  const float2 x = __half22float2(a);
+  return max_nan(x.x, x.y);
+}
+
+// Two fp32 at a time: an instruction each, with the roundings of the single ones.
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ float2 both() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r(0.f, 0.f);
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r(0.f, 0.f);
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
 }
 
 // A step's 16 logits at the maximum that is in place.  2^((z - m) log2 e) as 2^(y - r) with y = z log2 e - M, M = fl(m log2 e)
-// and r = m log2 e - M, each one rounding of an exact product: r is the same for all and comes off the sums.  Needs
-// products that do not overflow; the other rows (masked tokens among them) go logit by logit.
-__device__ __forceinline__ void add_step(SoftStats& st, const float* v, float lo) {
-  if (lo >= -1e38f && fabsf(st.m) <= 1e38f) {
-    const float M = st.m * kLog2e, r = fmaf(st.m, kLog2e, -M);
-    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f;
+// and r = m log2 e - M, each one rounding of an exact product: r is the same for all and comes off the sums.  Needs products
+// that do not overflow.  One that does, of a masked token or a logit below -2.3e38, is a y of -inf, whose 0 * y makes t NaN: such
+// steps, and rows of a maximum beyond 1e38, go logit by logit.  (Looking for the smallest logit instead took half an instruction
+// per logit of the ten or so that bound this kernel; the sums two at a time save one and a half.)
+__device__ __forceinline__ void add_step(SoftStats& st, const float* v) {
+  const float M = st.m * kLog2e, r = fmaf(st.m, kLog2e, -M);
+  const F2 scale(kLog2e, kLog2e), less(-M, -M);
+  F2 s2(0.f, 0.f), t2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-      const float y0 = fmaf(v[i], kLog2e, -M), y1 = fmaf(v[i + 1], kLog2e, -M);
-      const float e0 = exp2f(y0), e1 = exp2f(y1);
-      s0 += e0;
-      s1 += e1;
-      t0 = fmaf(e0, y0, t0);
-      t1 = fmaf(e1, y1, t1);
-    }
-    const float f = exp2f(-r), sum = s0 + s1;
+  for (int i = 0; i < 16; i += 2) {
+    const F2 y = fma2(F2(v[i], v[i + 1]), scale, less);
+    const float2 p = y.both();
+    const F2 e(exp2f(p.x), exp2f(p.y));
+    s2 = add2(s2, e);
+    t2 = fma2(e, y, t2);
+  }
+  const float2 s = s2.both(), t = t2.both();
+  const float sum = s.x + s.y, weighted = t.x + t.y;
+  if (fabsf(st.m) <= 1e38f && weighted == weighted) {
+    const float f = exp2f(-r);
     st.s = fmaf(f, sum, st.s);
-    st.t = fmaf(f * 0.6931471805599453f, fmaf(-r, sum, t0 + t1), st.t);
+    st.t = fmaf(f * 0.6931471805599453f, fmaf(-r, sum, weighted), st.t);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) add(st, v[i]);
@@ -240,14 +255,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(co
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) q[j] = next[j];
     if (i + 1 < steps) fetch(i + 1, next);
-    float hi, lo;
-    extremes(q, &hi, &lo, T(0));
+    const float hi = largest_of(q, T(0));
     const float m = max_nan(st.m, hi);
     if (m != st.m) raise(st, m);
     float v[16];
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) unpack(q[j], v + j * kVec, T(0));
-    add_step(st, v, lo);
+    add_step(st, v);
     if (kTop) {
       highest = in == 0 ? hi : fmaxf(highest, hi);
       if (++in == stretch || i + 1 == steps) {
