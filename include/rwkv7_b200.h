@@ -386,7 +386,7 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
                             const uint16_t* scale, const uint16_t* zero, int epilogue, void* y);
 /* 4-bit weights with group scales (no counterpart in the reference): W[n,k] = (q[n,k] - zero[n,g]) * scale[n,g] with
  * g = k / group, group 32, 64 or 128, a short last group allowed (scale and zero are [N][ceil(K / group)]), zero NULL: 8
- * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 16 rows
+ * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 8 rows
  * the scale multiplies the group's fp32 sum, so no weight is rounded; with more rows weights count as
  * half((q - zero) * scale).  workspace is scratch of the size the first function returns (which may be 0); without it, or
  * with less, products of many rows run on fewer SMs.  Calls that may overlap on the GPU need one each. */

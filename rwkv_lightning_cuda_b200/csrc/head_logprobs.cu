@@ -4,7 +4,8 @@
 // where it is computed, and a second kernel merges a row's tiles (logprob.cuh).  fp16 operands, fp32 sums; int8 weights
 // are exact integers with the channel's scale on the sum, 4-bit weights half((q - zero) * scale).
 //
-// Bound by the weights' bytes up to some 256 rows, by the tensor cores above.  The products are tc_rows.cuh's (fp16 weights) and
+// Bound by the weights' bytes up to some 256 rows of fp16 weights, by the tensor cores above, and by the expansion of quantised ones in
+// between (128 x 65536 x 4096 fp16: 94 us, 5.7 TB/s; 2048 rows: 780 to 880 us as the power cap lets it).  The products are tc_rows.cuh's (fp16 weights) and
 // tc_packed.cuh's (quantised ones); here are their epilogues, which reduce a tile of logits to (m, s, t) per row, the merging of the
 // tiles, and the route for a few rows.
 #include <algorithm>
@@ -212,13 +213,13 @@ int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
 
 }  // namespace
 
-// Few rows: the weight-streaming kernels read the weights once at a better rate than the kernel above with its 128-row tiles
-// and expansion through shared memory, and the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said
-// otherwise), this route against the other: 4-bit 53 against 90 us at one row, 61 against 91 at eight (31 against 48 at two
-// and K = 2048); int8 61 against 74 us at four rows; fp16 84 against 94 us at one row, but 111 against 94 at four.  In
-// small matrices of 8- and 16-bit weights the second pass costs more than it saves (32003 x 768 int8: 18.5 against 15.5 us).
+// Few rows: the weight-streaming kernels read the weights once at a better rate than the kernels above with their 128-row or
+// 128-token tiles, and the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said otherwise), this
+// route against the other: 4-bit 50 us against 74 at eight rows (33 against 43 at K = 2048, 23 against 27 at K = 1024); int8 58
+// against 70 at four rows; fp16 83 against 91 at one row, but 111 against 94 at four.  In small matrices of 8- and 16-bit weights
+// the second pass costs more than it saves (int8 65536 x 1024 at two rows: 31 us against 24; 65536 x 2560: 42 against 47).
 constexpr int kFewRowsF16 = 1, kFewRowsW8 = 4, kFewRowsW4 = 8;
-constexpr double kFewRowsBytes = 64e6;
+constexpr double kFewRowsBytes = 128e6;
 
 size_t head_logprobs_workspace(int rows, int V) {
   const size_t tiles = (static_cast<size_t>(V) + kMinToks - 1) / kMinToks;

@@ -9,6 +9,10 @@
 // memory is a token, a column a row of x.  Up to 128 rows in a block there are two accumulators, and a unit's epilogue runs
 // under the next one's products; with more there is one.
 //
+// Bound up to 128 rows by the expansion, some 350 issue slots of each scheduler and 420 clocks for a K block of 4-bit weights, of which the
+// ANDs, permutations and half2 operations that a weight needs are 200; above by the tensor cores (24 rows of 65536 x 4096 in
+// 70 us, 256 rows of 16384 x 4096 in 32 us, 1.06 PFLOP/s).
+//
 // Warp roles: 0 loads packed tiles, 1 issues tcgen05.mma, 2..5 run the epilogue, 6 loads rows of x, 8..23 expand, four warps to a
 // K block in turn.  Every wait is bounded: one that runs out sets the device's failure word, every role leaves its loop, and the
 // CTA frees its tensor memory and returns.

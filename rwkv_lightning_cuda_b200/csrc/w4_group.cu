@@ -34,8 +34,9 @@ namespace {
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
 constexpr int kBoxWeights = 256;  // 128 bytes along a row: eight chunks of 32 weights
-constexpr int kMaxRows = 8;      // of a launch
-constexpr int kMatvecRows = 16;  // up to which the launches of eight rows are used, see w4_group_linear
+// Rows up to which the weights are streamed and never rounded.  Nine to sixteen rows in two such launches took 70 to 82 us at
+// 65536 x 4096, 24 at 16384 x 4096, 18 to 20 at 10240 x 2560 and 30 at 2560 x 10240; the kernel for many rows takes 69, 21, 15 and 13.
+constexpr int kMaxRows = 8;
 constexpr size_t kSmemLimit = 226 * 1024;
 
 struct MatvecMaps {
@@ -721,7 +722,7 @@ int many_rows(cudaStream_t stream, const W4GroupArgs& a, float* scratch, size_t 
 }  // namespace
 
 size_t w4_group_workspace(int M, int K, int N) {
-  if (M <= kMatvecRows || N % 4 != 0) return 0;
+  if (M <= kMaxRows || N % 4 != 0) return 0;
   int sms = 148;
   if (device_sms(&sms) != kOk) sms = 148;
   const tc::PackedShape h = many_rows_shape(M, K, N, ~static_cast<size_t>(0) / 8, sms);
@@ -738,7 +739,7 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, 
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
-  if (a.M > kMatvecRows) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
+  if (a.M > kMaxRows) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
   for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
     MatvecPlan p;

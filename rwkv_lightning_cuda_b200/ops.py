@@ -381,7 +381,7 @@ def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NO
         _refuse_linear_w4a16_group(x, q, scale, zero, group_size)
     y = torch.empty(M, N, dtype=_F32 if epilogue == L.EPI_F32 else _F16, device=dev)
     need, work = 0, None
-    if M > 16:
+    if M > 8:
         need = _scratch_bytes("rwkv7_b200_linear_w4a16_group_workspace", M, K, N)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(),

@@ -17,9 +17,9 @@ def ops():
 def check_product(y, x, weight, group, what):
     """fp32 sums of K products: at most K / 16 additions to one running sum and 64 more in the merges, each off by at most one step of what has
     been added up, codes and zeros apart: sum |x| (q + zero) scale.  Then one rounding to half (half a step, or of the smallest subnormal).
-    Beyond 16 rows the weights are rounded to half first."""
+    Beyond 8 rows the weights are rounded to half first."""
     x64 = x.cpu().double()
-    want = x64 @ w4_weights(*weight, group, rounded=x.shape[0] > 16).T
+    want = x64 @ w4_weights(*weight, group, rounded=x.shape[0] > 8).T
     size = x64.abs() @ w4_weights(*weight, group, parts=True).T
     bound = size * (x.shape[1] / 16 + 64) * 2 * U32 + want.abs() * U16 * (1 + 1e-3) + 2.0 ** -25
     got = y.detach().cpu().double()
