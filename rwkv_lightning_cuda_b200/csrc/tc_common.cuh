@@ -45,6 +45,11 @@ static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, const
     if (mbar_try_wait(bar, parity)) return true;
   return false;
 }
+// The wait of a kernel that has given up for its own copies and products in flight: a fraction of a second at most.
+static __device__ __noinline__ void settle(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 16); ++i)
+    if (mbar_try_wait(bar, parity)) return;
+}
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");

@@ -123,7 +123,7 @@ template <int kFmt, class Epi>
 __global__ void __launch_bounds__(kPackedThreads, 1)
     tc_packed_kernel(const __grid_constant__ PackedMaps maps, const Packed a, const PackedShape h, const Epi epilogue, int* timeout) {
   extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing], raw_full[kMaxRing], raw_empty[kMaxRing], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing], raw_full[kMaxRing], raw_empty[kMaxRing], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   constexpr uint32_t kRawBytes = kTileToks * raw_row<kFmt>();
@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       mbar_init(smem_u32(&acc_full[i]), 1);
       mbar_init(smem_u32(&acc_empty[i]), 4);
     }
+    mbar_init(smem_u32(&drained), 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -163,11 +164,12 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
 
   auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
   bool ok = true;
+  int it = 0;  // K blocks so far, of the roles that count them
   if (warp == 0 || warp == 6) {
     if (lane == 0) {
       const bool packed = warp == 0;
       const int stages = packed ? h.raws : h.ring;
-      int it = 0, s = 0, phase = 0;
+      int s = 0, phase = 0;
       for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
         const PackedUnit un = unit_of(h, u, kblocks);
         for (int kb = un.kb0; kb < un.kb0 + un.kblocks; ++kb, ++it) {
@@ -179,8 +181,6 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           if (++s == stages) { s = 0; phase ^= 1; }
         }
       }
-      if (!ok)  // leave no copy in flight behind
-        for (int i = it > stages ? it - stages : 0; i < it; ++i) mbar_wait(smem_u32(packed ? &raw_full[i % stages] : &full[i % stages]), (i / stages) & 1);
     }
   } else if (warp == 1) {
     // ---- products: K blocks of 64 as four instructions into the unit's accumulator.  The whole warp goes through the loop, so that the
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     const uint32_t none = ring >> 30;  // 0, which the compiler does not know, so that the constants stay in registers
     const uint32_t mul = 0x2c003c00u + none;
     const Expand4 e4 = {0x00f0000fu + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
-    int it = 0, rs = turn, raw_phase = 0, s = turn, phase = 0;
+    int rs = turn, raw_phase = 0, s = turn, phase = 0;
     for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
       const PackedUnit un = unit_of(h, u, kblocks);
       const int row = min(un.n0 + r, a.V - 1), kb_end = un.kb0 + un.kblocks;
@@ -353,6 +353,14 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0 && failed && timeout) atomicOr(timeout, kTimeoutGemm);
+  // One gave up: the copies in flight and the products issued end before the CTA does.
+  if (failed && (warp == 0 || warp == 6) && lane == 0) {
+    for (int i = max(it - (warp ? h.ring : h.raws), 0); i < it; ++i) settle(smem_u32(warp ? &full[i % h.ring] : &raw_full[i % h.raws]), (i / (warp ? h.ring : h.raws)) & 1);
+  }
+  if (failed && warp == 1 && elect_one()) {
+    commit(smem_u32(&drained));
+    settle(smem_u32(&drained), 0);
+  }
   __syncwarp();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }

@@ -38,7 +38,7 @@ template <class Epi>
 __global__ void __launch_bounds__(kRowsThreads, 1)
     tc_rows_kernel(const __grid_constant__ Maps maps, const int K, const int V, const Shape h, const Epi epilogue, int* timeout) {
   extern __shared__ unsigned char smem[];
-  __shared__ __align__(8) uint64_t full[kMaxTiles], empty[kMaxTiles], acc_full[2], acc_empty[2];
+  __shared__ __align__(8) uint64_t full[kMaxTiles], empty[kMaxTiles], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       mbar_init(smem_u32(&acc_full[i]), 1);
       mbar_init(smem_u32(&acc_empty[i]), 4);
     }
+    mbar_init(smem_u32(&drained), 1);
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -70,9 +71,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 
   auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
   bool ok = true;
+  int it = 0;  // K blocks so far, of the roles that count them
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0, s = 0, phase = 0;
+      int s = 0, phase = 0;
       for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
         const int r0 = u % h.row_blocks * kRows, n0 = u / h.row_blocks * h.toks;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
@@ -84,8 +86,6 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
           if (++s == h.ring) { s = 0; phase ^= 1; }
         }
       }
-      if (!ok)  // leave no copy in flight behind
-        for (int i = it > h.ring ? it - h.ring : 0; i < it; ++i) mbar_wait(smem_u32(&full[i % h.ring]), (i / h.ring) & 1);
     }
   } else if (warp == 1) {
     // ---- products: K blocks of 64 as four instructions into the unit's accumulator.  The whole warp goes through the loop, so that the
@@ -143,6 +143,14 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0 && failed && timeout) atomicOr(timeout, kTimeoutGemm);
+  // One gave up: the copies in flight and the products issued end before the CTA does.
+  if (failed && warp == 0 && lane == 0) {
+    for (int i = max(it - h.ring, 0); i < it; ++i) settle(smem_u32(&full[i % h.ring]), (i / h.ring) & 1);
+  }
+  if (failed && warp == 1 && elect_one()) {
+    commit(smem_u32(&drained));
+    settle(smem_u32(&drained), 0);
+  }
   __syncwarp();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
