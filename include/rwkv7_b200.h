@@ -210,7 +210,7 @@ int rwkv7_b200_token_logprobs(void* stream, int rows, int V, const void* logits,
 /* The same answers for x W^T without writing the logits: one given token per row (tokens and logprobs may both be NULL),
  * x [rows][K] half, weight [V][K] in `format` (RWKV7_B200_FMT_*; W8A16: scale [V]; W4A16: scale and zero
  * [V][ceil(K / group)], group 32, 64 or 128, zero NULL: 8).  Logits are fp32 sums, not rounded to half as forward's are;
- * 4-bit weights count as half((q - zero) * scale).  K % 32 == 0; x, weight and workspace 16-byte aligned.  workspace is
+ * 4-bit weights count as half((q - zero) * scale), zeros being whole numbers.  K % 32 == 0; x, weight and workspace 16-byte aligned.  workspace is
  * scratch of the size the first function returns; calls that may overlap on the GPU need one each. */
 int rwkv7_b200_head_logprobs_workspace(int rows, int V, size_t* bytes);
 int rwkv7_b200_head_logprobs(void* stream, int rows, int K, int V, const uint16_t* x, const void* weight, int format,
@@ -388,7 +388,7 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
  * g = k / group, group 32, 64 or 128, a short last group allowed (scale and zero are [N][ceil(K / group)]), zero NULL: 8
  * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 8 rows
  * the scale multiplies the group's fp32 sum, so no weight is rounded; with more rows weights count as
- * half((q - zero) * scale).  workspace is scratch of the size the first function returns (which may be 0); without it, or
+ * half((q - zero) * scale), and zeros have to be whole numbers.  workspace is scratch of the size the first function returns (which may be 0); without it, or
  * with less, products of many rows run on fewer SMs.  Calls that may overlap on the GPU need one each. */
 int rwkv7_b200_linear_w4a16_group_workspace(int M, int K, int N, size_t* bytes);
 int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q,

@@ -371,7 +371,8 @@ def _refuse_linear_w4a16_group(x, q, scale, zero, group_size):
 
 def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NONE):
     """x W^T for 4-bit weights with group scales: W = (q - zero) * scale per group of 32, 64 or 128 inputs; x fp16 [M, K], q
-    uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N."""
+    uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N.  Up to 8
+    rows no weight is rounded; with more a weight counts as half((q - zero) * scale), and zeros have to be whole numbers."""
     ok = isinstance(x, torch.Tensor) and isinstance(q, torch.Tensor) and x.dim() == 2 and q.dim() == 2 and x.is_cuda
     if ok:
         (M, K), N, dev = x.shape, q.shape[0], x.device
