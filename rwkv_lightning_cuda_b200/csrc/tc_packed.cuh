@@ -324,6 +324,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
               const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
               g = group4(pick(sc, i), pick(ze, i));
             }
+            if (c == 1 && kb * kBK + 32 >= a.K) g.scale = __floats2half2_rn(0.f, 0.f);  // behind K: code 0, which may stand for an infinite weight
             const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {

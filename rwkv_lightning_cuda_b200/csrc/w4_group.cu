@@ -354,6 +354,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
                 zero_hi[i] = __hfma2(u2h(z2), __floats2half2_rn(-1.f, -1.f), __floats2half2_rn(-64.f, -64.f));
               }
             }
+            if ((kb << 8) + 32 * c >= a.K) {  // behind K: code 0, which may stand for an infinite weight
+#pragma unroll
+              for (int i = 0; i < 2 * kBlk; ++i) scale2[i] = __floats2half2_rn(0.f, 0.f);
+            }
 #pragma unroll
             for (int b = 0; b < kBlk; ++b) {
               uint32_t ra[4], rb[4];
@@ -574,7 +578,8 @@ int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p, bool 
 
 bool w4_rounded_fits(const W4GroupArgs& a, int sms) {
   MatvecPlan p;
-  return a.M <= kMaxRows && plan_matvec(a, sms, &p, true);
+  const long long groups = (a.K + a.group - 1) / a.group;
+  return a.M <= kMaxRows && a.N * groups < (1ll << 31) && plan_matvec(a, sms, &p, true);  // (a row's first group is kept in 32 bits)
 }
 
 int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {

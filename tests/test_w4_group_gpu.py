@@ -109,6 +109,28 @@ def test_small_and_special_activations(ops, M):
         assert torch.equal(got[keep], clean[keep]) and bool(torch.isnan(got[1]).all())
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("K", [32, 96, 288, 544])
+def test_nothing_behind_k_counts(ops, K, group):
+    """Scales at which code 0 would be an infinite half, but no code that is there: the places behind K, which read as code 0, add nothing."""
+    gen = torch.Generator().manual_seed(K + group)
+    N = 70
+    w = torch.randint(8, 12, (N, K), generator=gen, dtype=torch.uint8)
+    q = (w[:, 0::2] | (w[:, 1::2] << 4)).cuda()
+    s = torch.full((N, -(-K // group)), 16384.0).half().cuda()
+    for M in (1, 8, 20):
+        x = (torch.randn(M, K, generator=gen) * 1e-4).half().cuda()
+        check_product(ops.linear_w4a16_group(x, q, s, None, group), x, (q, s, None), group, f"{M} rows of {K}")
+        want = torch.log_softmax(x.cpu().double() @ w4_weights(q, s, None, group, rounded=True).T, dim=1)
+        tok = torch.randint(0, N, (M,), generator=gen)
+        lp, entropy, lse = ops.head_logprobs(x, q, tok.cuda(), scale=s, group_size=group)
+        # logits: as in check_product without the rounding to half; log probabilities twice that and some steps of their own
+        size = (x.cpu().double().abs() @ w4_weights(q, s, None, group, parts=True).T).max()
+        tol = 2 * float(size) * (K / 16 + 64) * 2 * U32 + 200 * U32 * (1 + float(want.abs().max()))
+        assert float((lp.cpu().double() - want[torch.arange(M), tok]).abs().max()) <= tol
+        assert bool(torch.isfinite(entropy).all()) and bool(torch.isfinite(lse).all())
+
+
 def test_codes_one_at_a_time(ops):
     """Each of the 16 codes at each place of a word, and each group's own scale: one weight at a time against one activation."""
     K, group = 288, 32
