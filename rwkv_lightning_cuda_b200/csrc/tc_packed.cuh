@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     // lanes of a quarter warp meet in a bank.  (No barrier's phase is missed by taking every fourth K block: the packed ring is a multiple of four; and
     // in the other ring of T >= 4 stages block i waits until block i - T is used, when block i - 4 has shown that i - 4 - T is, so
     // the fill of this stage before that one, i - 2 T, is too.)
-    const int r = threadIdx.x & 127, turn = (static_cast<int>(threadIdx.x) - 256) >> 7;
+    const int r = threadIdx.x & 127, turn = (warp - 8) >> 2;
     const uint32_t raw = raw_ring + r * raw_row<kFmt>(), raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
     const uint32_t operand = tmem + kOperandAt + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
     const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
