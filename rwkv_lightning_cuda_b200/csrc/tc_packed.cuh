@@ -276,6 +276,15 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     const uint32_t none = ring >> 30;  // 0, which the compiler does not know, so that the constants stay in registers
     const uint32_t mul = 0x2c003c00u + none;
     const Expand4 e4 = {0x00f0000fu + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
+    // A K block is handed over when this warp has the next one's weights in registers: the stores end under those loads.  (Nothing
+    // that a packed tile waits for comes after the K blocks four or more before it, so no wait closes a circle.)
+    int stored = -1;
+    auto hand_over = [&](int stage) {
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) arrive(smem_u32(&full[stage]));
+    };
     int rs = turn, raw_phase = 0, s = turn, phase = 0;
     for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
       const PackedUnit un = unit_of(h, u, kblocks);
@@ -304,6 +313,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
         for (int c = 0; c < (kFmt == 1 ? 4 : 2); ++c) q[c] = lds16(src + ((16 * c) ^ raw_swz));
         __syncwarp();
         if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
+        if (stored >= 0) hand_over(stored);
         ok = __all_sync(0xffffffffu, first_round || wait(empty[s], phase ^ 1));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -337,11 +347,8 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           }
           tmem_st16(operand + s * kOperandCols + 16 * c, o);
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         if (kFmt == 2 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive(smem_u32(&full[s]));
+        stored = s;
         rs += kTurns;
         if (rs >= h.raws) { rs -= h.raws; raw_phase ^= 1; }
         s += kTurns;
@@ -349,6 +356,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       }
       it += un.kblocks;
     }
+    if (stored >= 0 && ok) hand_over(stored);
   }
   if (!ok) failed = 1;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
