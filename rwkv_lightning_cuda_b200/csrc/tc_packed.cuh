@@ -165,23 +165,33 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
   bool ok = true;
   int it = 0;  // K blocks so far, of the roles that count them
-  if (warp == 0 || warp == 6) {
-    if (lane == 0) {
-      const bool packed = warp == 0;
-      const int stages = packed ? h.raws : h.ring;
-      int s = 0, phase = 0;
-      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
-        const PackedUnit un = unit_of(h, u, kblocks);
-        for (int kb = un.kb0; kb < un.kb0 + un.kblocks; ++kb, ++it) {
-          if (it >= stages && !(ok = wait(packed ? raw_empty[s] : empty[s], phase ^ 1))) break;
-          const uint32_t bar = smem_u32(packed ? &raw_full[s] : &full[s]);
-          mbar_expect_tx(bar, packed ? kRawBytes : x_bytes);
-          if (packed) tma_2d(raw_ring + s * kRawBytes, &maps.w, bar, kb * raw_row<kFmt>(), un.n0);
-          else tma_2d(ring + s * x_bytes, &maps.x, bar, kb * kBK, un.r0);
-          if (++s == stages) { s = 0; phase ^= 1; }
+  // Copies: as below the whole warp goes through the loop, one lane issues, and the next stage is asked for ahead.  (One lane alone took
+  // 480 to 560 clocks a K block, more than anything else.)
+  auto fetch = [&](uint64_t* filled, uint64_t* used, int stages, uint32_t bytes, auto&& copy) {
+    const bool issuer = elect_one();
+    int s = 0, phase = 1;
+    bool free = true;  // the first round's stages are
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+      const PackedUnit un = unit_of(h, u, kblocks);
+      for (int kb = un.kb0; kb < un.kb0 + un.kblocks; ++kb) {
+        if (!__all_sync(0xffffffffu, free) && !(ok = __all_sync(0xffffffffu, wait(used[s], phase)))) break;
+        if (issuer) {
+          const uint32_t bar = smem_u32(&filled[s]);
+          mbar_expect_tx(bar, bytes);
+          copy(s, bar, kb, un);
         }
+        ++it;
+        if (++s == stages) { s = 0; phase ^= 1; }
+        free = it < stages || mbar_test(smem_u32(&used[s]), phase);
+        __syncwarp();
       }
     }
+  };
+  if (warp == 0) {
+    fetch(raw_full, raw_empty, h.raws, kRawBytes,
+          [&](int s, uint32_t bar, int kb, const PackedUnit& un) { tma_2d(raw_ring + s * kRawBytes, &maps.w, bar, kb * raw_row<kFmt>(), un.n0); });
+  } else if (warp == 6) {
+    fetch(full, empty, h.ring, x_bytes, [&](int s, uint32_t bar, int kb, const PackedUnit& un) { tma_2d(ring + s * x_bytes, &maps.x, bar, kb * kBK, un.r0); });
   } else if (warp == 1) {
     // ---- products: K blocks of 64 as four instructions into the unit's accumulator.  The whole warp goes through the loop, so that the
     // operands are computed in uniform registers, and one lane issues (700 clocks a K block when one lane did all of it, between

@@ -73,18 +73,24 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   bool ok = true;
   int it = 0;  // K blocks so far, of the roles that count them
   if (warp == 0) {
-    if (lane == 0) {
-      int s = 0, phase = 0;
-      for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
-        const int r0 = u % h.row_blocks * kRows, n0 = u / h.row_blocks * h.toks;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          if (it >= h.ring && !(ok = wait(empty[s], phase ^ 1))) break;
+    // ---- copies: as below the whole warp goes through the loop, one lane issues, and the next stage is asked for ahead
+    const bool issuer = elect_one();
+    int s = 0, phase = 1;
+    bool free = true;  // the first round's stages are
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+      const int r0 = u % h.row_blocks * kRows, n0 = u / h.row_blocks * h.toks;
+      for (int kb = 0; kb < kblocks; ++kb) {
+        if (!__all_sync(0xffffffffu, free) && !(ok = __all_sync(0xffffffffu, wait(empty[s], phase)))) break;
+        if (issuer) {
           const uint32_t bar = smem_u32(&full[s]), dst = ring + s * h.tile_bytes;
           mbar_expect_tx(bar, 128 * (h.x_rows + h.toks));
           tma_2d(dst, &maps.x, bar, kb * kBK, r0);
           tma_2d(dst + h.x_bytes, &maps.w, bar, kb * kBK, n0);
-          if (++s == h.ring) { s = 0; phase ^= 1; }
         }
+        ++it;
+        if (++s == h.ring) { s = 0; phase ^= 1; }
+        free = it < h.ring || mbar_test(smem_u32(&empty[s]), phase);
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
