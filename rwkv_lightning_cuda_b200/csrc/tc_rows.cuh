@@ -106,18 +106,18 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t acc = tmem + (n & 1) * kToks;
       for (int kb = 0; kb < kblocks; ++kb) {
-        if (!__all_sync(0xffffffffu, ready) && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+        if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t dx = tile_desc(ring + s * h.tile_bytes), dw = tile_desc(ring + s * h.tile_bytes + h.x_bytes);
         const uint32_t done = smem_u32(&empty[s]);
         if (++s == h.ring) { s = 0; phase ^= 1; }
-        ready = mbar_test(smem_u32(&full[s]), phase);
+        const bool next = mbar_test(smem_u32(&full[s]), phase);
         if (issuer) {
 #pragma unroll
           for (int k4 = 0; k4 < kBK / 16; ++k4) mma(acc, dx + 2 * k4, dw + 2 * k4, idesc, (kb | k4) != 0);
           commit(done);
         }
-        __syncwarp();
+        ready = __all_sync(0xffffffffu, next);
       }
       if (ok && issuer) commit(smem_u32(&acc_full[n & 1]));
       __syncwarp();
