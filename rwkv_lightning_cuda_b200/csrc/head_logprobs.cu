@@ -61,8 +61,8 @@ struct StatsEpilogue {
 // The same where a thread has one token and all rows: 32 tokens x 32 rows at a time go through shared memory, after which a lane has
 // one row's 32 tokens; the four warps' parts of a row are merged at the end of the unit.
 struct PackedStatsEpilogue {
-  static constexpr int kPitch = 36, kWarpFloats = 32 * kPitch, kParts = 4 * tc::kMaxBlockRows;
-  static constexpr int kScratch = 4 * kWarpFloats * 4 + kParts * 16;
+  static constexpr int kPitch = 36, kWarpFloats = 32 * kPitch;
+  static int scratch(int block_rows) { return 4 * kWarpFloats * 4 + 4 * block_rows * 16; }
   float4* part;   // [tiles][rows]
   float* given;   // [rows]
   const int64_t* tokens;
@@ -109,7 +109,7 @@ struct PackedStatsEpilogue {
       for (int i = 0; i < 4; ++i) st[i].m = m;
 #pragma unroll
       for (int i = 0; i < 32; ++i) add(st[i & 3], v[i]);
-      parts[quad * tc::kMaxBlockRows + c + lane] =
+      parts[quad * rows + c + lane] =
           make_float4(m, (st[0].s + st[1].s) + (st[2].s + st[3].s), (st[0].t + st[1].t) + (st[2].t + st[3].t), 0.f);
     }
     __syncwarp();
@@ -121,7 +121,7 @@ struct PackedStatsEpilogue {
       SoftStats all;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float4 p = parts[w * tc::kMaxBlockRows + r];
+        const float4 p = parts[w * rows + r];
         SoftStats b;
         b.m = p.x; b.s = p.y; b.t = p.z;
         all = merge(all, b);
@@ -198,7 +198,8 @@ int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
   tc::set_row_blocks(&h, a.rows);
   h.tiles = (a.V + tc::kTileToks - 1) / tc::kTileToks;
   h.splits = 1;
-  h.kb_per_split = (a.K + tc::kBK - 1) / tc::kBK;
+  const int stage = tc::kBK * tc::subs(h.block_rows);
+  h.kb_per_split = (a.K + stage - 1) / stage;
   const long long units = static_cast<long long>(h.tiles) * h.row_blocks;
   RK_REQUIRE(units < 0x7fffffff, kShape, "head_logprobs: too many rows");
   h.units = static_cast<int>(units);

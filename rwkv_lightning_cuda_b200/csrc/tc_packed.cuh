@@ -9,12 +9,12 @@
 // memory is a token, a column a row of x.  Up to 128 rows in a block there are two accumulators, and a unit's epilogue runs
 // under the next one's products; with more there is one.
 //
-// Bound up to 128 rows by the expansion, some 350 issue slots of each scheduler and 420 clocks for a K block of 4-bit weights, of which the
-// ANDs, permutations and half2 operations that a weight needs are 200; above by the tensor cores (24 rows of 65536 x 4096 in
-// 70 us, 256 rows of 16384 x 4096 in 32 us, 1.06 PFLOP/s).
+// Bound up to 128 rows by what the roles do per stage and weight: of 128 of K, some 800 clocks, in which the expansion of 4-bit weights
+// has 300 to 350 issue slots of each scheduler; above by the tensor cores.  (24 rows of 65536 x 4096 in 59 us, with stages of 64
+// in 65; 128 rows of 16384 x 4096 in 22; 256 in 32 us, 1.09 PFLOP/s.)
 //
 // Warp roles: 0 loads packed tiles, 1 issues tcgen05.mma, 2..5 run the epilogue, 6 loads rows of x, 8..23 expand, four warps to a
-// K block in turn.  Every wait is bounded: one that runs out sets the device's failure word, every role leaves its loop, and the
+// stage in turn.  Every wait is bounded: one that runs out sets the device's failure word, every role leaves its loop, and the
 // CTA frees its tensor memory and returns.
 #pragma once
 
@@ -25,13 +25,15 @@ namespace tc {
 
 constexpr int kTileToks = 128;    // tokens per unit = MMA M
 constexpr int kMaxBlockRows = 256;
-constexpr int kTurns = 4;         // groups of four warps that expand K blocks in turn
+constexpr int kTurns = 4;         // groups of four warps that expand stages in turn
 constexpr int kMaxRing = 8;
 constexpr int kPackedThreads = 256 + kTurns * 128;
-constexpr int kOperandCols = kBK / 2;  // of tensor memory that a K block of weights takes
-constexpr int kOperandAt = 256;        // behind the accumulators
+constexpr int kOperandAt = 256;    // columns of tensor memory behind the accumulators: 256 for stages of expanded weights
 
-template <int kFmt> __host__ __device__ constexpr int raw_row() { return kFmt == 1 ? kBK : kBK / 2; }  // bytes of a packed row of a K block
+// kSub: K blocks of 64 to a stage.  Two with up to 128 rows, where what every role does once per stage bounds; with more rows there is
+// no room for four such stages.
+__host__ __device__ constexpr int subs(int block_rows) { return block_rows <= 128 ? 2 : 1; }
+template <int kFmt, int kSub> __host__ __device__ constexpr int raw_row() { return kSub * (kFmt == 1 ? kBK : kBK / 2); }  // bytes of a packed row of a stage
 
 // int8 with a scale per token (applied to the sums), or 4 bits with scales and zeros per group (half((q - zero) * scale)).
 struct Packed {
@@ -42,7 +44,7 @@ struct Packed {
 struct PackedShape {
   int tiles;                 // of 128 tokens
   int rows, row_blocks, block_rows;  // rows of x; block_rows: a multiple of 16, at most kMaxBlockRows
-  int splits, kb_per_split;  // ranges of K and their K blocks (the last one may have fewer)
+  int splits, kb_per_split;  // ranges of K and their stages of 64 subs(block_rows) (the last one may have fewer)
   int units;
   int ring, raws;            // stages of x and weights, and of packed tiles (set by launch_packed)
 };
@@ -118,18 +120,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 
 // Epi: a copy per epilogue thread and unit, all 128 of which are asked; begin(token, r0, rows, split, scratch) while the products are under
 // way, then chunk(c, z, here) for every 32 rows r0 + c .. (here of them valid), where z[i] is the result of row r0 + c + i, then end();
-// scratch: Epi::kScratch bytes of shared memory.  The threads may meet at barrier 1.
-template <int kFmt, class Epi>
+// scratch: Epi::scratch(block_rows) bytes of shared memory.  The threads may meet at barrier 1.
+template <int kFmt, int kSub, class Epi>
 __global__ void __launch_bounds__(kPackedThreads, 1)
     tc_packed_kernel(const __grid_constant__ PackedMaps maps, const Packed a, const PackedShape h, const Epi epilogue, int* timeout) {
   extern __shared__ unsigned char smem[];
   __shared__ __align__(8) uint64_t full[kMaxRing], empty[kMaxRing], raw_full[kMaxRing], raw_empty[kMaxRing], acc_full[2], acc_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
-  constexpr uint32_t kRawBytes = kTileToks * raw_row<kFmt>();
+  constexpr int kStage = kSub * kBK;  // weights of a token per stage
+  constexpr uint32_t kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const uint32_t x_bytes = h.block_rows * 128, ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring * x_bytes;
-  const int kblocks = (a.K + kBK - 1) / kBK;
+  const uint32_t x_sub = h.block_rows * 128, x_bytes = kSub * x_sub, ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring * x_bytes;
+  const int kblocks = (a.K + kStage - 1) / kStage;
   const int accs = h.block_rows <= 128 ? 2 : 1;
 
   if (threadIdx.x == 0) {
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
 
   auto wait = [&](uint64_t& bar, int parity) { return mbar_try_wait(smem_u32(&bar), parity) || wait_on(smem_u32(&bar), parity, &failed); };
   bool ok = true;
-  int it = 0;  // K blocks so far, of the roles that count them
+  int it = 0;  // stages so far, of the roles that count them
   // Copies: as below the whole warp goes through the loop, one lane issues, and the next stage is asked for ahead.  (One lane alone took
   // 480 to 560 clocks a K block, more than anything else.)
   auto fetch = [&](uint64_t* filled, uint64_t* used, int stages, uint32_t bytes, auto&& copy) {
@@ -189,11 +192,14 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   };
   if (warp == 0) {
     fetch(raw_full, raw_empty, h.raws, kRawBytes,
-          [&](int s, uint32_t bar, int kb, const PackedUnit& un) { tma_2d(raw_ring + s * kRawBytes, &maps.w, bar, kb * raw_row<kFmt>(), un.n0); });
+          [&](int s, uint32_t bar, int kb, const PackedUnit& un) { tma_2d(raw_ring + s * kRawBytes, &maps.w, bar, kb * kRawRow, un.n0); });
   } else if (warp == 6) {
-    fetch(full, empty, h.ring, x_bytes, [&](int s, uint32_t bar, int kb, const PackedUnit& un) { tma_2d(ring + s * x_bytes, &maps.x, bar, kb * kBK, un.r0); });
+    fetch(full, empty, h.ring, x_bytes, [&](int s, uint32_t bar, int kb, const PackedUnit& un) {
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) tma_2d(ring + s * x_bytes + i * x_sub, &maps.x, bar, kb * kStage + i * kBK, un.r0);
+    });
   } else if (warp == 1) {
-    // ---- products: K blocks of 64 as four instructions into the unit's accumulator.  The whole warp goes through the loop, so that the
+    // ---- products: four instructions for each 64 of K into the unit's accumulator.  The whole warp goes through the loop, so that the
     // operands are computed in uniform registers, and one lane issues (700 clocks a K block when one lane did all of it, between
     // the instructions of 16 other warps); the next stage's barrier is asked, without waiting, before this one's products are issued.
     const uint32_t idesc = instruction_desc(h.block_rows);
@@ -209,12 +215,13 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
         if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t dx = tile_desc(ring + s * x_bytes);
-        const uint32_t dw = tmem + kOperandAt + s * kOperandCols, done = smem_u32(&empty[s]);
+        const uint32_t dw = tmem + kOperandAt + s * (kStage / 2), done = smem_u32(&empty[s]);
         if (++s == h.ring) { s = 0; phase ^= 1; }
         const bool next = mbar_test(smem_u32(&full[s]), phase);
         if (issuer) {
 #pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4) mma_from_tmem(tmem + acc * 128, dw + 8 * k4, dx + 2 * k4, idesc, (kb | k4) != 0);
+          for (int k = 0; k < kStage / 16; ++k)
+            mma_from_tmem(tmem + acc * 128, dw + 8 * k, dx + (k / 4) * (x_sub >> 4) + 2 * (k % 4), idesc, (kb | k) != 0);
           commit(done);
         }
         ready = __all_sync(0xffffffffu, next);
@@ -258,13 +265,13 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       epi.end();
     }
   } else if (warp >= 8) {
-    // ---- expansion: a thread owns a token of the tile, 64 weights a K block; four warps take every fourth K block.  A packed row of 64
-    // (32) bytes has its 16-byte chunk c at c ^ (r / 2 & 3) (c ^ (r / 4 & 1)), the swizzles of 64- and 32-byte rows, so that no two
-    // lanes of a quarter warp meet in a bank.  (No barrier's phase is missed by taking every fourth K block: the packed ring is a multiple of four; and
-    // in the other ring of T >= 4 stages block i waits until block i - T is used, when block i - 4 has shown that i - 4 - T is, so
-    // the fill of this stage before that one, i - 2 T, is too.)
+    // ---- expansion: a thread owns a token of the tile, all its weights of a stage; four warps take every fourth stage.  A packed row of
+    // 128 (64, 32) bytes has its 16-byte chunk c at c ^ (r & 7) (c ^ (r / 2 & 3), c ^ (r / 4 & 1)), the swizzles of such rows, so that
+    // no two lanes of a quarter warp meet in a bank.  (No barrier's phase is missed by taking every fourth stage: the packed ring is a
+    // multiple of four; and in the other ring of T >= 4 places block i waits until block i - T is used, when block i - 4 has shown that
+    // i - 4 - T is, so the fill of this place before that one, i - 2 T, is too.)
     const int r = threadIdx.x & 127, turn = (warp - 8) >> 2;
-    const uint32_t raw = raw_ring + r * raw_row<kFmt>(), raw_swz = kFmt == 1 ? ((r >> 1) & 3) << 4 : ((r >> 2) & 1) << 4;
+    const uint32_t raw = raw_ring + r * kRawRow, raw_swz = (kRawRow == 32 ? (r >> 2) & 1 : kRawRow == 64 ? (r >> 1) & 3 : r & 7) << 4;
     const uint32_t operand = tmem + kOperandAt + (static_cast<uint32_t>(warp & 3) << 21);  // this warp's 32 lanes
     const int shift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7, groups = (a.K + a.group - 1) >> shift;
     // Scales and zeros: eight groups at a time as one 16-byte load each, the next eight under way; where a row of them is no
@@ -278,16 +285,23 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       sc_next = reinterpret_cast<const uint4*>(sp)[block];
       if (zp) ze_next = reinterpret_cast<const uint4*>(zp)[block];
     };
-    auto load_runs = [&](int kb) {  // a K block's two runs of 32 weights into the first two halves
-      const int g0 = min((kb * kBK) >> shift, groups - 1), g1 = min((kb * kBK + 32) >> shift, groups - 1);
-      sc_next.x = sp[g0] | (static_cast<uint32_t>(sp[g1]) << 16);
-      if (zp) ze_next.x = zp[g0] | (static_cast<uint32_t>(zp[g1]) << 16);
+    auto load_runs = [&](int kb) {  // a stage's runs of 32 weights into the first halves
+      auto run = [&](const uint16_t* of, int i) {
+        return of[min((kb * kStage + 64 * i) >> shift, groups - 1)] | (static_cast<uint32_t>(of[min((kb * kStage + 64 * i + 32) >> shift, groups - 1)]) << 16);
+      };
+      sc_next.x = run(sp, 0);
+      if (kSub == 2) sc_next.y = run(sp, 1);
+      if (zp) {
+        ze_next.x = run(zp, 0);
+        if (kSub == 2) ze_next.y = run(zp, 1);
+      }
     };
+    auto eight_of = [&](int kb) { return (kb * kStage) >> (shift + 3); };
     const uint32_t none = ring >> 30;  // 0, which the compiler does not know, so that the constants stay in registers
     const uint32_t mul = 0x2c003c00u + none;
     const Expand4 e4 = {0x00f0000fu + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
-    // A K block is handed over when this warp has the next one's weights in registers: the stores end under those loads.  (Nothing
-    // that a packed tile waits for comes after the K blocks four or more before it, so no wait closes a circle.)
+    // A stage is handed over when this warp has the next one's weights in registers: the stores end under those loads.  (A packed tile
+    // waits for nothing later than the stage four before it, and a place for the one T before, so no wait closes a circle.)
     int stored = -1;
     auto hand_over = [&](int stage) {
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -300,63 +314,73 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       const PackedUnit un = unit_of(h, u, kblocks);
       const int row = min(un.n0 + r, a.V - 1), kb_end = un.kb0 + un.kblocks;
       int kb = un.kb0 + ((turn - it) & (kTurns - 1));
-      int block = -1;
+      int block = -1, ahead = -1;
       if (kFmt == 2 && kb < kb_end) {
         sp = reinterpret_cast<const uint16_t*>(a.scale) + static_cast<size_t>(row) * groups;
         if (a.zero) zp = reinterpret_cast<const uint16_t*>(a.zero) + static_cast<size_t>(row) * groups;
-        if (eights) load8((kb * kBK) >> (shift + 3));
+        if (eights) load8(ahead = eight_of(kb));
         else load_runs(kb);
       }
       for (; kb < kb_end; kb += kTurns) {
         const bool first_round = it + kb - un.kb0 < h.ring;
-        if (kFmt == 2 && (!eights || (kb * kBK) >> (shift + 3) != block)) {
+        if (kFmt == 2 && (!eights || ahead != block)) {
           sc = sc_next;
           ze = ze_next;
-          block = (kb * kBK) >> (shift + 3);
-          if (eights) load8(block + 1);
+          block = ahead;
         }
+        if (kFmt == 2 && eights && eight_of(kb + kTurns) != block) load8(ahead = eight_of(kb + kTurns));
         ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase));
         if (!ok) break;
         const uint32_t src = raw + rs * kRawBytes;
-        uint4 q[kFmt == 1 ? 4 : 2];
-#pragma unroll
-        for (int c = 0; c < (kFmt == 1 ? 4 : 2); ++c) q[c] = lds16(src + ((16 * c) ^ raw_swz));
-        __syncwarp();
-        if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
-        if (stored >= 0) hand_over(stored);
-        ok = __all_sync(0xffffffffu, first_round || wait(empty[s], phase ^ 1));
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         Group4 g;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 32 weights at a time: the whole K block's would take too many registers
-          uint32_t o[16];
-          if (kFmt == 1) {
-            const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
+        for (int sub = 0; sub < kSub; ++sub) {
+          constexpr int kLoads = kFmt == 1 ? 4 : 2;
+          uint4 q[kLoads];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint2 p = expand8(w[i]);
-              o[2 * i] = p.x;
-              o[2 * i + 1] = p.y;
-            }
-          } else {
-            if (c == 0 || shift == 5) {
-              const int i = eights ? ((kb * kBK + 32 * c) >> shift) & 7 : c;
-              g = group4(pick(sc, i), pick(ze, i));
-            }
-            if (c == 1 && kb * kBK + 32 >= a.K) g.scale = __floats2half2_rn(0.f, 0.f);  // behind K: code 0, which may stand for an infinite weight
-            const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint4 p = expand4(w[j], g, e4);
-              o[4 * j] = p.x;
-              o[4 * j + 1] = p.y;
-              o[4 * j + 2] = p.z;
-              o[4 * j + 3] = p.w;
-            }
+          for (int c = 0; c < kLoads; ++c) q[c] = lds16(src + ((16 * (kLoads * sub + c)) ^ raw_swz));
+          if (sub == kSub - 1) {
+            __syncwarp();
+            if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
           }
-          tmem_st16(operand + s * kOperandCols + 16 * c, o);
+          if (sub == 0) {
+            if (stored >= 0) hand_over(stored);
+            ok = __all_sync(0xffffffffu, first_round || wait(empty[s], phase ^ 1));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {  // 32 weights at a time: more would take too many registers
+            uint32_t o[16];
+            if (kFmt == 1) {
+              const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint2 p = expand8(w[i]);
+                o[2 * i] = p.x;
+                o[2 * i + 1] = p.y;
+              }
+            } else {
+              const int run = 2 * sub + c, k = kb * kStage + 32 * run;
+              if (run == 0 || shift == 5 || (shift == 6 && c == 0)) {
+                const int i = eights ? (k >> shift) & 7 : run;
+                g = group4(pick(sc, i), pick(ze, i));
+              }
+              if (run > 0 && k >= a.K) g.scale = __floats2half2_rn(0.f, 0.f);  // behind K: code 0, which may stand for an infinite weight
+              const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint4 p = expand4(w[j], g, e4);
+                o[4 * j] = p.x;
+                o[4 * j + 1] = p.y;
+                o[4 * j + 2] = p.z;
+                o[4 * j + 3] = p.w;
+              }
+            }
+            tmem_st16(operand + s * (kStage / 2) + 32 * sub + 16 * c, o);
+          }
         }
+        if (!ok) break;
         if (kFmt == 2 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
         stored = s;
         rs += kTurns;
@@ -391,27 +415,31 @@ inline void set_row_blocks(PackedShape* h, int rows) {
   h->block_rows = ((rows + h->row_blocks - 1) / h->row_blocks + 15) & ~15;
 }
 
-template <int kFmt, class Epi>
-int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, PackedShape h, const Epi& epi, int sms) {
+template <int kFmt, int kSub, class Epi>
+int launch_stages(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, PackedShape h, const Epi& epi, int sms) {
+  constexpr int kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow, kMost = kMaxRing / kSub;
   PackedMaps maps;
   int s = encode_map(what, &maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, h.rows, a.K, kBK, h.block_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s == kOk)
-    s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.V, kFmt == 1 ? a.K : a.K / 2, raw_row<kFmt>(), kTileToks,
-                   kFmt == 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+    s = encode_map(what, &maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w, a.V, kFmt == 1 ? a.K : a.K / 2, kRawRow, kTileToks,
+                   kRawRow == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : kRawRow == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != kOk) return s;
-  constexpr int kRawBytes = kTileToks * raw_row<kFmt>();
-  const int budget = static_cast<int>(kSmemBytes) - 1024 - Epi::kScratch;
+  const int x_bytes = kSub * h.block_rows * 128, scratch = Epi::scratch(h.block_rows), budget = static_cast<int>(kSmemBytes) - 1024 - scratch;
   for (h.raws = kMaxRing;; h.raws = kTurns) {  // the rows of x go first: four stages of them at least
-    h.ring = std::min(kMaxRing, (budget - h.raws * kRawBytes) / (h.block_rows * 128));
+    h.ring = std::min(kMost, (budget - h.raws * kRawBytes) / x_bytes);
     if (h.ring >= kTurns || h.raws == kTurns) break;
   }
-  const size_t smem = 1024 + Epi::kScratch + static_cast<size_t>(h.ring) * h.block_rows * 128 + static_cast<size_t>(h.raws) * kRawBytes;
+  const size_t smem = 1024 + scratch + static_cast<size_t>(h.ring) * x_bytes + static_cast<size_t>(h.raws) * kRawBytes;
   RK_REQUIRE(h.ring >= kTurns, kShape, "%s: no room for four stages", what);
-  const auto kernel = tc_packed_kernel<kFmt, Epi>;
+  const auto kernel = tc_packed_kernel<kFmt, kSub, Epi>;
   RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
   RK_CUDA(launch_pdl(kernel, dim3(std::min(h.units, sms)), dim3(kPackedThreads), smem, stream, maps, a, h, epi, timeout_word_or_null()));
   RK_LAUNCH_CHECK(what);
   return kOk;
+}
+template <int kFmt, class Epi>
+int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, const PackedShape& h, const Epi& epi, int sms) {
+  return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1>(stream, what, x, w, a, h, epi, sms);
 }
 
 }  // namespace tc

@@ -595,7 +595,7 @@ __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("
 
 // A token's (channel's) results for the unit's rows to y, or to the unit's plane of partial sums; a warp's 32 channels are neighbours.
 struct ProductEpilogue {
-  static constexpr int kScratch = 4 * 2048;
+  static int scratch(int) { return 4 * 2048; }
   void* y;
   float* partial;  // [splits][rows][N], or nullptr
   int n_rows, N, epi;
@@ -682,26 +682,27 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
     *reinterpret_cast<uint2*>(static_cast<half*>(p.y) + i) = make_uint2(h2u(__floats2half2_rn(e[0], e[1])), h2u(__floats2half2_rn(e[2], e[3])));
 }
 
-// K ranges with the least time by this account, in clocks of an SM: a K block takes the expansion 420, or the tensor cores 2.35 a
-// row; a unit's results take 25 a row, hidden under the next unit's products where there are two accumulators; the second
-// kernel 3000, 200 a range and its traffic.  (64 rows of 1024 x 1024: 7.5 us whole, 6.5 in eight ranges, 7.9 in sixteen; 96 rows
-// of 10240 x 2560: 15.7 whole, 19.0 in two, 16.2 in three; 96 rows of 2560 x 10240: 43.7 whole, 15.7 in seven, 19.6 in nine, which
-// is a second wave.)
+// K ranges with the least time by this account, in clocks of an SM: 64 of K take what is done per weight and stage 380, or the tensor
+// cores 2.35 a row; a unit's results take 25 a row, hidden under the next unit's products where there are two accumulators; the
+// second kernel 3000, 200 a range and its traffic.  (64 rows of 1024 x 1024: 7.5 us whole, 6.5 in eight ranges, 7.9 in sixteen; 96
+// rows of 10240 x 2560: 15.7 whole, 19.0 in two, 16.2 in three; 96 rows of 2560 x 10240: 43.7 whole, 15.7 in seven, 19.6 in nine,
+// which is a second wave: with stages of 64, those of 128 take a tenth less of all of them.)
 tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
   tc::PackedShape best = {};
   double least = 0;
-  const int kblocks = (K + tc::kBK - 1) / tc::kBK;
+  tc::PackedShape rows = {};
+  tc::set_row_blocks(&rows, M);
+  const int stage = tc::kBK * tc::subs(rows.block_rows), kblocks = (K + stage - 1) / stage;
   const size_t plane = static_cast<size_t>(M) * N;
   for (int want = 1; want <= 16 && want <= kblocks; ++want) {
-    tc::PackedShape h = {};
-    tc::set_row_blocks(&h, M);
+    tc::PackedShape h = rows;
     h.tiles = (N + tc::kTileToks - 1) / tc::kTileToks;
     h.kb_per_split = (kblocks + want - 1) / want;
     h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
     const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;
-    double cost = waves * (h.kb_per_split * std::max(420.0, 2.35 * h.block_rows)) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
+    double cost = waves * (h.kb_per_split * std::max(stage * 6.0, stage * h.block_rows / 27.0)) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
     if (h.splits > 1) cost += 3000 + 200 * h.splits + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
     if (best.units == 0 || cost < least) { least = cost; best = h; }
