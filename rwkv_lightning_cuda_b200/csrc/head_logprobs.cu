@@ -214,12 +214,12 @@ int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
 
 }  // namespace
 
-// Few rows: the weight-streaming kernels read the weights once at a better rate than the kernels above with their 128-row or
-// 128-token tiles, and the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said otherwise), this
-// route against the other: 4-bit 50 us against 74 at eight rows (33 against 43 at K = 2048, 23 against 27 at K = 1024); int8 58
-// against 70 at four rows; fp16 83 against 91 at one row, but 111 against 94 at four.  In small matrices of 8- and 16-bit weights
-// the second pass costs more than it saves (int8 65536 x 1024 at two rows: 31 us against 24; 65536 x 2560: 42 against 47).
-constexpr int kFewRowsF16 = 1, kFewRowsW8 = 4, kFewRowsW4 = 8;
+// Few rows: where the weight-streaming kernels read the weights at a better rate than the kernels above with their 128-row or
+// 128-token tiles, the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said otherwise), this route
+// against the other: 4-bit 51 us against 56 at eight rows (30 against 35 at two and K = 2048, 24 against 23 at eight and K = 1024);
+// fp16 83 against 91 at one row, but 111 against 94 at four, and below 128 MB of weights the second pass takes what is saved.  int8
+// has no such route: 58 against 51 at four rows, 42 against 35 at two and K = 2560.
+constexpr int kFewRowsF16 = 1, kFewRowsW4 = 8;
 constexpr double kFewRowsBytes = 128e6;
 
 size_t head_logprobs_workspace(int rows, int V) {
@@ -237,8 +237,7 @@ bool few_rows(const HeadLogprobsArgs& a, int sms) {
     w.M = a.rows; w.K = a.K; w.N = a.V; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
     return a.rows <= kFewRowsW4 && w4_rounded_fits(w, sms);
   }
-  const double bytes = static_cast<double>(a.V) * a.K * (a.fmt == 0 ? 2 : 1);
-  return a.rows <= (a.fmt == 0 ? kFewRowsF16 : kFewRowsW8) && a.K <= 16384 && bytes >= kFewRowsBytes;
+  return a.fmt == 0 && a.rows <= kFewRowsF16 && a.K <= 16384 && 2.0 * a.V * a.K >= kFewRowsBytes;
 }
 // Logits into the workspace, then their statistics.
 int logits_then_stats(cudaStream_t stream, const HeadLogprobsArgs& a, float* logits, int sms) {
@@ -250,7 +249,7 @@ int logits_then_stats(cudaStream_t stream, const HeadLogprobsArgs& a, float* log
     s = w4_rounded_linear(stream, w, sms);
   } else {
     LinearArgs l;
-    l.M = a.rows; l.K = a.K; l.N = a.V; l.x = a.x; l.w = a.w; l.fmt = a.fmt; l.scale = a.scale; l.epi = kEpiRawF32; l.y = logits;
+    l.M = a.rows; l.K = a.K; l.N = a.V; l.x = a.x; l.w = a.w; l.fmt = a.fmt; l.epi = kEpiRawF32; l.y = logits;
     s = linear(stream, l);
   }
   if (s != kOk) return s;
