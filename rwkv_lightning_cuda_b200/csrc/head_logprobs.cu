@@ -62,6 +62,7 @@ struct StatsEpilogue {
 // one row's 32 tokens; the four warps' parts of a row are merged at the end of the unit.
 struct PackedStatsEpilogue {
   static constexpr int kPitch = 36, kWarpFloats = 32 * kPitch;
+  static constexpr bool kExact = true;
   static int scratch(int block_rows) { return 4 * kWarpFloats * 4 + 4 * block_rows * 16; }
   float4* part;   // [tiles][rows]
   float* given;   // [rows]
@@ -160,14 +161,16 @@ __global__ void __launch_bounds__(kMergeThreads) head_merge_kernel(HeadLogprobsA
 
 // The token tile that lets the units come out in the fewest full rounds over the SMs (65536 tokens in tiles of 256 are 1.7 rounds
 // of 148, in tiles of 224 two full ones); a unit is counted as its tokens and 32 more for its beginning and end.
-tc::Shape head_shape(int rows, int V, int sms) {
+tc::Shape head_shape(int rows, int V, int K, int sms) {
   tc::Shape best = {};
   long long least = -1;
-  for (int toks = tc::kToks; toks >= kMinToks; toks -= 16) {
+  const bool whole = K <= tc::kWholeK;
+  for (int toks = whole ? tc::kToks : tc::kRangeToks; toks >= kMinToks; toks -= 16) {
     tc::Shape h;
     h.toks = toks;
     h.tiles = (V + toks - 1) / toks;
     h.row_blocks = (rows + tc::kRows - 1) / tc::kRows;
+    h.seg = (whole ? tc::kWholeK : tc::kRangeK) / tc::kBK;
     h.x_rows = std::min(tc::kRows, (rows + 7) & ~7);
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks, cost = (units + sms - 1) / sms * (toks + 32);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
@@ -183,7 +186,7 @@ int merge_tiles(cudaStream_t stream, const HeadLogprobsArgs& a, int tiles) {
 }
 
 int head_f16(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
-  const tc::Shape h = head_shape(a.rows, a.V, sms);
+  const tc::Shape h = head_shape(a.rows, a.V, a.K, sms);
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "head_logprobs: too many rows");
   a.given = reinterpret_cast<float*>(a.part + static_cast<size_t>(h.tiles) * a.rows);
   StatsEpilogue epi;
@@ -195,11 +198,13 @@ int head_f16(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
 template <int kFmt>
 int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
   tc::PackedShape h = {};
-  tc::set_row_blocks(&h, a.rows);
+  const bool whole = a.K <= tc::kWholeK;
+  tc::set_row_blocks(&h, a.rows, whole ? tc::kMaxBlockRows : 128);
   h.tiles = (a.V + tc::kTileToks - 1) / tc::kTileToks;
   h.splits = 1;
   const int stage = tc::kBK * tc::subs(h.block_rows);
   h.kb_per_split = (a.K + stage - 1) / stage;
+  h.seg = whole ? h.kb_per_split : tc::kRangeK / stage;
   const long long units = static_cast<long long>(h.tiles) * h.row_blocks;
   RK_REQUIRE(units < 0x7fffffff, kShape, "head_logprobs: too many rows");
   h.units = static_cast<int>(units);

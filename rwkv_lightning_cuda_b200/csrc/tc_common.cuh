@@ -45,6 +45,22 @@ static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, const
     if (mbar_try_wait(bar, parity)) return true;
   return false;
 }
+// 32 columns of this warp's lanes, there when the call returns.
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+        "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]), "f"(v[21]),
+        "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// The tensor cores cut off what they add to a running sum, so its error grows faster than the sum: logits of 4096 products came out
+// 2.8e-6 of their size off and longer ones more, against 7e-7 at any K when ranges of 1024 are added up by themselves, each rounded
+// to nearest into a sum beside the accumulators.  So the head does above kWholeK; at 65536 x 4096 that costs nothing at 128 fp16 rows,
+// 4 % at 16 quantised ones, 8 % at 2048 fp16 ones (narrower tiles) and 16 % at 2048 quantised ones (128 rows to a block, not 256).
+constexpr int kWholeK = 2048, kRangeK = 1024;
 // The wait of a kernel that has given up for its own copies and products in flight: a fraction of a second at most.
 static __device__ __noinline__ void settle(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 16); ++i)

@@ -46,6 +46,7 @@ struct PackedShape {
   int rows, row_blocks, block_rows;  // rows of x; block_rows: a multiple of 16, at most kMaxBlockRows
   int splits, kb_per_split;  // ranges of K and their stages of 64 subs(block_rows) (the last one may have fewer)
   int units;
+  int seg;                   // stages that are added up in one accumulator: all of a unit's, or kRangeK's where K is long (block_rows at most 128 then)
   int ring, raws;            // stages of x and weights, and of packed tiles (set by launch_packed)
 };
 struct PackedMaps {
@@ -120,8 +121,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
 
 // Epi: a copy per epilogue thread and unit, all 128 of which are asked; begin(token, r0, rows, split, scratch) while the products are under
 // way, then chunk(c, z, here) for every 32 rows r0 + c .. (here of them valid), where z[i] is the result of row r0 + c + i, then end();
-// scratch: Epi::scratch(block_rows) bytes of shared memory.  The threads may meet at barrier 1.
-template <int kFmt, int kSub, class Epi>
+// scratch: Epi::scratch(block_rows) bytes of shared memory; Epi::kExact: a long K may be added up in ranges.  The threads may meet at barrier 1.
+template <int kFmt, int kSub, bool kRanges, class Epi>
 __global__ void __launch_bounds__(kPackedThreads, 1)
     tc_packed_kernel(const __grid_constant__ PackedMaps maps, const Packed a, const PackedShape h, const Epi epilogue, int* timeout) {
   extern __shared__ unsigned char smem[];
@@ -133,7 +134,9 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t x_sub = h.block_rows * 128, x_bytes = kSub * x_sub, ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring * x_bytes;
   const int kblocks = (a.K + kStage - 1) / kStage;
-  const int accs = h.block_rows <= 128 ? 2 : 1;
+  const int accs = h.block_rows <= (kRanges ? 64 : 128) ? 2 : 1, seg = kRanges ? h.seg : kblocks;
+  constexpr int acc_cols = kRanges ? 64 : 128;
+  constexpr uint32_t kSumAt = 128;  // of the ranges of a long K, behind the accumulators
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < h.ring; ++i) {
@@ -206,63 +209,79 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     const bool issuer = elect_one();
     int n = 0, s = 0, phase = 0;
     bool ready = false;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
-      const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
-      if (use >= 1 && !(ok = __all_sync(0xffffffffu, wait(acc_empty[acc], (use - 1) & 1)))) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
       const int here = unit_of(h, u, kblocks).kblocks;
-      for (int kb = 0; kb < here; ++kb) {
-        if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+      for (int first = 0; first < here && ok; first += seg, ++n) {
+        const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n, upto = min(here, first + seg);
+        if (use >= 1 && !(ok = __all_sync(0xffffffffu, wait(acc_empty[acc], (use - 1) & 1)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t dx = tile_desc(ring + s * x_bytes);
-        const uint32_t dw = tmem + kOperandAt + s * (kStage / 2), done = smem_u32(&empty[s]);
-        if (++s == h.ring) { s = 0; phase ^= 1; }
-        const bool next = mbar_test(smem_u32(&full[s]), phase);
-        if (issuer) {
+        for (int kb = first; kb < upto; ++kb) {
+          if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dx = tile_desc(ring + s * x_bytes);
+          const uint32_t dw = tmem + kOperandAt + s * (kStage / 2), done = smem_u32(&empty[s]);
+          if (++s == h.ring) { s = 0; phase ^= 1; }
+          const bool next = mbar_test(smem_u32(&full[s]), phase);
+          if (issuer) {
 #pragma unroll
-          for (int k = 0; k < kStage / 16; ++k)
-            mma_from_tmem(tmem + acc * 128, dw + 8 * k, dx + (k / 4) * (x_sub >> 4) + 2 * (k % 4), idesc, (kb | k) != 0);
-          commit(done);
+            for (int k = 0; k < kStage / 16; ++k)
+              mma_from_tmem(tmem + acc * acc_cols, dw + 8 * k, dx + (k / 4) * (x_sub >> 4) + 2 * (k % 4), idesc, kb != first || k != 0);
+            commit(done);
+          }
+          ready = __all_sync(0xffffffffu, next);
         }
-        ready = __all_sync(0xffffffffu, next);
+        if (ok && issuer) commit(smem_u32(&acc_full[acc]));
+        __syncwarp();
       }
-      if (ok && issuer) commit(smem_u32(&acc_full[acc]));
-      __syncwarp();
     }
   } else if (warp >= 2 && warp < 6) {
     // ---- epilogue: a thread owns a token, its TMEM lane, and takes the unit's rows 32 at a time
     const int quad = warp & 3;
     unsigned char* const scratch = smem + (raw_ring - smem_u32(smem)) + h.raws * kRawBytes;
     int n = 0;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
       const PackedUnit un = unit_of(h, u, kblocks);
       const int token = un.n0 + quad * 32 + lane, rows = min(h.block_rows, h.rows - un.r0);
+      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
       const float scale = kFmt == 1 && token < a.V ? __half2float(a.scale[token]) : 1.f;
-      const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
       Epi epi = epilogue;
       epi.begin(token, un.r0, rows, un.split, scratch);
-      // (asleep: these four warps' polling of a wait this long cost the expansion a quarter of its time)
-      for (uint32_t i = 0; i < kSpinLimit && !(ok = mbar_test(smem_u32(&acc_full[acc]), use & 1)) && !failed; ++i) __nanosleep(100);
-      {  // all four warps stay or leave together: an epilogue may have them meet at a barrier
-        uint32_t all;
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.and.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
-        ok = all != 0;
-      }
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (int c = 0; c < rows; c += 32) {
-        float z[32];
-        tmem_ld32(tmem + acc * 128 + c + (static_cast<uint32_t>(quad * 32) << 16), z);
-        if (kFmt == 1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] *= scale;
+      for (int first = 0; first < un.kblocks; first += seg, ++n) {
+        const int acc = accs == 2 ? n & 1 : 0, use = accs == 2 ? n >> 1 : n;
+        const bool last = !kRanges || first + seg >= un.kblocks;
+        // (asleep: these four warps' polling of a wait this long cost the expansion a quarter of its time)
+        for (uint32_t i = 0; i < kSpinLimit && !(ok = mbar_test(smem_u32(&acc_full[acc]), use & 1)) && !failed; ++i) __nanosleep(100);
+        {  // all four warps stay or leave together: an epilogue may have them meet at a barrier
+          uint32_t all;
+          asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\tbar.red.and.pred p, 1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(all) : "r"(static_cast<uint32_t>(ok)) : "memory");
+          ok = all != 0;
         }
-        epi.chunk(c, z, min(32, rows - c));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int c = 0; c < rows; c += 32) {
+          float z[32];
+          tmem_ld32(tmem + lanes + acc * acc_cols + c, z);
+          if (kRanges && first > 0) {
+            float before[32];
+            tmem_ld32(tmem + lanes + kSumAt + c, before);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] += before[i];
+          }
+          if (!last) {
+            tmem_st32(tmem + lanes + kSumAt + c, z);
+            continue;
+          }
+          if (kFmt == 1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] *= scale;
+          }
+          epi.chunk(c, z, min(32, rows - c));
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&acc_empty[acc]));
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive(smem_u32(&acc_empty[acc]));
-      epi.end();
+      if (ok) epi.end();
     }
   } else if (warp >= 8) {
     // ---- expansion: a thread owns a token of the tile, all its weights of a stage; four warps take every fourth stage.  A packed row of
@@ -408,14 +427,14 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// Blocks of rows as equal as sixteens allow, at most kMaxBlockRows each.
-inline void set_row_blocks(PackedShape* h, int rows) {
+// Blocks of rows as equal as sixteens allow, at most `most` each.
+inline void set_row_blocks(PackedShape* h, int rows, int most = kMaxBlockRows) {
   h->rows = rows;
-  h->row_blocks = (rows + kMaxBlockRows - 1) / kMaxBlockRows;
+  h->row_blocks = (rows + most - 1) / most;
   h->block_rows = ((rows + h->row_blocks - 1) / h->row_blocks + 15) & ~15;
 }
 
-template <int kFmt, int kSub, class Epi>
+template <int kFmt, int kSub, bool kRanges, class Epi>
 int launch_stages(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, PackedShape h, const Epi& epi, int sms) {
   constexpr int kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow, kMost = kMaxRing / kSub;
   PackedMaps maps;
@@ -431,7 +450,7 @@ int launch_stages(cudaStream_t stream, const char* what, const half* x, const vo
   }
   const size_t smem = 1024 + scratch + static_cast<size_t>(h.ring) * x_bytes + static_cast<size_t>(h.raws) * kRawBytes;
   RK_REQUIRE(h.ring >= kTurns, kShape, "%s: no room for four stages", what);
-  const auto kernel = tc_packed_kernel<kFmt, kSub, Epi>;
+  const auto kernel = tc_packed_kernel<kFmt, kSub, kRanges, Epi>;
   RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemBytes)));
   RK_CUDA(launch_pdl(kernel, dim3(std::min(h.units, sms)), dim3(kPackedThreads), smem, stream, maps, a, h, epi, timeout_word_or_null()));
   RK_LAUNCH_CHECK(what);
@@ -439,7 +458,9 @@ int launch_stages(cudaStream_t stream, const char* what, const half* x, const vo
 }
 template <int kFmt, class Epi>
 int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, const PackedShape& h, const Epi& epi, int sms) {
-  return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1>(stream, what, x, w, a, h, epi, sms);
+  if constexpr (Epi::kExact)
+    if (h.seg < h.kb_per_split) return launch_stages<kFmt, 2, true>(stream, what, x, w, a, h, epi, sms);
+  return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2, false>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
 }
 
 }  // namespace tc

@@ -17,6 +17,7 @@ namespace tc {
 
 constexpr int kRows = 128;  // rows of x per unit = MMA M
 constexpr int kToks = 256;  // tokens per unit = MMA N, at most (Shape::toks)
+constexpr int kRangeToks = 160;  // two accumulators and the sum of the ranges fit into tensor memory
 constexpr int kMaxTiles = 8;
 constexpr int kRowsThreads = 192;
 
@@ -25,6 +26,7 @@ struct Shape {
   int row_blocks;   // blocks of 128 rows
   int units;
   int x_rows;       // rows of x that a block loads: all there are, in eights, up to 128 (the rest of the tile is not read out)
+  int seg;          // K blocks that are added up in one accumulator: all, or kRangeK's where K is long (toks at most kRangeToks then)
   int ring;         // stages; a stage is a tile of x, then one of weights (set by launch_rows, like the next two)
   uint32_t x_bytes, tile_bytes;
 };
@@ -44,6 +46,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t ring = (smem_u32(smem) + 1023u) & ~1023u;
   const int kblocks = (K + kBK - 1) / kBK;
+  const uint32_t acc_cols = h.seg < kblocks ? kRangeToks : kToks, sum_at = 2 * kRangeToks;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < h.ring; ++i) {
@@ -101,48 +104,61 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
     const bool issuer = elect_one();
     int n = 0, s = 0, phase = 0;
     bool ready = false;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
-      if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait(acc_empty[n & 1], ((n >> 1) - 1) & 1)))) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t acc = tmem + (n & 1) * kToks;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
+      for (int first = 0; first < kblocks && ok; first += h.seg, ++n) {
+        if (n >= 2 && !(ok = __all_sync(0xffffffffu, wait(acc_empty[n & 1], ((n >> 1) - 1) & 1)))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t dx = tile_desc(ring + s * h.tile_bytes), dw = tile_desc(ring + s * h.tile_bytes + h.x_bytes);
-        const uint32_t done = smem_u32(&empty[s]);
-        if (++s == h.ring) { s = 0; phase ^= 1; }
-        const bool next = mbar_test(smem_u32(&full[s]), phase);
-        if (issuer) {
+        const uint32_t acc = tmem + (n & 1) * acc_cols;
+        for (int kb = first, upto = min(kblocks, first + h.seg); kb < upto; ++kb) {
+          if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t dx = tile_desc(ring + s * h.tile_bytes), dw = tile_desc(ring + s * h.tile_bytes + h.x_bytes);
+          const uint32_t done = smem_u32(&empty[s]);
+          if (++s == h.ring) { s = 0; phase ^= 1; }
+          const bool next = mbar_test(smem_u32(&full[s]), phase);
+          if (issuer) {
 #pragma unroll
-          for (int k4 = 0; k4 < kBK / 16; ++k4) mma(acc, dx + 2 * k4, dw + 2 * k4, idesc, (kb | k4) != 0);
-          commit(done);
+            for (int k4 = 0; k4 < kBK / 16; ++k4) mma(acc, dx + 2 * k4, dw + 2 * k4, idesc, kb != first || k4 != 0);
+            commit(done);
+          }
+          ready = __all_sync(0xffffffffu, next);
         }
-        ready = __all_sync(0xffffffffu, next);
+        if (ok && issuer) commit(smem_u32(&acc_full[n & 1]));
+        __syncwarp();
       }
-      if (ok && issuer) commit(smem_u32(&acc_full[n & 1]));
-      __syncwarp();
     }
   } else {
     // ---- epilogue: a thread owns a row of x, its TMEM lane, and takes the unit's tokens 32 at a time
     const int quad = warp & 3;
     int n = 0;
-    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x, ++n) {
+    for (int u = blockIdx.x; u < h.units && ok; u += gridDim.x) {
       const int r = u % h.row_blocks * kRows + quad * 32 + lane, n0 = u / h.row_blocks * h.toks, toks = min(h.toks, V - n0);
-      ok = __all_sync(0xffffffffu, wait(acc_full[n & 1], (n >> 1) & 1));
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      Epi epi = epilogue;
       const bool some = r - lane < epilogue.rows();  // (nothing to do for a warp beyond the last row)
-      if (r < epilogue.rows()) epi.begin(r, n0, toks);
-      for (int c = 0; c < toks && some; c += 32) {
-        float z[32];
-        tmem_ld32(tmem + (n & 1) * kToks + c + (static_cast<uint32_t>(quad * 32) << 16), z);
-        if (r < epilogue.rows()) epi.chunk(c, z, min(32, toks - c));
+      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+      Epi epi = epilogue;
+      for (int first = 0; first < kblocks; first += h.seg, ++n) {
+        const bool last = first + h.seg >= kblocks;
+        ok = __all_sync(0xffffffffu, wait(acc_full[n & 1], (n >> 1) & 1));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (last && r < epilogue.rows()) epi.begin(r, n0, toks);
+        for (int c = 0; c < toks && some; c += 32) {
+          float z[32];
+          tmem_ld32(tmem + lanes + (n & 1) * acc_cols + c, z);
+          if (first > 0) {
+            float before[32];
+            tmem_ld32(tmem + lanes + sum_at + c, before);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] += before[i];
+          }
+          if (!last) tmem_st32(tmem + lanes + sum_at + c, z);
+          else if (r < epilogue.rows()) epi.chunk(c, z, min(32, toks - c));
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&acc_empty[n & 1]));
       }
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) arrive(smem_u32(&acc_empty[n & 1]));
-      if (r < epilogue.rows()) epi.end();
+      if (ok && r < epilogue.rows()) epi.end();
     }
   }
   if (!ok) failed = 1;

@@ -595,6 +595,7 @@ __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("
 
 // A token's (channel's) results for the unit's rows to y, or to the unit's plane of partial sums; a warp's 32 channels are neighbours.
 struct ProductEpilogue {
+  static constexpr bool kExact = false;  // (the result is rounded to half, beside which the sum's error is small)
   static int scratch(int) { return 4 * 2048; }
   void* y;
   float* partial;  // [splits][rows][N], or nullptr
@@ -699,6 +700,7 @@ tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int 
     h.tiles = (N + tc::kTileToks - 1) / tc::kTileToks;
     h.kb_per_split = (kblocks + want - 1) / want;
     h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
+    h.seg = h.kb_per_split;
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
     const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;

@@ -209,6 +209,13 @@ def test_head_shapes(ops, rows, V, K, fmt, group, symmetric):
     check_head(ops, x, tok, weight, w64, group, f"{fmt} {rows}x{V}x{K}")
 
 
+@pytest.mark.parametrize("fmt,group", [("f16", 128), ("w8", 128), ("w4", 32), ("w4", 64), ("w4", 128)])
+@pytest.mark.parametrize("rows,V,K", [(9, 300, 2080), (70, 129, 4128), (130, 515, 8192), (300, 200, 3136)])
+def test_head_long_k(ops, rows, V, K, fmt, group):
+    """Long sums go in ranges: tiles and blocks of their own, tails of a range and of a stage."""
+    check_head(ops, *head_case(rows, V, K, fmt, group, seed=K), group, f"{rows}x{V}x{K} {fmt} g{group}")
+
+
 def test_head_special_rows(ops):
     """A row whose logits overflow answers NaN and leaves its neighbours alone; ids outside the vocabulary; no tokens at all."""
     x, tok, (w, _, _), w64 = head_case(6, 300, 64, "f16", 128)
