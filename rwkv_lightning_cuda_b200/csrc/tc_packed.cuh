@@ -358,10 +358,6 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           uint4 q[kLoads];
 #pragma unroll
           for (int c = 0; c < kLoads; ++c) q[c] = lds16(src + ((16 * (kLoads * sub + c)) ^ raw_swz));
-          if (sub == kSub - 1) {
-            __syncwarp();
-            if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
-          }
           if (sub == 0) {
             if (stored >= 0) hand_over(stored);
             ok = __all_sync(0xffffffffu, first_round || wait(empty[s], phase ^ 1));
@@ -400,6 +396,10 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           }
         }
         if (!ok) break;
+        // The packed tile is given back only now that its words have gone into the stores above: an arrival right behind the loads did
+        // not wait for them, and the next tile came in under them.
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
         if (kFmt == 2 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
         stored = s;
         rs += kTurns;
