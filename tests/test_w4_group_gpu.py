@@ -131,6 +131,18 @@ def test_nothing_behind_k_counts(ops, K, group):
         assert bool(torch.isfinite(entropy).all()) and bool(torch.isfinite(lse).all())
 
 
+@pytest.mark.parametrize("M,N,K", [(100, 200, 6176), (128, 200, 3136), (200, 2000, 6176)])
+def test_long_products_again_and_again(ops, M, N, K):
+    """Rings that go round many times under slow expansion (two groups to 64 weights): the same right answer every time."""
+    gen = torch.Generator().manual_seed(K)
+    q, s, z = random_w4(N, K, 32, False, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    first = ops.linear_w4a16_group(x, q, s, z, 32)
+    check_product(first, x, (q, s, z), 32, "first")
+    for _ in range(30):
+        assert torch.equal(ops.linear_w4a16_group(x, q, s, z, 32), first)
+
+
 def test_codes_one_at_a_time(ops):
     """Each of the 16 codes at each place of a word, and each group's own scale: one weight at a time against one activation."""
     K, group = 288, 32
