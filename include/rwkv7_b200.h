@@ -51,6 +51,7 @@ extern "C" {
 #define RWKV7_B200_EPI_NONE 0
 #define RWKV7_B200_EPI_RELU2 1
 #define RWKV7_B200_EPI_F32 3
+#define RWKV7_B200_EPI_EXACT 16  /* or-ed to the epilogue of rwkv7_b200_linear_w4a16_group: no weight is rounded */
 
 const char* rwkv7_b200_last_error(void);
 /* Compiled-in facts a binding can check at load time: head size (64) and ABI version. */
@@ -387,9 +388,11 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
 /* 4-bit weights with group scales (no counterpart in the reference): W[n,k] = (q[n,k] - zero[n,g]) * scale[n,g] with
  * g = k / group, group 32, 64 or 128, a short last group allowed (scale and zero are [N][ceil(K / group)]), zero NULL: 8
  * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 8 rows
- * the scale multiplies the group's fp32 sum, so no weight is rounded; with more rows weights count as
- * half((q - zero) * scale), and zeros have to be whole numbers.  workspace is scratch of the size the first function returns (which may be 0); without it, or
- * with less, products of many rows run on fewer SMs.  Calls that may overlap on the GPU need one each. */
+ * the scale multiplies the group's fp32 sum, so no weight is rounded.  With more rows weights count as
+ * half((q - zero) * scale); with RWKV7_B200_EPI_EXACT or-ed to the epilogue none is rounded there either, at twice the
+ * products (a weight is the sum of two halves then, so it has to be below 65504).  With more than 8 rows zeros have to be
+ * whole numbers.  workspace is scratch of the size the first function returns (which may be 0); without it, or with less,
+ * products of many rows run on fewer SMs.  Calls that may overlap on the GPU need one each. */
 int rwkv7_b200_linear_w4a16_group_workspace(int M, int K, int N, size_t* bytes);
 int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q,
                                   const uint16_t* scale, const uint16_t* zero, int group, int epilogue, void* y,

@@ -368,7 +368,8 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
 int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q, const uint16_t* scale,
                                   const uint16_t* zero, int group, int epilogue, void* y, void* workspace, size_t workspace_bytes) {
   rk::W4GroupArgs a;
-  a.M = M; a.K = K; a.N = N; a.group = group; a.x = h(x); a.q = q; a.scale = h(scale); a.zero = h(zero); a.epi = epilogue; a.y = y;
+  a.M = M; a.K = K; a.N = N; a.group = group; a.x = h(x); a.q = q; a.scale = h(scale); a.zero = h(zero); a.y = y;
+  a.epi = epilogue & ~RWKV7_B200_EPI_EXACT; a.exact = (epilogue & RWKV7_B200_EPI_EXACT) != 0;
   return rk::w4_group_linear(st(stream), a, workspace, workspace_bytes);
 }
 int rwkv7_b200_linear_w4a16_group_workspace(int M, int K, int N, size_t* bytes) {

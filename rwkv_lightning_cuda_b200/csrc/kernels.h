@@ -224,6 +224,7 @@ struct W4GroupArgs {
   const half* scale = nullptr;  // [N, ceil(K / group)]
   const half* zero = nullptr;   // as scale, or nullptr: 8
   int epi = kEpiNone;           // kEpiNone, kEpiRelu2 or kEpiF32 (w4_rounded_linear: kEpiRawF32 too)
+  bool exact = false;           // more than eight rows: no weight is rounded there either
   void* y = nullptr;            // half [M, N], or float for kEpiF32
 };
 // The product of up to eight rows with weights rounded to half, half((q - zero) * scale), as the tensor-core kernels take them.

@@ -33,9 +33,13 @@ constexpr int kOperandAt = 256;    // columns of tensor memory behind the accumu
 // kSub: K blocks of 64 to a stage.  Two with up to 128 rows, where what every role does once per stage bounds; with more rows there is
 // no room for four such stages.
 __host__ __device__ constexpr int subs(int block_rows) { return block_rows <= 128 ? 2 : 1; }
+// kFmt: 1 int8; 2 and 3 4-bit, the weights as halves, or (3) as two halves whose sum they are exactly, each multiplied with x.
+// Two halves take twice the columns of a stage, so that stages are of 64 then.
+template <int kFmt, int kSub> __host__ __device__ constexpr int stage_cols() { return kSub * kBK / 2 * (kFmt == 3 ? 2 : 1); }
 template <int kFmt, int kSub> __host__ __device__ constexpr int raw_row() { return kSub * (kFmt == 1 ? kBK : kBK / 2); }  // bytes of a packed row of a stage
 
-// int8 with a scale per token (applied to the sums), or 4 bits with scales and zeros per group (half((q - zero) * scale)).
+// int8 with a scale per token (applied to the sums), or 4 bits with scales and zeros per group: half((q - zero) * scale), or that and the
+// half that is missing to (q - zero) * scale.
 struct Packed {
   int V, K;
   int group;                 // 4 bits: 32, 64 or 128
@@ -96,6 +100,22 @@ __device__ __forceinline__ uint4 expand4(uint32_t w, const Group4& g, const Expa
   }
   return make_uint4(h[0], h[1], h[2], h[3]);
 }
+// The same and what the rounding took off.  (q - zero) * scale is a whole number of at most four bits times the scale, so it is a
+// multiple of the scale's last place, and so is what it is off its rounding: a half, which the fused multiply-add gives exactly.
+__device__ __forceinline__ void expand4(uint32_t w, const Group4& g, const Expand4& e, uint4* high, uint4* low) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const uint32_t both = __byte_perm(w, 0u, 0x4040u + 0x0101u * b);
+    uint32_t pair;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(pair) : "r"(both), "r"(e.nibbles), "r"(e.bias));
+    const __half2 d = __hfma2(*reinterpret_cast<__half2*>(&pair), e.mul, g.sub), v = __hmul2(d, g.scale), o = __hfma2(d, g.scale, __hneg2(v));
+    h[b] = *reinterpret_cast<const uint32_t*>(&v);
+    l[b] = *reinterpret_cast<const uint32_t*>(&o);
+  }
+  *high = make_uint4(h[0], h[1], h[2], h[3]);
+  *low = make_uint4(l[0], l[1], l[2], l[3]);
+}
 // Four int8 codes to four halves, exactly: code + 128 under the exponent of 1024, less 1152.
 __device__ __forceinline__ uint2 expand8(uint32_t w) {
   const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
@@ -130,6 +150,9 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int failed;
   constexpr int kStage = kSub * kBK;  // weights of a token per stage
+  constexpr bool kTwo = kFmt == 3;    // two halves to a weight
+  constexpr int kCols = stage_cols<kFmt, kSub>();
+  static_assert(kTurns * kCols <= static_cast<int>(kTmemCols) - kOperandAt, "four stages of expanded weights at least");
   constexpr uint32_t kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const uint32_t x_sub = h.block_rows * 128, x_bytes = kSub * x_sub, ring = (smem_u32(smem) + 1023u) & ~1023u, raw_ring = ring + h.ring * x_bytes;
@@ -219,13 +242,16 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           if (!ready && !(ok = __all_sync(0xffffffffu, wait(full[s], phase)))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint64_t dx = tile_desc(ring + s * x_bytes);
-          const uint32_t dw = tmem + kOperandAt + s * (kStage / 2), done = smem_u32(&empty[s]);
+          const uint32_t dw = tmem + kOperandAt + s * kCols, done = smem_u32(&empty[s]);
           if (++s == h.ring) { s = 0; phase ^= 1; }
           const bool next = mbar_test(smem_u32(&full[s]), phase);
           if (issuer) {
 #pragma unroll
-            for (int k = 0; k < kStage / 16; ++k)
-              mma_from_tmem(tmem + acc * acc_cols, dw + 8 * k, dx + (k / 4) * (x_sub >> 4) + 2 * (k % 4), idesc, kb != first || k != 0);
+            for (int k = 0; k < kStage / 16; ++k) {
+              const uint64_t dxk = dx + (k / 4) * (x_sub >> 4) + 2 * (k % 4);
+              mma_from_tmem(tmem + acc * acc_cols, dw + 8 * k, dxk, idesc, kb != first || k != 0);
+              if (kTwo) mma_from_tmem(tmem + acc * acc_cols, dw + kCols / 2 + 8 * k, dxk, idesc, 1);
+            }
             commit(done);
           }
           ready = __all_sync(0xffffffffu, next);
@@ -334,7 +360,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       const int row = min(un.n0 + r, a.V - 1), kb_end = un.kb0 + un.kblocks;
       int kb = un.kb0 + ((turn - it) & (kTurns - 1));
       int block = -1, ahead = -1;
-      if (kFmt == 2 && kb < kb_end) {
+      if (kFmt != 1 && kb < kb_end) {
         sp = reinterpret_cast<const uint16_t*>(a.scale) + static_cast<size_t>(row) * groups;
         if (a.zero) zp = reinterpret_cast<const uint16_t*>(a.zero) + static_cast<size_t>(row) * groups;
         if (eights) load8(ahead = eight_of(kb));
@@ -342,12 +368,12 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
       }
       for (; kb < kb_end; kb += kTurns) {
         const bool first_round = it + kb - un.kb0 < h.ring;
-        if (kFmt == 2 && (!eights || ahead != block)) {
+        if (kFmt != 1 && (!eights || ahead != block)) {
           sc = sc_next;
           ze = ze_next;
           block = ahead;
         }
-        if (kFmt == 2 && eights && eight_of(kb + kTurns) != block) load8(ahead = eight_of(kb + kTurns));
+        if (kFmt != 1 && eights && eight_of(kb + kTurns) != block) load8(ahead = eight_of(kb + kTurns));
         ok = __all_sync(0xffffffffu, wait(raw_full[rs], raw_phase));
         if (!ok) break;
         const uint32_t src = raw + rs * kRawBytes;
@@ -366,7 +392,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
           }
 #pragma unroll
           for (int c = 0; c < 2; ++c) {  // 32 weights at a time: more would take too many registers
-            uint32_t o[16];
+            uint32_t o[16], rest[16];  // (rest: kTwo)
             if (kFmt == 1) {
               const uint32_t w[8] = {q[2 * c].x, q[2 * c].y, q[2 * c].z, q[2 * c].w, q[2 * c + 1].x, q[2 * c + 1].y, q[2 * c + 1].z, q[2 * c + 1].w};
 #pragma unroll
@@ -385,14 +411,21 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
               const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const uint4 p = expand4(w[j], g, e4);
+                uint4 p, r = make_uint4(0u, 0u, 0u, 0u);
+                if (kTwo) expand4(w[j], g, e4, &p, &r);
+                else p = expand4(w[j], g, e4);
                 o[4 * j] = p.x;
                 o[4 * j + 1] = p.y;
                 o[4 * j + 2] = p.z;
                 o[4 * j + 3] = p.w;
+                rest[4 * j] = r.x;
+                rest[4 * j + 1] = r.y;
+                rest[4 * j + 2] = r.z;
+                rest[4 * j + 3] = r.w;
               }
             }
-            tmem_st16(operand + s * (kStage / 2) + 32 * sub + 16 * c, o);
+            tmem_st16(operand + s * kCols + 32 * sub + 16 * c, o);
+            if (kTwo) tmem_st16(operand + s * kCols + kCols / 2 + 32 * sub + 16 * c, rest);
           }
         }
         if (!ok) break;
@@ -400,7 +433,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
         // not wait for them, and the next tile came in under them.
         __syncwarp();
         if (lane == 0) arrive(smem_u32(&raw_empty[rs]));
-        if (kFmt == 2 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
+        if (kFmt != 1 && !eights && kb + kTurns < kb_end) load_runs(kb + kTurns);  // under way until this thread's next turn
         stored = s;
         rs += kTurns;
         if (rs >= h.raws) { rs -= h.raws; raw_phase ^= 1; }
@@ -436,7 +469,7 @@ inline void set_row_blocks(PackedShape* h, int rows, int most = kMaxBlockRows) {
 
 template <int kFmt, int kSub, bool kRanges, class Epi>
 int launch_stages(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, PackedShape h, const Epi& epi, int sms) {
-  constexpr int kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow, kMost = kMaxRing / kSub;
+  constexpr int kRawRow = raw_row<kFmt, kSub>(), kRawBytes = kTileToks * kRawRow, kMost = std::min<int>(kMaxRing, (kTmemCols - kOperandAt) / stage_cols<kFmt, kSub>());
   PackedMaps maps;
   int s = encode_map(what, &maps.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x, h.rows, a.K, kBK, h.block_rows, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s == kOk)
@@ -460,7 +493,8 @@ template <int kFmt, class Epi>
 int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, const PackedShape& h, const Epi& epi, int sms) {
   if constexpr (Epi::kExact)
     if (h.seg < h.kb_per_split) return launch_stages<kFmt, 2, true>(stream, what, x, w, a, h, epi, sms);
-  return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2, false>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
+  if constexpr (kFmt == 3) return launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
+  else return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2, false>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
 }
 
 }  // namespace tc

@@ -588,7 +588,9 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
   return matvec(stream, a, p, true);
 }
 
-// ---- more rows: the tensor-core skeleton of tc_packed.cuh, weights rounded to half
+// ---- more rows: the tensor-core skeleton of tc_packed.cuh, weights rounded to half, or as two halves each where the caller wants none
+// rounded: an instruction more per two weights, twice the stores and products, and stages of 64 (96 rows of 10240 x 2560 19.2 us, 14.0 rounded;
+// 24 of 65536 x 4096 81 and 59; 256 of 16384 x 4096 48 and 30; nine of 10240 x 2560 16.2 and 13.8).
 namespace {
 
 __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
@@ -687,13 +689,14 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
 // cores 2.35 a row; a unit's results take 25 a row, hidden under the next unit's products where there are two accumulators; the
 // second kernel 3000, 200 a range and its traffic.  (64 rows of 1024 x 1024: 7.5 us whole, 6.5 in eight ranges, 7.9 in sixteen; 96
 // rows of 10240 x 2560: 15.7 whole, 19.0 in two, 16.2 in three; 96 rows of 2560 x 10240: 43.7 whole, 15.7 in seven, 19.6 in nine,
-// which is a second wave: with stages of 64, those of 128 take a tenth less of all of them.)
-tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int sms) {
+// which is a second wave: with stages of 64, those of 128 take a tenth less of all of them.)  Exact weights, two halves each, have
+// stages of 64, which take 600 to 760 clocks, and twice the products.
+tc::PackedShape many_rows_shape(int M, int K, int N, bool exact, size_t scratch_floats, int sms) {
   tc::PackedShape best = {};
   double least = 0;
   tc::PackedShape rows = {};
   tc::set_row_blocks(&rows, M);
-  const int stage = tc::kBK * tc::subs(rows.block_rows), kblocks = (K + stage - 1) / stage;
+  const int stage = tc::kBK * (exact ? 1 : tc::subs(rows.block_rows)), kblocks = (K + stage - 1) / stage;
   const size_t plane = static_cast<size_t>(M) * N;
   for (int want = 1; want <= 16 && want <= kblocks; ++want) {
     tc::PackedShape h = rows;
@@ -704,7 +707,7 @@ tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int 
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
     const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;
-    double cost = waves * (h.kb_per_split * std::max(stage * 6.0, stage * h.block_rows / 27.0)) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
+    double cost = waves * (h.kb_per_split * std::max(stage * (exact ? 10.0 : 6.0), stage * h.block_rows / (exact ? 13.5 : 27.0))) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
     if (h.splits > 1) cost += 3000 + 200 * h.splits + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
     if (best.units == 0 || cost < least) { least = cost; best = h; }
@@ -713,13 +716,14 @@ tc::PackedShape many_rows_shape(int M, int K, int N, size_t scratch_floats, int 
 }
 
 int many_rows(cudaStream_t stream, const W4GroupArgs& a, float* scratch, size_t scratch_bytes, int sms) {
-  const tc::PackedShape h = many_rows_shape(a.M, a.K, a.N, scratch ? scratch_bytes / sizeof(float) : 0, sms);
+  const tc::PackedShape h = many_rows_shape(a.M, a.K, a.N, a.exact, scratch ? scratch_bytes / sizeof(float) : 0, sms);
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "linear_w4a16_group: too many rows");
   tc::Packed w;
   w.V = a.N; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
   ProductEpilogue epi;
   epi.y = a.y; epi.partial = h.splits > 1 ? scratch : nullptr; epi.n_rows = a.M; epi.N = a.N; epi.epi = a.epi;
-  const int s = tc::launch_packed<2>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms);
+  const int s = a.exact ? tc::launch_packed<3>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms)
+                        : tc::launch_packed<2>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms);
   if (s != kOk || h.splits == 1) return s;
   const size_t quads = static_cast<size_t>(a.M) * a.N / 4;
   RK_CUDA(launch_pdl(w4_reduce_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, epi, h.splits));
@@ -733,8 +737,9 @@ size_t w4_group_workspace(int M, int K, int N) {
   if (M <= kMaxRows || N % 4 != 0) return 0;
   int sms = 148;
   if (device_sms(&sms) != kOk) sms = 148;
-  const tc::PackedShape h = many_rows_shape(M, K, N, ~static_cast<size_t>(0) / 8, sms);
-  return h.splits > 1 ? static_cast<size_t>(h.splits) * M * N * sizeof(float) : 0;
+  const size_t any = ~static_cast<size_t>(0) / 8;
+  const int splits = std::max(many_rows_shape(M, K, N, false, any, sms).splits, many_rows_shape(M, K, N, true, any, sms).splits);
+  return splits > 1 ? static_cast<size_t>(splits) * M * N * sizeof(float) : 0;
 }
 
 int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, size_t workspace_bytes) {

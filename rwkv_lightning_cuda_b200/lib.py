@@ -11,6 +11,7 @@ FMT_F16, FMT_W8A16, FMT_W4A16 = 0, 1, 2
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 ACT_NONE, ACT_TANH, ACT_SIGMOID = 0, 1, 2
 EPI_NONE, EPI_RELU2, EPI_F32 = 0, 1, 3
+EPI_EXACT = 16  # or-ed to the epilogue of linear_w4a16_group
 
 STATUS_NAMES = {0: "OK", 1: "BAD_ARG", 2: "SHAPE", 3: "PRECISION", 4: "CUDA", 5: "NCCL", 6: "TIMEOUT", 7: "NOT_READY"}
 

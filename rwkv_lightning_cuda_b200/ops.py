@@ -369,10 +369,11 @@ def _refuse_linear_w4a16_group(x, q, scale, zero, group_size):
     _need(False, "linear_w4a16_group: bad argument")
 
 
-def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NONE):
+def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NONE, exact=False):
     """x W^T for 4-bit weights with group scales: W = (q - zero) * scale per group of 32, 64 or 128 inputs; x fp16 [M, K], q
     uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N.  Up to 8
-    rows no weight is rounded; with more a weight counts as half((q - zero) * scale), and zeros have to be whole numbers."""
+    rows no weight is rounded; with more a weight counts as half((q - zero) * scale), unless ``exact`` asks for weights that are not
+    rounded there either (at twice the products).  With more than 8 rows zeros have to be whole numbers."""
     ok = isinstance(x, torch.Tensor) and isinstance(q, torch.Tensor) and x.dim() == 2 and q.dim() == 2 and x.is_cuda
     if ok:
         (M, K), N, dev = x.shape, q.shape[0], x.device
@@ -386,7 +387,7 @@ def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NO
         need = _scratch_bytes("rwkv7_b200_linear_w4a16_group_workspace", M, K, N)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _enqueue(dev, L.load_library().rwkv7_b200_linear_w4a16_group, M, K, N, x.data_ptr(), q.data_ptr(), scale.data_ptr(),
-             None if zero is None else zero.data_ptr(), group_size, epilogue, y.data_ptr(), work.data_ptr() if need else None, need)
+             None if zero is None else zero.data_ptr(), group_size, epilogue | L.EPI_EXACT if exact else epilogue, y.data_ptr(), work.data_ptr() if need else None, need)
     return y
 
 

@@ -58,6 +58,21 @@ def test_linear_w4a16_group_refusals(lib):
     assert unpack(None, 0, 64, 32, P, P, P, P) == 1 and unpack(None, 4, 64, 32, P, P, P, None) == 1
 
 
+def test_exact_flag_of_the_4bit_product(lib):
+    """Or-ed to a known epilogue it is none of its own; other bits, and other linear layers, stay refused.  The scratch asked for serves both forms."""
+    from rwkv_lightning_cuda_b200 import lib as L
+    def call(epi, K=72):
+        return lib.rwkv7_b200_linear_w4a16_group(None, 1, K, 4, P, P, P, None, 32, epi, P, None, 0)
+    for epi in (0, 1, 3):
+        assert call(epi | L.EPI_EXACT) == 2 and b"multiple of 32" in lib.rwkv7_b200_last_error()  # (refused for its K)
+    for epi in (2, 4, 32, 64):
+        assert call(epi | L.EPI_EXACT, 64) == 1 and b"epilogue" in lib.rwkv7_b200_last_error()
+    assert lib.rwkv7_b200_linear_w4a16(None, 1, 128, 4, P, P, P, P, L.EPI_EXACT, P) == 1
+    need = C.c_size_t()
+    assert lib.rwkv7_b200_linear_w4a16_group_workspace(96, 10272, 2560, C.byref(need)) == 0 and need.value > 0
+    assert lib.rwkv7_b200_linear_w4a16_group_workspace(8, 10272, 2560, C.byref(need)) == 0 and need.value == 0
+
+
 def test_python_layer_refuses_before_it_calls():
     """CPU tensors, wrong types, shapes and layouts: an error that names the argument (the device tensors' own checks run in the
     GPU tests)."""

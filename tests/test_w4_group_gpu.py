@@ -76,6 +76,75 @@ def test_many_rows(ops, M, N, K, group, symmetric):
     check_product(ops.linear_w4a16_group(x, q, s, z, group), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
 
 
+def check_exact(y, x, weight, group, what):
+    """As check_product at any number of rows: no weight is rounded.  With 9 rows and more a weight is two halves, whose products come one after the
+    other: K / 8 additions to the running sum instead of K / 16."""
+    x64 = x.cpu().double()
+    want = x64 @ w4_weights(*weight, group).T
+    size = x64.abs() @ w4_weights(*weight, group, parts=True).T
+    bound = size * (x.shape[1] / 8 + 64) * 2 * U32 + want.abs() * U16 * (1 + 1e-3) + 2.0 ** -25
+    off = (y.detach().cpu().double() - want).abs() - bound
+    assert float(off.max()) <= 0, f"{what}: off by {float((y.cpu().double() - want).abs().max()):.3g}"
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 288), (8, 33, 96), (9, 33, 288), (16, 65, 32), (17, 128, 128), (33, 130, 416), (65, 300, 64), (96, 1024, 2560), (129, 128, 160),
+                                   (200, 37, 1056), (256, 516, 288), (300, 40, 4128), (513, 4, 96)])
+def test_exact_products(ops, M, N, K, group, symmetric):
+    """Asked for, no weight is rounded with many rows either: at short K the rounding of the weights is several times what this allows."""
+    gen = torch.Generator().manual_seed(M + N + K + group)
+    q, s, z = random_w4(N, K, group, symmetric, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    check_exact(ops.linear_w4a16_group(x, q, s, z, group, exact=True), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
+
+
+def test_exact_products_one_weight_at_a_time(ops):
+    """Every code, zero and place of a word against one activation: the weight itself, rounded once to half, at scales that need all their bits."""
+    K, N, group = 256, 256, 32
+    for code in range(16):
+        w = torch.full((N, K), 5, dtype=torch.uint8)
+        w[torch.arange(N), torch.arange(K)] = code
+        q = (w[:, 0::2] | (w[:, 1::2] << 4)).cuda()
+        s = (1 + torch.arange(1, N * K // group + 1).reshape(N, -1) / 1024 * 0.999).half().cuda()
+        z = (torch.arange(N * K // group).reshape(N, -1) % 16).half().cuda()
+        x = torch.eye(K).half().cuda()  # row m picks weight m of every channel
+        y = ops.linear_w4a16_group(x, q, s, z, group, exact=True)
+        want = w4_weights(q, s, z, group).T
+        assert torch.equal(y.cpu(), want.half())
+        assert torch.equal(ops.linear_w4a16_group(torch.cat([x, -x]), q, s, z, group, exact=True)[K:], -y)
+
+
+def test_exact_products_keep_what_rounding_takes_off(ops):
+    """Activations of opposite sign on two weights whose difference is not a whole number of the steps they would be rounded to: it survives."""
+    M, N, K, group = 40, 64, 64, 32
+    w = torch.zeros(N, K, dtype=torch.uint8)
+    w[:, 0], w[:, 32] = 15, 15
+    q = (w[:, 0::2] | (w[:, 1::2] << 4)).cuda()
+    base = 1 + torch.arange(N) / 1024
+    s = torch.stack([base, base + 1 / 1024], 1).half().cuda()  # 15 * 2^-10 apart, weights with steps of 2^-7
+    z = torch.zeros(N, 2).half().cuda()
+    x = torch.zeros(M, K).half().cuda()
+    x[:, 0], x[:, 32] = -1, 1
+    want = (15 * (s[:, 1].double() - s[:, 0].double())).half()
+    assert torch.equal(ops.linear_w4a16_group(x, q, s, z, group, exact=True), want.expand(M, N))
+
+
+def test_exact_epilogues_and_repeats(ops):
+    from rwkv_lightning_cuda_b200 import lib as L
+    gen = torch.Generator().manual_seed(12)
+    q, s, z = random_w4(516, 2080, 32, False, gen)
+    for M in (5, 9, 20, 70, 150, 260):
+        x = torch.randn(M, 2080, generator=gen).half().cuda()
+        y = ops.linear_w4a16_group(x, q, s, z, 32, exact=True)
+        y32 = ops.linear_w4a16_group(x, q, s, z, 32, epilogue=L.EPI_F32, exact=True)
+        assert y32.dtype == torch.float32 and torch.equal(y32, y.float())
+        relu2 = ops.linear_w4a16_group(x, q, s, z, 32, epilogue=L.EPI_RELU2, exact=True)
+        assert torch.equal(relu2, (y.float().clamp(min=0) ** 2).half())
+        for _ in range(10):
+            assert torch.equal(ops.linear_w4a16_group(x, q, s, z, 32, exact=True), y)
+
+
 def test_epilogues(ops):
     from rwkv_lightning_cuda_b200 import lib as L
     gen = torch.Generator().manual_seed(2)
