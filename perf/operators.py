@@ -136,7 +136,7 @@ def run(state):
             names = ("logprobs", "entropy", "lse", "top_ids", "top_logprobs")
             return dict(zip(names, ops.token_logprobs(state["logits"], state["tokens"], top_k=state["top"])))
         if state["op"] == "w4":
-            return {"y": ops.linear_w4a16_group(state["x"], state["q"], state["scale"], state["zero"], group_size=state["group"])}
+            return {"y": ops.linear_w4a16_group(state["x"], state["q"], state["scale"], state["zero"], group_size=state["group"], exact=True)}
         names = ("logprobs", "entropy", "lse")
         return dict(zip(names, ops.head_logprobs(state["x"], state["w"], state["tokens"], scale=state["scale"], zero=state["zero"],
                                                  group_size=state["group"])))
