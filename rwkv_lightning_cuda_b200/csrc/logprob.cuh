@@ -8,7 +8,8 @@
 //   all masked    lse -inf, every log probability -inf, entropy 0
 //   NaN or +inf   the row has no distribution: lse, entropy and log probabilities are NaN, there are no alternatives
 // m starts at -FLT_MAX instead of -inf, so that z - m is never inf - inf for a masked token, and takes part in a maximum
-// that keeps NaN; differences are cut off below at kFar (their exponential is 0 long before), so that 0 * -inf never is.
+// that keeps NaN; differences are cut off below at kFar (their exponential is 0 long before, and its product with a sum of 2^30
+// terms is finite), so that 0 * -inf never is.
 #pragma once
 
 #include <cfloat>
@@ -20,7 +21,7 @@ namespace rk {
 #ifdef __CUDACC__
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kFar = -1e30f;
+constexpr float kFar = -1e28f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -93,12 +94,13 @@ __device__ __forceinline__ float ln_from_one(float x) {
 __device__ __forceinline__ RowResult finish(const SoftStats& a) {
   RowResult r;
   r.m = a.m;
-  r.poisoned = !(a.m <= FLT_MAX);
+  r.poisoned = !(a.m <= FLT_MAX) || a.s != a.s;  // (a sum that is no number is not passed off as one)
   r.empty = !r.poisoned && a.s == 0.f;
   r.log_s = r.empty ? 0.f : ln_from_one(fmaxf(a.s, 1.f));  // (the largest logit alone is 1, but for the rounding of rescalings)
   const float nan = __int_as_float(0x7fffffff);
   r.lse = r.poisoned ? nan : r.empty ? -INFINITY : a.m + r.log_s;
-  r.entropy = r.poisoned ? nan : r.empty ? 0.f : fmaxf(r.log_s - __fdiv_rn(a.t, a.s), 0.f);
+  r.entropy = r.poisoned ? nan : r.empty ? 0.f : r.log_s - __fdiv_rn(a.t, a.s);
+  if (r.entropy < 0.f) r.entropy = 0.f;  // (NaN stays)
   return r;
 }
 

@@ -148,9 +148,10 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 }
 
 // A step's 16 logits at the maximum that is in place.  2^((z - m) log2 e) as 2^(y - r) with y = z log2 e - M, M = fl(m log2 e)
-// and r = m log2 e - M, each one rounding of an exact product: r is the same for all and comes off the sums.  Needs products
-// that do not overflow.  One that does, of a masked token or a logit below -2.3e38, is a y of -inf, whose 0 * y makes t NaN: such
-// steps, and rows of a maximum beyond 1e38, go logit by logit.  (Looking for the smallest logit instead took half an instruction
+// and r = m log2 e - M, each one rounding of an exact product: r is the same for all and comes off the sums.  r is up to half a
+// step of M: 8 for |m| up to 1e8, but 128 and more, where 2^y and 2^-r overflow, from some 1.5e9 on.  A larger maximum, be it only that
+// of a thread whose first logits are all masked with a large finite number, goes logit by logit.  So does a step with a product that
+// overflows, of a logit below -2.3e38 or a masked token: a y of -inf, whose 0 * y makes t NaN.  (Looking for the smallest logit instead took half an instruction
 // per logit of the ten or so that bound this kernel; the sums two at a time save one and a half.)
 __device__ __forceinline__ void add_step(SoftStats& st, const float* v) {
   const float M = st.m * kLog2e, r = fmaf(st.m, kLog2e, -M);
@@ -166,7 +167,7 @@ __device__ __forceinline__ void add_step(SoftStats& st, const float* v) {
   }
   const float2 s = s2.both(), t = t2.both();
   const float sum = s.x + s.y, weighted = t.x + t.y;
-  if (fabsf(st.m) <= 1e38f && weighted == weighted) {
+  if (fabsf(st.m) <= 1e8f && weighted == weighted) {
     const float f = exp2f(-r);
     st.s = fmaf(f, sum, st.s);
     st.t = fmaf(f * 0.6931471805599453f, fmaf(-r, sum, weighted), st.t);

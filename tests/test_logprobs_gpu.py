@@ -76,6 +76,47 @@ def test_far_and_peaked_rows(ops, shift):
     run_and_check(ops, z + shift, torch.tensor([17, 5, 2999]).cuda(), 3, "far")
 
 
+def strict(ops, z, tokens, top, what):
+    """Log probabilities and entropy come from differences to the maximum, so its size adds nothing to what they may be off; lse is held to the
+    relative half steps of check_logprobs, which wants NaN where the reference has it and nowhere else.  (30: twice the span of the logits that count.)"""
+    got = ops.token_logprobs(z, tokens, top_k=top)
+    check_logprobs(got, ref_logprobs(z, tokens, top), softmax_tolerance(z.shape[1], 30.0), what)
+
+
+@pytest.mark.parametrize("rows,V", [(8, 100), (8, 5000), (8, 65536), (320, 9001)])
+@pytest.mark.parametrize("mask", [-1e7, -1e8, -1e9, -1e10, -1e20, -1e30, -1e37, -1e38, LOW])
+def test_finite_masks(ops, mask, rows, V):
+    """Tokens masked with a large finite number, as samplers and grammars do: most of a row, all of it, the beginning (where a thread sees nothing
+    else at first), all but the last, together with -inf; and logits that are themselves of that size."""
+    z = logits(rows, V, seed=3)
+    gen = torch.Generator().manual_seed(4)
+    z[0][(torch.rand(V, generator=gen) < 0.9).cuda()] = mask
+    z[1] = mask
+    z[2, :V // 2] = mask
+    z[3, :V - 1] = mask
+    z[4] = mask
+    z[4, ::3] = NEG
+    z[5, V // 3:] = mask
+    z[5, ::2] = NEG
+    z[6] = mask
+    z[6, 1::2] = mask * 0.5
+    if rows > 8:
+        z[8:][(torch.rand(rows - 8, V, generator=gen) < 0.9).cuda()] = mask
+    tokens = torch.randint(0, V, (rows, 2), generator=gen).cuda()
+    for top in (0, 1, 20):
+        strict(ops, z, tokens, top, f"mask {mask:g} V={V} top={top}")
+
+
+@pytest.mark.parametrize("shift", [1e8, -1e8, 1.6e9, -1.6e9, 1e10, -1e10, 1e20, -1e30, 1e38, -2e38])
+def test_logits_of_any_size(ops, shift):
+    """Rows whose logits are all large: few values a step of fp32 apart, sums of the equal ones.  (At -2e38 the last row holds infinities.)"""
+    z = logits(6, 20011, seed=6) + shift
+    z[5] = (torch.arange(20011) % 3).cuda() * abs(shift) * 1e-7 + shift
+    tokens = torch.randint(0, 20011, (6,), generator=torch.Generator().manual_seed(2)).cuda()
+    for top in (0, 5):
+        strict(ops, z, tokens, top, f"shift {shift:g} top={top}")
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_rows_that_start_anywhere(ops, half):
     """Slices: a column offset, a row stride of its own and values behind the rows that must not count."""
