@@ -45,6 +45,7 @@ bool gemv_tma_fits(int M, int K);  // gemv_tma.cu
 struct GemvBatch {
   int n_seg;
   GemvSeg seg[kMaxSeg];
+  int after;     // for the launch: the weights may have been written by the kernel before, so that this one begins after it
   int* timeout;  // the device's failure word (kernels.h): a bounded wait that runs out ORs kTimeoutGemv into it
 };
 

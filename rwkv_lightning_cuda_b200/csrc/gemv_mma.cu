@@ -577,7 +577,9 @@ int gemv_mma_launch(cudaStream_t stream, const GemvBatch& b, int M, const GemvMm
   }
   auto launch = [&](auto kernel) -> int {
     RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
-    RK_CUDA(launch_pdl(kernel, dim3(plan.grid), dim3(kWarps * 32), plan.smem_bytes, stream, maps, b, plan.n_slots, plan.x_pitch));
+    const dim3 grid(plan.grid), block(kWarps * 32);
+    RK_CUDA(b.after ? launch_after(kernel, grid, block, plan.smem_bytes, stream, maps, b, plan.n_slots, plan.x_pitch)
+                    : launch_pdl(kernel, grid, block, plan.smem_bytes, stream, maps, b, plan.n_slots, plan.x_pitch));
     return kOk;
   };
   int s;

@@ -333,7 +333,8 @@ int gemv_tma_launch(cudaStream_t stream, const GemvBatch& b, int M, size_t smem_
   const int x_bytes = static_cast<int>(smem_bytes - static_cast<size_t>(kWarps) * n_slots * slot_stride);
   auto launch = [&](auto kernel) -> int {
     RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
-    RK_CUDA(launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), smem_bytes, stream, b, x_bytes, n_slots, slot_stride));
+    RK_CUDA(b.after ? launch_after(kernel, dim3(grid), dim3(kWarps * 32), smem_bytes, stream, b, x_bytes, n_slots, slot_stride)
+                    : launch_pdl(kernel, dim3(grid), dim3(kWarps * 32), smem_bytes, stream, b, x_bytes, n_slots, slot_stride));
     return kOk;
   };
   bool quant = false;

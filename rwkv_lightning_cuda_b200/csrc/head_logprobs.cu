@@ -255,6 +255,7 @@ int logits_then_stats(cudaStream_t stream, const HeadLogprobsArgs& a, float* log
   } else {
     LinearArgs l;
     l.M = a.rows; l.K = a.K; l.N = a.V; l.x = a.x; l.w = a.w; l.fmt = a.fmt; l.epi = kEpiRawF32; l.y = logits;
+    l.after = !a.resident;  // (a caller may have made the weights just before)
     s = linear(stream, l);
   }
   if (s != kOk) return s;

@@ -132,6 +132,7 @@ struct HeadLogprobsArgs {
   float* logprobs = nullptr;        // [rows]
   float* entropy = nullptr;         // [rows], optional
   float* lse = nullptr;             // [rows], optional
+  bool resident = false;            // the weights are not written by the kernel launched just before
   float4* part = nullptr;           // set by head_logprobs: (m, s, t) of a tile's part of a row, [tiles, rows]
   float* given = nullptr;           // set by head_logprobs: the given token's logit, [rows]
 };
@@ -168,6 +169,9 @@ struct LinearArgs {
   // tensor-core path: true when w may have been written by the kernel launched just before this call on the same
   // stream (then its tiles are not requested until that kernel has completed); a model's resident weights set false
   bool w_dynamic = true;
+  // the kernels of up to 4 rows, which ask for weights before their predecessor has ended: true where w may be what the kernel
+  // launched just before writes
+  bool after = false;
   // 2..4 rows normally take the GEMV kernels (whose time grows with the row count); set this to send a large fp16
   // product of 2..4 rows to the tensor-core kernel instead, which streams the weights once whatever the row count
   bool prefer_tc = false;

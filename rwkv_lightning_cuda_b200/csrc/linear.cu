@@ -228,6 +228,8 @@ int linear_batch(cudaStream_t stream, const LinearArgs* args, int n) {
     max_fmt = std::max(max_fmt, a.fmt);
   }
   for (int i = n; i < kMaxSeg; ++i) b.seg[i] = b.seg[0];
+  b.after = 0;
+  for (int i = 0; i < n; ++i) b.after |= args[i].after ? 1 : 0;
   b.timeout = timeout_word_or_null();
 
   // The kernel built on the warp-level tensor-core instruction (gemv_mma.cu) takes, by default (option gemv_mma = 3):
@@ -277,7 +279,7 @@ int linear_batch(cudaStream_t stream, const LinearArgs* args, int n) {
   const dim3 grid(cta), block(kWarps * 32);
   auto launch = [&](auto kernel) -> int {
     if (smem > 48 * 1024) RK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
-    RK_CUDA(launch_pdl(kernel, grid, block, smem, stream, b));
+    RK_CUDA(b.after ? launch_after(kernel, grid, block, smem, stream, b) : launch_pdl(kernel, grid, block, smem, stream, b));
     return kOk;
   };
   auto by_m = [&](auto fmt_tag) -> int {

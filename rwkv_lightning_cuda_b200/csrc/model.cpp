@@ -842,7 +842,7 @@ int Model::enqueue(Workspace& ws, int B, int T, half* shift, void* wkv, int* ela
     HeadLogprobsArgs h;
     h.rows = rows; h.K = C; h.V = cfg_.vocab; h.x = ws.n1; h.w = head_.w.p; h.fmt = head_.fmt; h.group = 128;
     h.scale = head_.scale.as<half>(); h.zero = head_.zero.as<half>(); h.tokens = score->targets;
-    h.logprobs = score->logprobs; h.entropy = score->entropy;
+    h.logprobs = score->logprobs; h.entropy = score->entropy; h.resident = true;
     const size_t at = (static_cast<size_t>(rows) * sizeof(int64_t) + 15) & ~static_cast<size_t>(15);  // behind the given tokens
     RK_TRY(head_logprobs(st, h, score_.as<char>() + at, score_.bytes - at));
     if (!logits) return kOk;

@@ -283,3 +283,25 @@ def test_head_equals_product_then_logprobs(ops):
     biggest = float(z.abs().max())
     assert float((one[0] - two[0]).abs().max()) <= 2 * biggest * 2 ** -11 + 1e-4  # both the given logit and the sum move by a half step of fp16
     assert float((one[2] - two[2]).abs().max()) <= biggest * 2 ** -11 + 1e-4
+
+
+def test_head_weights_made_just_before(ops):
+    """One row on a large fp16 matrix that the kernel before it on the stream writes, itself one that lets its successor begin early: the answer is that
+    of the finished weights, every time."""
+    gen = torch.Generator().manual_seed(21)
+    V, K = 65536, 1024
+    q, s, _ = random_w4(K, 32, 32, True, gen)
+    made = [torch.randn(V, 32, generator=gen).half().cuda() for _ in range(2)]
+    x, tok = torch.randn(1, K, generator=gen).half().cuda(), torch.tensor([V - 1]).cuda()
+    first = []
+    for m in made:
+        w = ops.linear_w4a16_group(m, q, s, None, 32)
+        torch.cuda.synchronize()
+        first.append(ops.head_logprobs(x, w, tok))
+        del w
+    for i in range(12):
+        w = ops.linear_w4a16_group(made[i % 2], q, s, None, 32)
+        got = ops.head_logprobs(x, w, tok)
+        for a, b in zip(got, first[i % 2]):
+            assert torch.equal(a, b)
+        del w, got
