@@ -153,10 +153,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
   };
   int q_tile = 0, q_kb = team_warp - team_warps, q_slot = 0;
   advance(q_tile, q_kb);
-  auto issue = [&]() {
+  // used: 0, computed from what the slot's last contents went into, so that they have been read when the copy is issued.
+  auto issue = [&](uint32_t used) {
     if (lane == 0) {
       const uint32_t bar = smem_u32(&bars[warp][q_slot]);
-      const uint32_t dst = ring + q_slot * p.slot_bytes;
+      const uint32_t dst = ring + q_slot * p.slot_bytes + used;
       const int n = row0 + q_tile * row_step;
       mbar_expect_tx(bar, p.h * (128 + (kCopied ? (a.zero ? 32 : 16) : 0)));
       tma_2d(dst, &maps.q, bar, q_kb << 7, n);
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
     if (++q_slot == p.slots) q_slot = 0;
     advance(q_tile, q_kb);
   };
-  for (int i = 0; i < p.slots && q_tile < tiles; ++i) issue();
+  for (int i = 0; i < p.slots && q_tile < tiles; ++i) issue(0u);
 
   // A lane's share of a box's scales and zeros, for the rows g, g + 8, g + 16, g + 24: groups of 32: the pair 2t, 2t + 1 of the
   // box's eight; of 64: group t of four; of 128: group t / 2 of two.
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
   for (int b = 0; b < kBlk; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[b][i] = 0.f;
-  const uint32_t one = 0x64006400u + (base >> 30);  // (a shared-memory address is below 2^30, which the compiler does not know)
+  const uint32_t none = base >> 30, one = 0x64006400u + none;  // (a shared-memory address is below 2^30, which the compiler does not know)
   int cur = 0, slot = 0, phase = 0;
   bool dead = false;  // a wait ran out: no more work, but the barriers are kept
   for (;;) {
@@ -414,8 +415,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
         }
       }
     }
-    __syncwarp();  // every lane has read the slot: it may be overwritten
-    if (!dead && q_tile < tiles) issue();
+    // Every lane has read the slot: it may be overwritten.  The barrier alone orders the loads' issue, not their results, and the
+    // products that take those might be placed behind the copy; its address waits for the sums that they and the scales went into (a
+    // product takes all lanes' operands, so lane 0's sums stand for the warp's).
+    __syncwarp();
+    if (!dead && q_tile < tiles) {
+      uint32_t used = 0;
+#pragma unroll
+      for (int b = 0; b < kBlk; ++b) used |= __float_as_uint(acc[b][0]) | __float_as_uint(acc[b][2]);
+      issue(used & none);
+    }
     if (++slot == p.slots) { slot = 0; phase ^= 1; }
   }
 }

@@ -212,6 +212,21 @@ def test_long_products_again_and_again(ops, M, N, K):
         assert torch.equal(ops.linear_w4a16_group(x, q, s, z, 32), first)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 8192), (1, 20000, 2080), (2, 5000, 4096), (3, 2561, 6176), (5, 9000, 3136), (8, 4000, 8192)])
+def test_streamed_products_again_and_again(ops, M, N, K, group):
+    """Few rows, whose rings are refilled behind the products: the right answer, and the same one every time; the head's form of them too."""
+    gen = torch.Generator().manual_seed(K + M)
+    q, s, z = random_w4(N, K, group, False, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    tok = torch.randint(0, N, (M,), generator=gen).cuda()
+    first, scores = ops.linear_w4a16_group(x, q, s, z, group), ops.head_logprobs(x, q, tok, scale=s, zero=z, group_size=group)
+    check_product(first, x, (q, s, z), group, "first")
+    got = [(ops.linear_w4a16_group(x, q, s, z, group), ops.head_logprobs(x, q, tok, scale=s, zero=z, group_size=group)) for _ in range(40)]
+    for y, l in got:
+        assert torch.equal(y, first) and all(torch.equal(u, v) for u, v in zip(l, scores))
+
+
 def test_codes_one_at_a_time(ops):
     """Each of the 16 codes at each place of a word, and each group's own scale: one weight at a time against one activation."""
     K, group = 288, 32
