@@ -211,7 +211,7 @@ int rwkv7_b200_token_logprobs(void* stream, int rows, int V, const void* logits,
 /* The same answers for x W^T without writing the logits: one given token per row (tokens and logprobs may both be NULL),
  * x [rows][K] half, weight [V][K] in `format` (RWKV7_B200_FMT_*; W8A16: scale [V]; W4A16: scale and zero
  * [V][ceil(K / group)], group 32, 64 or 128, zero NULL: 8).  Logits are fp32 sums, not rounded to half as forward's are;
- * 4-bit weights count as half((q - zero) * scale), zeros being whole numbers.  K % 32 == 0; x, weight and workspace 16-byte aligned.  workspace is
+ * 4-bit weights count as half((q - zero) * scale), as in rwkv7_b200_linear_w4a16_group with many rows.  K % 32 == 0; x, weight and workspace 16-byte aligned.  workspace is
  * scratch of the size the first function returns; calls that may overlap on the GPU need one each. */
 int rwkv7_b200_head_logprobs_workspace(int rows, int V, size_t* bytes);
 int rwkv7_b200_head_logprobs(void* stream, int rows, int K, int V, const uint16_t* x, const void* weight, int format,
@@ -390,9 +390,10 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
  * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 8 rows
  * the scale multiplies the group's fp32 sum, so no weight is rounded.  With more rows weights count as
  * half((q - zero) * scale); with RWKV7_B200_EPI_EXACT or-ed to the epilogue none is rounded there either, at twice the
- * products (a weight is the sum of two halves then, so it has to be below 65504).  With more than 8 rows zeros have to be
- * whole numbers.  workspace is scratch of the size the first function returns (which may be 0); without it, or with less,
- * products of many rows run on fewer SMs.  Calls that may overlap on the GPU need one each. */
+ * products (a weight is the sum of two halves then, so it has to be below 65504).  Zeros need not be whole numbers; with
+ * more than 8 rows other ones (from -32 on) put a weight off by 2^-17 of its scale (EXACT: 2^-15) at most.  workspace is
+ * scratch of the size the first function returns (which may be 0); without it, or with less, products of many rows run on
+ * fewer SMs.  Calls that may overlap on the GPU need one each. */
 int rwkv7_b200_linear_w4a16_group_workspace(int M, int K, int N, size_t* bytes);
 int rwkv7_b200_linear_w4a16_group(void* stream, int M, int K, int N, const uint16_t* x, const uint8_t* q,
                                   const uint16_t* scale, const uint16_t* zero, int group, int epilogue, void* y,

@@ -70,13 +70,21 @@ __device__ __forceinline__ PackedUnit unit_of(const PackedShape& h, int u, int k
   return r;
 }
 
-// Eight 4-bit codes to eight halves half((q - zero) * scale): a nibble under the exponent of 1024 is 1024 + q (the high ones
-// arrive as 1024 + 16 q), so one subtraction or fused multiply-add leaves q - zero exactly and the product rounds once.
+// Eight 4-bit codes to eight halves half((q - zero) * scale): a nibble in the middle of a byte under the exponent of 1024 is 1024 + 16 q, so
+// that a sixteenth of it less 64 + zero, in one fused multiply-add, is q - zero, and a second one multiplies and rounds.  64 + zero is
+// itself rounded, to sixteenths for zeros up to 64; what that leaves over, times the scale, is the second one's addend: nothing for whole
+// zeros, and otherwise at most a 32nd of the scale, whose own rounding puts a weight off by 2^-17 of the scale.  (q - zero so rounded
+// is a half exactly for zeros from -32 on.)
 struct Group4 {
-  __half2 scale, sub;  // (s, s) and (-(1024 + z), -(64 + z))
+  __half2 scale, sub, rest;  // twice each: s, -(64 + z) rounded, -(what z has beyond that) s
 };
+__device__ __forceinline__ __half2 zero_sub(__half2 z) { return __hsub2(__floats2half2_rn(-64.f, -64.f), z); }
+__device__ __forceinline__ __half2 zero_rest(__half2 z, __half2 sub, __half2 scale) {
+  return __hmul2(__hsub2(__hsub2(__floats2half2_rn(-64.f, -64.f), sub), z), scale);
+}
 __device__ __forceinline__ Group4 group4(uint32_t s2, uint32_t z2) {  // the group's scale and zero, twice each
-  return {*reinterpret_cast<const __half2*>(&s2), __hsub2(__floats2half2_rn(-1024.f, -64.f), *reinterpret_cast<const __half2*>(&z2))};
+  const __half2 s = *reinterpret_cast<const __half2*>(&s2), z = *reinterpret_cast<const __half2*>(&z2), sub = zero_sub(z);
+  return {s, sub, zero_rest(z, sub, s)};
 }
 // Half i of eight, twice.
 __device__ __forceinline__ uint32_t pick(const uint4& v, int i) {
@@ -85,31 +93,32 @@ __device__ __forceinline__ uint32_t pick(const uint4& v, int i) {
 }
 // The constants are the caller's registers: as literals, mask and bias of the AND-OR would not fit into one instruction.
 struct Expand4 {
-  uint32_t nibbles, bias;  // 0x00f0000f, 0x64006400
-  __half2 mul;             // 1, 1/16
+  uint32_t nibbles, bias;  // 0x00f000f0, 0x64006400
+  __half2 mul;             // 1/16 twice
+  // Byte b's codes as 1024 + 16 q; up: the word shifted up by a nibble.
+  __device__ __forceinline__ __half2 pair(uint32_t up, uint32_t w, int b) const {
+    const uint32_t both = __byte_perm(up, w, 0x4400u + 0x1111u * b);
+    uint32_t p;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(p) : "r"(both), "r"(nibbles), "r"(bias));
+    return *reinterpret_cast<const __half2*>(&p);
+  }
 };
 __device__ __forceinline__ uint4 expand4(uint32_t w, const Group4& g, const Expand4& e) {
   uint32_t h[4];
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const uint32_t both = __byte_perm(w, 0u, 0x4040u + 0x0101u * b);  // the byte in both halves
-    uint32_t pair;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(pair) : "r"(both), "r"(e.nibbles), "r"(e.bias));
-    const __half2 v = __hmul2(__hfma2(*reinterpret_cast<__half2*>(&pair), e.mul, g.sub), g.scale);
+    const __half2 v = __hfma2(__hfma2(e.pair(w << 4, w, b), e.mul, g.sub), g.scale, g.rest);
     h[b] = *reinterpret_cast<const uint32_t*>(&v);
   }
   return make_uint4(h[0], h[1], h[2], h[3]);
 }
-// The same and what the rounding took off.  (q - zero) * scale is a whole number of at most four bits times the scale, so it is a
-// multiple of the scale's last place, and so is what it is off its rounding: a half, which the fused multiply-add gives exactly.
+// The same and what the rounding took off.  With a whole zero (q - zero) * scale is a multiple of the scale's last place, and so is what it is
+// off its rounding: a half, which the fused multiply-add gives exactly.  With others the low half is off by up to 2^-17 of the scale more.
 __device__ __forceinline__ void expand4(uint32_t w, const Group4& g, const Expand4& e, uint4* high, uint4* low) {
   uint32_t h[4], l[4];
 #pragma unroll
   for (int b = 0; b < 4; ++b) {
-    const uint32_t both = __byte_perm(w, 0u, 0x4040u + 0x0101u * b);
-    uint32_t pair;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(pair) : "r"(both), "r"(e.nibbles), "r"(e.bias));
-    const __half2 d = __hfma2(*reinterpret_cast<__half2*>(&pair), e.mul, g.sub), v = __hmul2(d, g.scale), o = __hfma2(d, g.scale, __hneg2(v));
+    const __half2 d = __hfma2(e.pair(w << 4, w, b), e.mul, g.sub), v = __hmul2(d, g.scale), o = __hadd2(__hfma2(d, g.scale, __hneg2(v)), g.rest);
     h[b] = *reinterpret_cast<const uint32_t*>(&v);
     l[b] = *reinterpret_cast<const uint32_t*>(&o);
   }
@@ -343,8 +352,8 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
     };
     auto eight_of = [&](int kb) { return (kb * kStage) >> (shift + 3); };
     const uint32_t none = ring >> 30;  // 0, which the compiler does not know, so that the constants stay in registers
-    const uint32_t mul = 0x2c003c00u + none;
-    const Expand4 e4 = {0x00f0000fu + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
+    const uint32_t mul = 0x2c002c00u + none;
+    const Expand4 e4 = {0x00f000f0u + none, 0x64006400u + none, *reinterpret_cast<const __half2*>(&mul)};
     // A stage is handed over when this warp has the next one's weights in registers: the stores end under those loads.  (A packed tile
     // waits for nothing later than the stage four before it, and a place for the one T before, so no wait closes a circle.)
     int stored = -1;
@@ -407,7 +416,7 @@ __global__ void __launch_bounds__(kPackedThreads, 1)
                 const int i = eights ? (k >> shift) & 7 : run;
                 g = group4(pick(sc, i), pick(ze, i));
               }
-              if (run > 0 && k >= a.K) g.scale = __floats2half2_rn(0.f, 0.f);  // behind K: code 0, which may stand for an infinite weight
+              if (run > 0 && k >= a.K) g.scale = g.rest = __floats2half2_rn(0.f, 0.f);  // behind K: code 0, which may stand for an infinite weight
               const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
               for (int j = 0; j < 4; ++j) {

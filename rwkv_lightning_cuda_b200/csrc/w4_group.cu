@@ -22,6 +22,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -79,7 +80,7 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uin
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 // The eight weights of a word as pairs (0, 4), (1, 5), (2, 6), (3, 7): a nibble under the exponent of 1024 is 1024 + q, a high one
-// 1024 + 16 q; less 1024 + zero (or / 16 less 64 + zero) that is q - zero exactly, and the product rounds once.  one: 0x64006400 in a
+// 1024 + 16 q; less 1024 + zero (or / 16 less 64 + zero) that is q - zero, exactly where zero is whole, and the product rounds once.  one: 0x64006400 in a
 // register of the caller's (as a literal beside the mask it would take an instruction of its own).
 template <uint32_t kMask> __device__ __forceinline__ __half2 under_1024(uint32_t u, uint32_t one) {
   uint32_t v;
@@ -93,6 +94,19 @@ __device__ __forceinline__ void round4(uint32_t u, uint32_t one, __half2 s, __ha
   o[1] = h2u(__hmul2(__hfma2(under_1024<0x00f000f0u>(u, one), sixteenth, zhi), s));
   o[2] = h2u(__hmul2(__hsub2(under_1024<0x000f000fu>(v, one), zlo), s));
   o[3] = h2u(__hmul2(__hfma2(under_1024<0x00f000f0u>(v, one), sixteenth, zhi), s));
+}
+// 0 where both of two zeros are whole numbers up to 1024, which 1024 + zero and 64 + zero hold exactly.
+__device__ __forceinline__ uint32_t not_whole(uint32_t z2) {
+  const uint32_t size = z2 & 0x7fff7fffu;
+  const __half2 big = __floats2half2_rn(1024.f, 1024.f);
+  return h2u(__hsub2(__hadd2(u2h(size), big), big)) ^ size;
+}
+// round4 for any zeros: the product in fp32, rounded from there.
+__device__ __forceinline__ void round4_any(uint32_t u, float s, float z, uint32_t (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = h2u(__floats2half2_rn(__fmul_rn(__fsub_rn(static_cast<float>(u >> (4 * i) & 15), z), s),
+                                 __fmul_rn(__fsub_rn(static_cast<float>(u >> (4 * i + 16) & 15), z), s)));
 }
 __device__ __forceinline__ float half_of(uint32_t pair, int i) {
   const float2 f = h2f2(pair);
@@ -329,91 +343,110 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
       const uint32_t x_now = x_row + (kb << 9);
       float lo[kBlk][4], hi[kBlk][4];
       __half2 scale2[2 * kBlk], zero_lo[2 * kBlk], zero_hi[2 * kBlk];  // kRounded
+      auto work = [&](auto any) {
+        // kRounded: whatever the zeros are (zero_lo then holds them as they are); in a loop, so that it leaves the other form its registers
+        constexpr bool kAny = decltype(any)::value;
+        constexpr int kUnroll = kAny ? 1 : 4;
+#pragma unroll kUnroll
+        for (int c2 = 0; c2 < 4; ++c2) {
+          // Two chunks of 16 rows: the matrices are (rows 0-7, rows 8-15) x (chunk 2 c2, chunk 2 c2 + 1), 16 bytes a row, and a lane gets
+          // the word t of row g.  The 128-byte swizzle puts chunk c of row r at c ^ (r mod 8).
+          uint32_t w[kBlk][4];
 #pragma unroll
-      for (int c2 = 0; c2 < 4; ++c2) {
-        // Two chunks of 16 rows: the matrices are (rows 0-7, rows 8-15) x (chunk 2 c2, chunk 2 c2 + 1), 16 bytes a row, and a lane gets
-        // the word t of row g.  The 128-byte swizzle puts chunk c of row r at c ^ (r mod 8).
-        uint32_t w[kBlk][4];
+          for (int b = 0; b < kBlk; ++b) ldmatrix4(w[b], wbase + b * 2048 + (w_lane ^ (c2 << 5)));
 #pragma unroll
-        for (int b = 0; b < kBlk; ++b) ldmatrix4(w[b], wbase + b * 2048 + (w_lane ^ (c2 << 5)));
+          for (int cc = 0; cc < 2; ++cc) {
+            const int c = 2 * c2 + cc;
+            uint4 xv;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
+                         : "r"((kSlots == 1 || slot_of_lane == c % kSlots ? x_now : zero_now) + (c << 6)));
+            if (kRounded) {
+              if (c % kGroupChunks == 0) {  // a new group: its parameters for the rows g and g + 8 of each block
+                const int from = kShift == 7 ? (c >> 2) << 1 : c >> 1;
 #pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-          const int c = 2 * c2 + cc;
-          uint4 xv;
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(xv.x), "=r"(xv.y), "=r"(xv.z), "=r"(xv.w)
-                       : "r"((kSlots == 1 || slot_of_lane == c % kSlots ? x_now : zero_now) + (c << 6)));
-          if (kRounded) {
-            if (c % kGroupChunks == 0) {  // a new group: its parameters for the rows g and g + 8 of each block
-              const int from = kShift == 7 ? (c >> 2) << 1 : c >> 1;
-#pragma unroll
-              for (int i = 0; i < 2 * kBlk; ++i) {
-                const uint32_t sp = __shfl_sync(0xffffffffu, s_now[i], (lane & ~3) | from), zp = __shfl_sync(0xffffffffu, z_now[i], (lane & ~3) | from);
-                const uint32_t sel = kShift == 5 && (c & 1) ? 0x3232 : 0x1010;
-                const uint32_t s2 = __byte_perm(sp, 0u, sel), z2 = __byte_perm(zp, 0u, sel);
-                scale2[i] = u2h(s2);
-                zero_lo[i] = __hadd2(u2h(z2), __floats2half2_rn(1024.f, 1024.f));
-                zero_hi[i] = __hfma2(u2h(z2), __floats2half2_rn(-1.f, -1.f), __floats2half2_rn(-64.f, -64.f));
+                for (int i = 0; i < 2 * kBlk; ++i) {
+                  const uint32_t sp = __shfl_sync(0xffffffffu, s_now[i], (lane & ~3) | from), zp = __shfl_sync(0xffffffffu, z_now[i], (lane & ~3) | from);
+                  const uint32_t sel = kShift == 5 && (c & 1) ? 0x3232 : 0x1010;
+                  scale2[i] = u2h(__byte_perm(sp, 0u, sel));
+                  const __half2 z2 = u2h(__byte_perm(zp, 0u, sel));
+                  zero_lo[i] = kAny ? z2 : __hadd2(z2, __floats2half2_rn(1024.f, 1024.f));
+                  zero_hi[i] = __hfma2(z2, __floats2half2_rn(-1.f, -1.f), __floats2half2_rn(-64.f, -64.f));
+                }
               }
-            }
-            if ((kb << 8) + 32 * c >= a.K) {  // behind K: code 0, which may stand for an infinite weight
+              if ((kb << 8) + 32 * c >= a.K) {  // behind K: code 0, which may stand for an infinite weight
 #pragma unroll
-              for (int i = 0; i < 2 * kBlk; ++i) scale2[i] = __floats2half2_rn(0.f, 0.f);
+                for (int i = 0; i < 2 * kBlk; ++i) scale2[i] = __floats2half2_rn(0.f, 0.f);
+              }
+#pragma unroll
+              for (int b = 0; b < kBlk; ++b) {
+                uint32_t ra[4], rb[4];
+                if (!kAny) {
+                  round4(w[b][2 * cc], one, scale2[2 * b], zero_lo[2 * b], zero_hi[2 * b], ra);
+                  round4(w[b][2 * cc + 1], one, scale2[2 * b + 1], zero_lo[2 * b + 1], zero_hi[2 * b + 1], rb);
+                } else {
+                  round4_any(w[b][2 * cc], __low2float(scale2[2 * b]), __low2float(zero_lo[2 * b]), ra);
+                  round4_any(w[b][2 * cc + 1], __low2float(scale2[2 * b + 1]), __low2float(zero_lo[2 * b + 1]), rb);
+                }
+                mma16816(lo[b], ra[0], rb[0], ra[2], rb[2], xv.x, xv.y, c == 0);
+                mma16816(hi[b], ra[1], rb[1], ra[3], rb[3], xv.z, xv.w, c == 0);
+                if (c == 7) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[b][i] += lo[b][i] + hi[b][i];
+                }
+              }
+              continue;
             }
+            const bool first = c % kPass == 0;
 #pragma unroll
             for (int b = 0; b < kBlk; ++b) {
-              uint32_t ra[4], rb[4];
-              round4(w[b][2 * cc], one, scale2[2 * b], zero_lo[2 * b], zero_hi[2 * b], ra);
-              round4(w[b][2 * cc + 1], one, scale2[2 * b + 1], zero_lo[2 * b + 1], zero_hi[2 * b + 1], rb);
-              mma16816(lo[b], ra[0], rb[0], ra[2], rb[2], xv.x, xv.y, c == 0);
-              mma16816(hi[b], ra[1], rb[1], ra[3], rb[3], xv.z, xv.w, c == 0);
-              if (c == 7) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[b][i] += lo[b][i] + hi[b][i];
-              }
+              const uint32_t wa = w[b][2 * cc], wb = w[b][2 * cc + 1], va = wa >> 8, vb = wb >> 8;
+              mma16816(lo[b], wa & 0x000f000fu, wb & 0x000f000fu, va & 0x000f000fu, vb & 0x000f000fu, xv.x, xv.y, first);
+              mma16816(hi[b], wa & 0x00f000f0u, wb & 0x00f000f0u, va & 0x00f000f0u, vb & 0x00f000f0u, xv.z, xv.w, first);
             }
-            continue;
-          }
-          const bool first = c % kPass == 0;
+            if ((c + 1) % kPass != 0) continue;
+            // the end of a pass: scales and zeros of the groups that this lane's two columns hold
+            const int pass = c / kPass;
+            const float2 xs = *reinterpret_cast<const float2*>(sums + (kb * kPasses + pass) * 8 + 2 * t);
+            // the chunk of the column 2t, and where its group's parameters are: (lane of the quad, half of the pair)
+            const int chunk = kM == 1 ? 2 * t : pass * kPass + (kM == 8 ? 0 : 2 * t / kM);
+            const int from = kShift == 5 ? chunk >> 1 : kShift == 6 ? chunk >> 1 : (chunk >> 2) << 1;
 #pragma unroll
-          for (int b = 0; b < kBlk; ++b) {
-            const uint32_t wa = w[b][2 * cc], wb = w[b][2 * cc + 1], va = wa >> 8, vb = wb >> 8;
-            mma16816(lo[b], wa & 0x000f000fu, wb & 0x000f000fu, va & 0x000f000fu, vb & 0x000f000fu, xv.x, xv.y, first);
-            mma16816(hi[b], wa & 0x00f000f0u, wb & 0x00f000f0u, va & 0x00f000f0u, vb & 0x00f000f0u, xv.z, xv.w, first);
-          }
-          if ((c + 1) % kPass != 0) continue;
-          // the end of a pass: scales and zeros of the groups that this lane's two columns hold
-          const int pass = c / kPass;
-          const float2 xs = *reinterpret_cast<const float2*>(sums + (kb * kPasses + pass) * 8 + 2 * t);
-          // the chunk of the column 2t, and where its group's parameters are: (lane of the quad, half of the pair)
-          const int chunk = kM == 1 ? 2 * t : pass * kPass + (kM == 8 ? 0 : 2 * t / kM);
-          const int from = kShift == 5 ? chunk >> 1 : kShift == 6 ? chunk >> 1 : (chunk >> 2) << 1;
+            for (int b = 0; b < kBlk; ++b) {
+              float s0[2], s1[2], z0[2], z1[2];  // rows g and g + 8: of the lane's first and second column
 #pragma unroll
-          for (int b = 0; b < kBlk; ++b) {
-            float s0[2], s1[2], z0[2], z1[2];  // rows g and g + 8: of the lane's first and second column
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t sp = s_now[2 * b + i], zp = z_now[2 * b + i];
-              if (kM > 1) {
-                sp = __shfl_sync(0xffffffffu, sp, (lane & ~3) | from);
-                zp = __shfl_sync(0xffffffffu, zp, (lane & ~3) | from);
+              for (int i = 0; i < 2; ++i) {
+                uint32_t sp = s_now[2 * b + i], zp = z_now[2 * b + i];
+                if (kM > 1) {
+                  sp = __shfl_sync(0xffffffffu, sp, (lane & ~3) | from);
+                  zp = __shfl_sync(0xffffffffu, zp, (lane & ~3) | from);
+                }
+                if (kM == 1 && kShift == 5) {
+                  s0[i] = half_of(sp, 0); s1[i] = half_of(sp, 1);
+                  z0[i] = half_of(zp, 0); z1[i] = half_of(zp, 1);
+                } else {
+                  const int odd = kShift == 5 ? chunk & 1 : 0;
+                  s0[i] = s1[i] = half_of(sp, odd);
+                  z0[i] = z1[i] = half_of(zp, odd);
+                }
               }
-              if (kM == 1 && kShift == 5) {
-                s0[i] = half_of(sp, 0); s1[i] = half_of(sp, 1);
-                z0[i] = half_of(zp, 0); z1[i] = half_of(zp, 1);
-              } else {
-                const int odd = kShift == 5 ? chunk & 1 : 0;
-                s0[i] = s1[i] = half_of(sp, odd);
-                z0[i] = z1[i] = half_of(zp, odd);
-              }
-            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float u = fmaf(hi[b][i], 0.0625f, lo[b][i]);
-              acc[b][i] = fmaf(i & 1 ? s1[i >> 1] : s0[i >> 1], fmaf(i & 1 ? z1[i >> 1] : z0[i >> 1], i & 1 ? xs.y : xs.x, u), acc[b][i]);
+              for (int i = 0; i < 4; ++i) {
+                const float u = fmaf(hi[b][i], 0.0625f, lo[b][i]);
+                acc[b][i] = fmaf(i & 1 ? s1[i >> 1] : s0[i >> 1], fmaf(i & 1 ? z1[i >> 1] : z0[i >> 1], i & 1 ? xs.y : xs.x, u), acc[b][i]);
+              }
             }
           }
         }
+      };
+      bool whole = true;  // the zeros of the box's groups are whole numbers (those of the tile's rows, behind which none have come)
+      if (kRounded && a.zero) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * kBlk; ++i) odd |= g + 8 * i < p.h ? not_whole(z_now[i]) : 0u;
+        whole = __all_sync(0xffffffffu, odd == 0);
       }
+      if (!kRounded || whole) work(std::false_type());
+      else work(std::true_type());
     }
     // Every lane has read the slot: it may be overwritten.  The barrier alone orders the loads' issue, not their results, and the
     // products that take those might be placed behind the copy; its address waits for the sums that they and the scales went into (a
@@ -598,8 +631,8 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
 }
 
 // ---- more rows: the tensor-core skeleton of tc_packed.cuh, weights rounded to half, or as two halves each where the caller wants none
-// rounded: an instruction more per two weights, twice the stores and products, and stages of 64 (96 rows of 10240 x 2560 19.2 us, 14.0 rounded;
-// 24 of 65536 x 4096 81 and 59; 256 of 16384 x 4096 48 and 30; nine of 10240 x 2560 16.2 and 13.8).
+// rounded: two instructions more per two weights, twice the stores and products, and stages of 64 (96 rows of 10240 x 2560 20.2 us, 14.0 rounded;
+// 24 of 65536 x 4096 87 and 59; 256 of 16384 x 4096 49 and 30; nine of 10240 x 2560 16.5 and 13.8).
 namespace {
 
 __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }

@@ -335,7 +335,7 @@ def _refuse_head_logprobs(x, weight, tokens, scale, zero, group_size):
 def head_logprobs(x, weight, tokens=None, scale=None, zero=None, group_size=128):
     """``token_logprobs`` of x W^T (x fp16 [rows, K]) without writing the logits: one given token per row (int64 [rows] or
     None).  ``weight`` is fp16 [V, K], int8 [V, K] with ``scale`` fp16 [V], or uint8 [V, K/2] (two 4-bit codes a byte) with
-    ``scale`` and ``zero`` (None: 8) fp16 [V, ceil(K / group_size)].  Returns (logprobs, entropy, lse), fp32 [rows]."""
+    ``scale`` and ``zero`` (None: 8) fp16 [V, ceil(K / group_size)], a weight counting as half((q - zero) * scale).  Returns (logprobs, entropy, lse), fp32 [rows]."""
     ok = isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor) and x.dim() == 2 and weight.dim() == 2 and x.is_cuda
     if ok:
         (rows, K), V, dev, fmt = x.shape, weight.shape[0], x.device, _HEAD_FORMATS.get(weight.dtype, -1)
@@ -373,7 +373,8 @@ def linear_w4a16_group(x, q, scale, zero=None, group_size=128, epilogue=L.EPI_NO
     """x W^T for 4-bit weights with group scales: W = (q - zero) * scale per group of 32, 64 or 128 inputs; x fp16 [M, K], q
     uint8 [N, K/2], scale and zero (None: 8) fp16 [N, ceil(K / group_size)]; K a multiple of 32, any M and N.  Up to 8
     rows no weight is rounded; with more a weight counts as half((q - zero) * scale), unless ``exact`` asks for weights that are not
-    rounded there either (at twice the products).  With more than 8 rows zeros have to be whole numbers."""
+    rounded there either (at twice the products).  Zeros need not be whole numbers; with more than 8
+    rows other ones (from -32 on) put a weight off by 2^-17 of its scale (``exact``: 2^-15) at most."""
     ok = isinstance(x, torch.Tensor) and isinstance(q, torch.Tensor) and x.dim() == 2 and q.dim() == 2 and x.is_cuda
     if ok:
         (M, K), N, dev = x.shape, q.shape[0], x.device

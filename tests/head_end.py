@@ -1,4 +1,5 @@
 """References in 64 bits, and derived tolerances, for the log-probability and group-scaled 4-bit operators."""
+import numpy as np
 import torch
 
 U32 = 2.0 ** -24  # half a step of fp32
@@ -88,6 +89,19 @@ def w4_weights(q, scale, zero, group, rounded=False, parts=False):
     z = 8.0 if zero is None else zero.cpu().double()[:, g]
     w = (w + z if parts else w - z) * scale[:, g]
     return w.half().double() if rounded else w
+
+
+def w4_rounded_any_zero(q, scale, zero, group):
+    """The halves that weights count as on the tensor cores when zeros need not be whole numbers: with e the zero as 64 + zero rounded to half
+    holds it, half((q - e) scale + half((e - zero) scale)).  Equal to half((q - zero) scale) for whole zeros up to 1024."""
+    q, s, z = q.cpu(), scale.cpu().double(), zero.cpu().double()
+    N, K = q.shape[0], q.shape[1] * 2
+    codes = torch.stack((q & 15, q >> 4), dim=2).reshape(N, K).double()
+    held = (64 + z).half().double() - 64
+    rest = ((held - z) * s).half().double()
+    g = torch.arange(K) // group
+    w = (codes - held[:, g]) * s[:, g] + rest[:, g]
+    return torch.from_numpy(w.numpy().astype(np.float16)).double()  # (numpy rounds once; torch goes through fp32, which loses a small addend of a tie)
 
 
 def random_w4(N, K, group, symmetric, gen, device="cuda"):

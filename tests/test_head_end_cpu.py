@@ -106,3 +106,16 @@ def test_references_agree_with_torch():
     up[:, 11] += h
     down[:, 11] -= h
     assert torch.allclose((ref_logprobs(up)[2] - ref_logprobs(down)[2]) / (2 * h), want[:, 11].exp(), atol=1e-8)
+
+
+def test_rounded_weights_of_any_zero():
+    """The halves that weights with any zero count as: half((q - zero) * scale) for whole zeros, and otherwise off that product by half a step and
+    2^-17 of the scale (a 32nd of the scale, rounded to half)."""
+    from tests.head_end import random_w4, w4_rounded_any_zero, w4_weights
+    gen = torch.Generator().manual_seed(5)
+    q, s, z = random_w4(40, 256, 32, False, gen, device="cpu")
+    assert torch.equal(w4_rounded_any_zero(q, s, z, 32), w4_weights(q, s, z, 32, rounded=True))
+    z = (torch.rand(z.shape, generator=gen) * 16).half()
+    off = (w4_rounded_any_zero(q, s, z, 32) - w4_weights(q, s, z, 32)).abs()
+    allowed = w4_weights(q, s, z, 32).abs() * 2.0 ** -11 * (1 + 1e-3) + s.double()[:, torch.arange(256) // 32] * 2.0 ** -17 + 2.0 ** -25
+    assert bool((off <= allowed).all()) and float(off.max()) > 0

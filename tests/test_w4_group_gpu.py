@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from tests.head_end import U16, U32, check_logprobs, random_w4, ref_logprobs, softmax_tolerance, w4_weights
+from tests.head_end import U16, U32, check_logprobs, random_w4, ref_logprobs, softmax_tolerance, w4_rounded_any_zero, w4_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -210,6 +210,71 @@ def test_long_products_again_and_again(ops, M, N, K):
     check_product(first, x, (q, s, z), 32, "first")
     for _ in range(30):
         assert torch.equal(ops.linear_w4a16_group(x, q, s, z, 32), first)
+
+
+def fractional_w4(N, K, group, gen, which):
+    """Zeros between whole numbers: everywhere, in one channel of forty, or in one group.  (For up to eight rows of the head from 2 on, so that
+    (q - zero) * scale has 24 bits at most and the 64-bit reference's single rounding to half is that of a product in fp32.)"""
+    q, s, z = random_w4(N, K, group, False, gen)
+    f = (2 + 13.99 * torch.rand(z.shape, generator=gen)).half().cuda()
+    if which == "channels":
+        z[::40] = f[::40]
+    elif which == "group":
+        z[:, z.shape[1] // 2] = f[:, z.shape[1] // 2]
+    else:
+        z = f
+    return q, s, z
+
+
+@pytest.mark.parametrize("which", ["all", "channels", "group"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 70, 288), (5, 33, 2080), (8, 200, 1024), (9, 33, 288), (17, 300, 1024), (33, 130, 416), (100, 516, 2048), (200, 200, 1056), (300, 130, 512)])
+def test_zeros_that_are_not_whole(ops, M, N, K, group, which):
+    """fp16 zeros as common formats have them: in products at any number of rows, and in the head, whose weights are halves."""
+    gen = torch.Generator().manual_seed(M + N + K + group)
+    q, s, z = fractional_w4(N, K, group, gen, which)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    x64, size = x.cpu().double(), x.cpu().double().abs() @ w4_weights(q, s, z, group, parts=True).T
+    halves = w4_weights(q, s, z, group, rounded=True) if M <= 8 else w4_rounded_any_zero(q, s, z, group)
+    # products: the bound of check_product; exact with nine rows and more: check_exact's, and 1.5 * 2^-16 of the scale (the rounding of what the zero
+    # leaves over, times the scale, a 32nd of it: 2^-17; and of the low half that it is added to, below a 16th: 2^-16) and the smallest half's per weight
+    y = ops.linear_w4a16_group(x, q, s, z, group).cpu().double()
+    want = x64 @ (w4_weights(q, s, z, group) if M <= 8 else halves).T
+    assert float(((y - want).abs() - size * (K / 16 + 64) * 2 * U32 - want.abs() * U16 * (1 + 1e-3) - 2.0 ** -25).max()) <= 0
+    y = ops.linear_w4a16_group(x, q, s, z, group, exact=True).cpu().double()
+    want = x64 @ w4_weights(q, s, z, group).T
+    slack = x64.abs() @ (1.5 * 2.0 ** -16 * s.cpu().double()[:, torch.arange(K) // group] + 2.0 ** -25).T
+    assert float(((y - want).abs() - size * (K / 8 + 64) * 2 * U32 - slack - want.abs() * U16 * (1 + 1e-3) - 2.0 ** -25).max()) <= 0
+    tok = torch.randint(0, N, (M,), generator=gen).cuda()
+    z64 = x64 @ halves.T
+    error = float((x64.abs() @ halves.abs().T).max()) * (K / 16 + 2) * 2 * U32  # as for every head: K / 16 additions to one running sum
+    got = ops.head_logprobs(x, q, tok, scale=s, zero=z, group_size=group)
+    check_logprobs(got, ref_logprobs(z64, tok), softmax_tolerance(N, float(z64.abs().max()), error), f"head {M}x{N}x{K} g{group}")
+
+
+def test_small_and_odd_zeros_one_weight_at_a_time(ops):
+    """Every code against zeros below 2, below 0 and far from the codes, weight by weight.  What 64 + zero leaves over is at most half a step of it,
+    2^-12 (64 + |zero|), times the scale: rounded once in a weight that is a half, and with the low half once more in one that is two."""
+    K, N, group = 128, 128, 32
+    zeros = torch.tensor([0.0, 0.1, 0.3337, 1.7, 1.999, -0.25, -3.3, 15.99, 16.5, 100.0, 100.3, 1023.0, 6e-8, -100.0, 7.5, 8.0]).half()
+    w = torch.arange(K)[None].add(torch.arange(N)[:, None]).remainder(16).to(torch.uint8)
+    q = (w[:, 0::2] | (w[:, 1::2] << 4)).cuda()
+    s = (1 + torch.arange(N * 4).reshape(N, 4) / 1024).half().cuda()
+    z = zeros[torch.arange(N * 4).reshape(N, 4).remainder(16)].cuda()
+    x = torch.eye(K).half().cuda()
+    want = w4_weights(q, s, z, group).T
+    g = torch.arange(K) // group
+    s64, z64 = s.cpu().double()[:, g].T, z.cpu().double()[:, g].T
+    left = 2.0 ** -12 * (64 + z64.abs()) * s64
+    for M in (8, 40, 128):
+        y = ops.linear_w4a16_group(x[:M], q, s, z, group, exact=True).cpu().double()
+        # (up to eight rows codes and zeros are summed apart in fp32: a few half steps of the larger one)
+        slack = 4 * U32 * ((15 + z64.abs()) * s64)[:M] if M <= 8 else 3 * U16 * left[:M] + 2.0 ** -25
+        assert float(((y - want[:M]).abs() - want[:M].abs() * U16 * (1 + 1e-3) - slack - 2.0 ** -25).max()) <= 0
+    halves = w4_rounded_any_zero(q, s, z, group).T
+    assert float(((halves - want).abs() - want.abs() * U16 * (1 + 1e-3) - U16 * left - 2.0 ** -25).max()) <= 0
+    for M in (40, 128):
+        assert torch.equal(ops.linear_w4a16_group(x[:M], q, s, z, group).cpu().double(), halves[:M])
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
