@@ -388,7 +388,7 @@ int rwkv7_b200_linear_w4a16(void* stream, int M, int K, int N, const uint16_t* x
 /* 4-bit weights with group scales (no counterpart in the reference): W[n,k] = (q[n,k] - zero[n,g]) * scale[n,g] with
  * g = k / group, group 32, 64 or 128, a short last group allowed (scale and zero are [N][ceil(K / group)]), zero NULL: 8
  * everywhere.  Nibbles as in W4A16.  Any M, N >= 1; K % 32 == 0; x, q, y and workspace 16-byte aligned.  Up to 8 rows
- * the scale multiplies the group's fp32 sum, so no weight is rounded.  With more rows weights count as
+ * the scale multiplies the group's fp32 sum, so no weight is rounded (a K of more than some 58,000: as EXACT).  With more rows weights count as
  * half((q - zero) * scale); with RWKV7_B200_EPI_EXACT or-ed to the epilogue none is rounded there either, at twice the
  * products (a weight is the sum of two halves then, so it has to be below 65504).  Zeros need not be whole numbers; with
  * more than 8 rows other ones (from -32 on) put a weight off by 2^-17 of its scale (EXACT: 2^-15) at most.  workspace is

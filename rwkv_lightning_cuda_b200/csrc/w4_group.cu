@@ -794,15 +794,19 @@ int w4_group_linear(cudaStream_t stream, const W4GroupArgs& a, void* workspace, 
   RK_REQUIRE(static_cast<long long>(a.N) * ((a.K + a.group - 1) / a.group) < (1ll << 31), kShape, "linear_w4a16_group: too many groups");
   int sms = 0, status = device_sms(&sms);
   if (status != kOk) return status;
-  if (a.M > kMaxRows) return many_rows(stream, a, static_cast<float*>(workspace), workspace_bytes, sms);
+  W4GroupArgs one = a;
+  MatvecPlan p;
+  one.M = 1;
+  const bool streamed = a.M <= kMaxRows && plan_matvec(one, sms, &p);
+  if (!streamed) {
+    W4GroupArgs b = a;
+    b.exact = a.exact || a.M <= kMaxRows;  // (a K of which not one row fits into shared memory, some 58,000: no weight is rounded either)
+    return many_rows(stream, b, static_cast<float*>(workspace), workspace_bytes, sms);
+  }
   for (int m0 = 0; m0 < a.M;) {
     W4GroupArgs b = a;
-    MatvecPlan p;
     b.M = std::min(a.M - m0, kMaxRows);
-    while (!plan_matvec(b, sms, &p)) {
-      RK_REQUIRE(b.M > 1, kShape, "linear_w4a16_group: K = %d is too long", a.K);
-      b.M = (b.M + 1) / 2;
-    }
+    while (!plan_matvec(b, sms, &p)) b.M = (b.M + 1) / 2;  // (one row fits)
     b.x = a.x + static_cast<size_t>(m0) * a.K;
     b.y = static_cast<char*>(a.y) + static_cast<size_t>(m0) * a.N * (a.epi == kEpiF32 ? 4 : 2);
     if ((status = matvec(stream, b, p)) != kOk) return status;

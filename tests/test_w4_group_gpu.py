@@ -212,6 +212,16 @@ def test_long_products_again_and_again(ops, M, N, K):
         assert torch.equal(ops.linear_w4a16_group(x, q, s, z, 32), first)
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 24, 57344), (1, 24, 65536), (3, 130, 70016), (8, 7, 98304), (9, 7, 98304)])
+def test_few_rows_of_a_long_k(ops, M, N, K, group):
+    """Rows that do not fit into shared memory go another way, with weights that are not rounded either."""
+    gen = torch.Generator().manual_seed(M + K)
+    q, s, z = random_w4(N, K, group, False, gen)
+    x = torch.randn(M, K, generator=gen).half().cuda()
+    check_exact(ops.linear_w4a16_group(x, q, s, z, group, exact=M > 8), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
+
+
 def fractional_w4(N, K, group, gen, which):
     """Zeros between whole numbers: everywhere, in one channel of forty, or in one group.  (For up to eight rows of the head from 2 on, so that
     (q - zero) * scale has 24 bits at most and the 64-bit reference's single rounding to half is that of a product in fp32.)"""
