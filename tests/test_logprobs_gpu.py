@@ -285,6 +285,32 @@ def test_head_equals_product_then_logprobs(ops):
     assert float((one[2] - two[2]).abs().max()) <= biggest * 2 ** -11 + 1e-4
 
 
+@pytest.mark.parametrize("V,K", [(65536, 1024), (70001, 1024), (65536, 1056), (33000, 2080), (16411, 4096), (4099, 16384), (8200, 16416)])
+def test_head_one_row_of_a_large_matrix(ops, V, K):
+    """The form of a scored decode step: one row on an fp16 head of 128 MB and more, which streams the weights (up to K = 16384) and keeps its
+    logits for a second pass; the given token, none given, ids outside, and the same call again."""
+    gen = torch.Generator(device="cuda").manual_seed(V + K)
+    w = torch.empty(V, K, dtype=torch.float16, device="cuda").normal_(0, 1.3 / K ** 0.5, generator=gen)
+    x = torch.randn(1, K, device="cuda", generator=gen).half()
+    z64, size = torch.empty(1, V, dtype=torch.float64), 0.0
+    for c in range(0, V, 8192):
+        part = w[c:c + 8192].double()
+        z64[:, c:c + 8192] = (x.double() @ part.T).cpu()
+        size = max(size, float((x.double().abs() @ part.abs().T).max()))
+        del part
+    tol = softmax_tolerance(V, float(z64.abs().max()), size * (K / 16 + 2) * 2 * U32)  # as check_head
+    for token in (0, V - 1, V // 3, -1, V):
+        tok = torch.tensor([token]).cuda()
+        got = ops.head_logprobs(x, w, tok)
+        check_logprobs(got, ref_logprobs(z64, tok), tol, f"{V}x{K} token {token}")
+        for a, b in zip(got, ops.head_logprobs(x, w, tok)):
+            assert torch.equal(a, b) or bool(torch.isnan(a).all() and torch.isnan(b).all())
+    none = ops.head_logprobs(x, w)
+    assert none[0] is None and torch.equal(none[1], got[1]) and torch.equal(none[2], got[2])
+    two = ops.head_logprobs(x.expand(2, K).contiguous(), w)  # (the other route)
+    assert float((two[2] - none[2]).abs().max()) <= 2 * tol
+
+
 def test_head_weights_made_just_before(ops):
     """One row on a large fp16 matrix that the kernel before it on the stream writes, itself one that lets its successor begin early: the answer is that
     of the finished weights, every time."""

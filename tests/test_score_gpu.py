@@ -110,3 +110,26 @@ def test_wide_vocabulary_model():
         assert float((lp[:, -1].cpu().double() - ref[0]).abs().max()) <= softmax_tolerance(d.vocab, biggest, biggest * U16)
         assert bool(torch.isfinite(lp).all()) and bool((H > 0).all())
     gm.close()
+
+
+def test_decode_step_on_a_large_fp16_head():
+    """One token on an fp16 head of 134 MB, whose logits are streamed into scratch: the answers follow from the logits of the same call, and a
+    prompt scored one token a call agrees with the prompt scored at once."""
+    from rwkv_lightning_cuda_b200 import backend as bk
+    d, _, gm = build_pair(orc.FMT_F16, False, oracle_model=False, dims=dict(TINY, layers=1, channels=1024, ffn=1024, vocab=65536))
+    T = 5
+    tok = prompt(1, T, d.vocab, 2)
+    want = torch.roll(tok, -1, 1)
+    whole, H = gm.forward_score(tok, gm.create_state(1), want)
+    st, lg = gm.create_state(1), bk.DeviceLogits()
+    for t in range(T):
+        lp, h = gm.forward_score(tok[:, t:t + 1], st, want[:, t:t + 1], lg)
+        ref = ref_logprobs(lg.values, want[:, t])
+        biggest = float(lg.values.abs().max())
+        tol = softmax_tolerance(d.vocab, biggest, biggest * U16)
+        assert float((lp[:, 0].cpu().double() - ref[0]).abs().max()) <= tol
+        assert float((h[:, 0].cpu().double() - ref[1]).abs().max()) <= (2 * float(ref[1].max()) + 1) * tol
+        assert float((lp[:, 0] - whole[:, t]).abs().max()) <= 2 * LOGITS
+        assert float((h[:, 0] - H[:, t]).abs().max()) <= (2 * float(ref[1].max()) + 1) * LOGITS
+    assert st.elapsed.tolist() == [T]
+    gm.close()
