@@ -27,7 +27,6 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "tc_packed.cuh"
-#include "tensormap.h"
 
 namespace rk {
 namespace {
@@ -70,12 +69,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&w)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-      : "memory");
 }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -174,11 +167,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
       const uint32_t dst = ring + q_slot * p.slot_bytes + used;
       const int n = row0 + q_tile * row_step;
       mbar_expect_tx(bar, p.h * (128 + (kCopied ? (a.zero ? 32 : 16) : 0)));
-      tma_2d(dst, &maps.q, bar, q_kb << 7, n);
+      tc::tma_2d(dst, &maps.q, bar, q_kb << 7, n);
       if (kCopied) {
         const int first = (q_kb << (8 - kShift)) & ~7;
-        tma_2d(dst + p.slot_bytes - 1024, &maps.scale, bar, first, n);
-        if (a.zero) tma_2d(dst + p.slot_bytes - 512, &maps.zero, bar, first, n);
+        tc::tma_2d(dst + p.slot_bytes - 1024, &maps.scale, bar, first, n);
+        if (a.zero) tc::tma_2d(dst + p.slot_bytes - 512, &maps.zero, bar, first, n);
       }
     }
     if (++q_slot == p.slots) q_slot = 0;
@@ -585,27 +578,17 @@ int launch_matvec(cudaStream_t stream, const MatvecMaps& maps, const W4GroupArgs
   return launch_matvec<kM, 7, kRounded>(stream, maps, a, p);
 }
 
-int encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, size_t row_bytes, int elem_bytes, int rows, int box_cols, int box_rows,
-           CUtensorMapSwizzle swizzle) {
-  const TensorMapEncodeFn fn = tensor_map_encode_fn();
-  RK_REQUIRE(fn, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled is not available from this driver");
-  const cuuint64_t dims[2] = {row_bytes / elem_bytes, static_cast<cuuint64_t>(rows)}, strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)}, elem[2] = {1, 1};
-  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  RK_REQUIRE(r == CUDA_SUCCESS, kCuda, "linear_w4a16_group: cuTensorMapEncodeTiled failed with %d (rows=%d, %zu bytes each)", static_cast<int>(r), rows, row_bytes);
-  return kOk;
-}
-
 int matvec(cudaStream_t stream, const W4GroupArgs& a, const MatvecPlan& p, bool rounded = false) {
   MatvecMaps maps;
-  int s = encode(&maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, a.K / 2, 1, a.N, 128, p.h, CU_TENSOR_MAP_SWIZZLE_128B);
+  const char* const what = "linear_w4a16_group";
+  int s = tc::encode_map(what, &maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.q, a.N, a.K / 2, 128, p.h, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s != kOk) return s;
   maps.scale = maps.zero = maps.q;
   if (p.copied) {
-    const size_t row_bytes = (a.K + a.group - 1) / a.group * sizeof(half);
-    if ((s = encode(&maps.scale, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.scale, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
-    if (a.zero && (s = encode(&maps.zero, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.zero, row_bytes, 2, a.N, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE)) != kOk) return s;
+    const size_t groups = (a.K + a.group - 1) / a.group;
+    s = tc::encode_map(what, &maps.scale, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.scale, a.N, groups, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (s == kOk && a.zero) s = tc::encode_map(what, &maps.zero, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, a.zero, a.N, groups, 8, p.h, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (s != kOk) return s;
   }
   if (rounded) return launch_matvec<8, true>(stream, maps, a, p);
   switch (columns(a.M)) {
