@@ -732,7 +732,7 @@ tc::PackedShape many_rows_shape(int M, int K, int N, bool exact, size_t scratch_
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
     const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;
-    double cost = waves * (h.kb_per_split * std::max(stage * (exact ? 10.0 : 6.0), stage * h.block_rows / (exact ? 13.5 : 27.0))) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
+    double cost = waves * (h.kb_per_split * std::max(stage * (exact ? 8.0 : 6.0), stage * h.block_rows / (exact ? 13.5 : 27.0))) + (h.block_rows <= 128 ? 500 * waves + results : results * waves);
     if (h.splits > 1) cost += 3000 + 200 * h.splits + 4.0 * (h.splits + 1) * plane / (48.0 * sms);
     h.units = static_cast<int>(std::min<long long>(units, 0x7fffffff));
     if (best.units == 0 || cost < least) { least = cost; best = h; }
