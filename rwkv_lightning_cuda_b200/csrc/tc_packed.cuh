@@ -501,7 +501,7 @@ int launch_stages(cudaStream_t stream, const char* what, const half* x, const vo
 template <int kFmt, class Epi>
 int launch_packed(cudaStream_t stream, const char* what, const half* x, const void* w, const Packed& a, const PackedShape& h, const Epi& epi, int sms) {
   if constexpr (Epi::kExact)
-    if (h.seg < h.kb_per_split) return launch_stages<kFmt, 2, true>(stream, what, x, w, a, h, epi, sms);
+    if (h.seg < h.kb_per_split) return launch_stages<kFmt, kFmt == 3 ? 1 : 2, true>(stream, what, x, w, a, h, epi, sms);
   if constexpr (kFmt == 3) return launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
   else return subs(h.block_rows) == 2 ? launch_stages<kFmt, 2, false>(stream, what, x, w, a, h, epi, sms) : launch_stages<kFmt, 1, false>(stream, what, x, w, a, h, epi, sms);
 }

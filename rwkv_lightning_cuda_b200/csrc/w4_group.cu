@@ -692,6 +692,11 @@ struct ProductEpilogue {
   __device__ __forceinline__ void end() {}
 };
 
+// The same where a long K may be added up in ranges.
+struct RangedEpilogue : ProductEpilogue {
+  static constexpr bool kExact = true;
+};
+
 // Adds the planes in order (the result does not depend on timing) and applies the epilogue: four channels per thread.
 __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p, int splits) {
   pdl_wait();
@@ -715,12 +720,16 @@ __global__ void __launch_bounds__(256) w4_reduce_kernel(const ProductEpilogue p,
 // second kernel 3000, 200 a range and its traffic.  (64 rows of 1024 x 1024: 7.5 us whole, 6.5 in eight ranges, 7.9 in sixteen; 96
 // rows of 10240 x 2560: 15.7 whole, 19.0 in two, 16.2 in three; 96 rows of 2560 x 10240: 43.7 whole, 15.7 in seven, 19.6 in nine,
 // which is a second wave: with stages of 64, those of 128 take a tenth less of all of them.)  Exact weights, two halves each, have
-// stages of 64, which take 600 to 760 clocks, and twice the products.
+// stages of 64, which take 600 to 760 clocks, and twice the products.  Their long sums go in ranges, because the tensor cores cut off of
+// what they add: 4.8e-6 of a result's size for 256 additions, which the result's rounding to half covers up to kLongExact, but not
+// in a K of any length.
+constexpr int kLongExact = 16384, kExactRange = 8192;
 tc::PackedShape many_rows_shape(int M, int K, int N, bool exact, size_t scratch_floats, int sms) {
   tc::PackedShape best = {};
   double least = 0;
   tc::PackedShape rows = {};
-  tc::set_row_blocks(&rows, M);
+  const bool ranges = exact && K > kLongExact;
+  tc::set_row_blocks(&rows, M, ranges ? 128 : tc::kMaxBlockRows);
   const int stage = tc::kBK * (exact ? 1 : tc::subs(rows.block_rows)), kblocks = (K + stage - 1) / stage;
   const size_t plane = static_cast<size_t>(M) * N;
   for (int want = 1; want <= 16 && want <= kblocks; ++want) {
@@ -728,7 +737,7 @@ tc::PackedShape many_rows_shape(int M, int K, int N, bool exact, size_t scratch_
     h.tiles = (N + tc::kTileToks - 1) / tc::kTileToks;
     h.kb_per_split = (kblocks + want - 1) / want;
     h.splits = (kblocks + h.kb_per_split - 1) / h.kb_per_split;
-    h.seg = h.kb_per_split;
+    h.seg = ranges ? std::min(h.kb_per_split, kExactRange / stage) : h.kb_per_split;
     if (h.splits > 1 && (N % 4 != 0 || h.splits * plane > scratch_floats)) continue;
     const long long units = static_cast<long long>(h.tiles) * h.row_blocks * h.splits;
     const double waves = static_cast<double>((units + sms - 1) / sms), results = 25.0 * h.block_rows;
@@ -745,13 +754,14 @@ int many_rows(cudaStream_t stream, const W4GroupArgs& a, float* scratch, size_t 
   RK_REQUIRE(h.units < 0x7fffffff, kShape, "linear_w4a16_group: too many rows");
   tc::Packed w;
   w.V = a.N; w.K = a.K; w.group = a.group; w.scale = a.scale; w.zero = a.zero;
-  ProductEpilogue epi;
+  RangedEpilogue epi;
   epi.y = a.y; epi.partial = h.splits > 1 ? scratch : nullptr; epi.n_rows = a.M; epi.N = a.N; epi.epi = a.epi;
+  const ProductEpilogue& plain = epi;
   const int s = a.exact ? tc::launch_packed<3>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms)
-                        : tc::launch_packed<2>(stream, "linear_w4a16_group", a.x, a.q, w, h, epi, sms);
+                        : tc::launch_packed<2>(stream, "linear_w4a16_group", a.x, a.q, w, h, plain, sms);
   if (s != kOk || h.splits == 1) return s;
   const size_t quads = static_cast<size_t>(a.M) * a.N / 4;
-  RK_CUDA(launch_pdl(w4_reduce_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, epi, h.splits));
+  RK_CUDA(launch_pdl(w4_reduce_kernel, dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(256), 0, stream, plain, h.splits));
   RK_LAUNCH_CHECK("linear_w4a16_group reduction launch");
   return kOk;
 }

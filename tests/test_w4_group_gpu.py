@@ -222,6 +222,22 @@ def test_few_rows_of_a_long_k(ops, M, N, K, group):
     check_exact(ops.linear_w4a16_group(x, q, s, z, group, exact=M > 8), x, (q, s, z), group, f"{M}x{N}x{K} g{group}")
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 8192, 65536), (9, 1024, 32768), (100, 512, 65536), (300, 256, 24576)])
+def test_exact_products_of_a_long_k_lose_no_more_than_a_range(ops, M, N, K):
+    """What the tensor cores cut off is a bias towards zero, which the mean over many results shows below their rounding to half: at most that of
+    8192 products, twice 512 additions, each off by half a step (2^-23) on average of a sum that averages half of the whole, 1024 / 4 * 2^-23."""
+    gen = torch.Generator(device="cuda").manual_seed(K + M)
+    q = torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device="cuda", generator=gen)
+    s = ((0.5 + torch.rand(N, K // 64, device="cuda", generator=gen)) * 0.02).half()
+    z = torch.randint(4, 12, (N, K // 64), device="cuda", generator=gen).half()
+    x = torch.randn(M, K, device="cuda", generator=gen).half()
+    y = ops.linear_w4a16_group(x, q, s, z, 64, exact=True).double()
+    want = x.double() @ w4_weights(q, s, z, 64).cuda().T
+    bias = float(((y - want) * want.sign()).sum() / want.abs().sum())
+    noise = 5 * float((want.abs() * U16).norm() / want.abs().sum())  # of the results' own rounding
+    assert abs(bias) <= 1024 / 4 * 2.0 ** -23 + noise, bias
+
+
 def fractional_w4(N, K, group, gen, which):
     """Zeros between whole numbers: everywhere, in one channel of forty, or in one group.  (For up to eight rows of the head from 2 on, so that
     (q - zero) * scale has 24 bits at most and the 64-bit reference's single rounding to half is that of a product in fp32.)"""
