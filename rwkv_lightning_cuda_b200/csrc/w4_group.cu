@@ -149,6 +149,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
     if (warp == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.q) : "memory");
   }
   if (threadIdx.x < 32) *reinterpret_cast<uint4*>(mem + p.zero_off + threadIdx.x * 16) = make_uint4(0u, 0u, 0u, 0u);  // what idle columns read, at the offsets of eight chunks
+  if (kRounded && kCopied && lane >= p.h) {  // what is read as the zeros of rows that the copies do not bring: 0, a whole number
+    for (int i = 0; i < p.slots; ++i) *reinterpret_cast<uint4*>(mem + (ring - base) + (i + 1) * p.slot_bytes - 512 + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
   __syncwarp();
   pdl_wait();
   pdl_trigger();
@@ -431,11 +434,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4_matvec_kernel(const __grid_con
           }
         }
       };
-      bool whole = true;  // the zeros of the box's groups are whole numbers (those of the tile's rows, behind which none have come)
+      bool whole = true;  // the zeros of the box's groups are whole numbers
       if (kRounded && a.zero) {
         uint32_t odd = 0;
 #pragma unroll
-        for (int i = 0; i < 2 * kBlk; ++i) odd |= g + 8 * i < p.h ? not_whole(z_now[i]) : 0u;
+        for (int i = 0; i < 2 * kBlk; i += 2) {
+          if (kShift == 5) odd |= not_whole(z_now[i]) | not_whole(z_now[i + 1]);
+          else odd |= not_whole(__byte_perm(z_now[i], z_now[i + 1], 0x5410));
+        }
         whole = __all_sync(0xffffffffu, odd == 0);
       }
       if (!kRounded || whole) work(std::false_type());
