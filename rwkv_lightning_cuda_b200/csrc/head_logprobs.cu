@@ -5,7 +5,7 @@
 // are exact integers with the channel's scale on the sum, 4-bit weights half((q - zero) * scale).
 //
 // Bound by the weights' bytes up to some 256 rows of fp16 weights, by the tensor cores above, and by the expansion of quantised ones in
-// between (128 x 65536 x 4096 fp16: 94 us, 5.7 TB/s; 2048 rows: 780 to 880 us as the power cap lets it).  The products are tc_rows.cuh's (fp16 weights) and
+// between (128 x 65536 x 4096 fp16: 94 us, 5.7 TB/s; 2048 rows: 800 to 940 us as the power cap lets it).  The products are tc_rows.cuh's (fp16 weights) and
 // tc_packed.cuh's (quantised ones); here are their epilogues, which reduce a tile of logits to (m, s, t) per row, the merging of the
 // tiles, and the route for a few rows.
 #include <algorithm>
@@ -221,9 +221,10 @@ int head_packed(cudaStream_t stream, HeadLogprobsArgs a, int sms) {
 
 // Few rows: where the weight-streaming kernels read the weights at a better rate than the kernels above with their 128-row or
 // 128-token tiles, the logits of so few rows are small.  Measured at 65536 tokens (K = 4096 unless said otherwise), this route
-// against the other: 4-bit 51 us against 56 at eight rows (30 against 35 at two and K = 2048, 24 against 23 at eight and K = 1024);
-// fp16 83 against 91 at one row, but 111 against 94 at four, and below 128 MB of weights the second pass takes what is saved.  int8
-// has no such route: 58 against 51 at four rows, 42 against 35 at two and K = 2560.
+// against the other: 4-bit 55 us against 64 at eight rows (31 against 35 at two and K = 2048, 24 against 25 at eight and K = 1024, but
+// 17 against 13 at eight rows of 32003 x 768); fp16 84 to 86 against 90 at one row, but 111 against 94 at four, and below 128 MB of
+// weights the second pass takes what is saved.   int8 has no such route: 58 against 51 at four rows, 42 against 35 at two and
+// K = 2560.
 constexpr int kFewRowsF16 = 1, kFewRowsW4 = 8;
 constexpr double kFewRowsBytes = 128e6;
 

@@ -11,7 +11,8 @@
 //
 // Bound up to 128 rows by what the roles do per stage and weight: of 128 of K, some 800 clocks, in which the expansion of 4-bit weights
 // has 300 to 350 issue slots of each scheduler; above by the tensor cores.  (24 rows of 65536 x 4096 in 59 us, with stages of 64
-// in 65; 128 rows of 16384 x 4096 in 22; 256 in 32 us, 1.09 PFLOP/s.)
+// in 65; 128 rows of 16384 x 4096 in 22; 256 in 30 us, 1.15 PFLOP/s.  Where a weight is
+// two halves: 88, 32 and 49.)
 //
 // Warp roles: 0 loads packed tiles, 1 issues tcgen05.mma, 2..5 run the epilogue, 6 loads rows of x, 8..23 expand, four warps to a
 // stage in turn.  Every wait is bounded: one that runs out sets the device's failure word, every role leaves its loop, and the

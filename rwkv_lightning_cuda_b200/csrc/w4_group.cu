@@ -35,7 +35,8 @@ constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
 constexpr int kBoxWeights = 256;  // 128 bytes along a row: eight chunks of 32 weights
 // Rows up to which the weights are streamed and never rounded.  Nine to sixteen rows in two such launches took 70 to 82 us at
-// 65536 x 4096, 24 at 16384 x 4096, 18 to 20 at 10240 x 2560 and 30 at 2560 x 10240; the kernel for many rows takes 69, 21, 15 and 13.
+// 65536 x 4096, 24 at 16384 x 4096, 18 to 20 at 10240 x 2560 and 30 at 2560 x 10240; the kernel for many rows takes 58, 18, 14 and 12,
+// and 85, 27, 17 and 15 with exact weights.
 constexpr int kMaxRows = 8;
 constexpr size_t kSmemLimit = 226 * 1024;
 
@@ -620,8 +621,8 @@ int w4_rounded_linear(cudaStream_t stream, const W4GroupArgs& a, int sms) {
 }
 
 // ---- more rows: the tensor-core skeleton of tc_packed.cuh, weights rounded to half, or as two halves each where the caller wants none
-// rounded: two instructions more per two weights, twice the stores and products, and stages of 64 (96 rows of 10240 x 2560 20.2 us, 14.0 rounded;
-// 24 of 65536 x 4096 87 and 59; 256 of 16384 x 4096 49 and 30; nine of 10240 x 2560 16.5 and 13.8).
+// rounded: two instructions more per two weights, twice the stores and products, and stages of 64 (96 rows of 10240 x 2560 20.1 us, 14.0 rounded;
+// 24 of 65536 x 4096 88 and 59; 256 of 16384 x 4096 49 and 30; nine of 10240 x 2560 17.0 and 13.8).
 namespace {
 
 __device__ __forceinline__ void sts4(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
