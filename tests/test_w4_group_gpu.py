@@ -238,6 +238,30 @@ def test_exact_products_of_a_long_k_lose_no_more_than_a_range(ops, M, N, K):
     assert abs(bias) <= 1024 / 4 * 2.0 ** -23 + noise, bias
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("off", [1, 2, 5])
+def test_scales_and_zeros_that_start_anywhere(ops, off, group):
+    """Parameters that begin off a 16-byte or 4-byte boundary, as slices of a file's buffer do: the answers of aligned ones."""
+    gen = torch.Generator().manual_seed(off + group)
+    N, K = 300, 2048
+    q, s, z = random_w4(N, K, group, False, gen)
+    z = (z + 0.25 * torch.randint(0, 2, z.shape, generator=gen).cuda()).half()
+
+    def moved(t):
+        store = torch.full((t.numel() + off,), float("nan"), dtype=torch.float16, device="cuda")
+        store[off:] = t.flatten()
+        return store[off:].view(t.shape)
+    for M in (1, 3, 8, 9, 70, 200):
+        x, tok = torch.randn(M, K, generator=gen).half().cuda(), torch.randint(0, N, (M,), generator=gen).cuda()
+        for zero in (z, None):
+            there = None if zero is None else moved(zero)
+            for exact in (False, True):
+                y = ops.linear_w4a16_group(x, q, moved(s), there, group, exact=exact)
+                assert torch.equal(y, ops.linear_w4a16_group(x, q, s, zero, group, exact=exact)), f"{M} rows, exact={exact}"
+            got, want = ops.head_logprobs(x, q, tok, scale=moved(s), zero=there, group_size=group), ops.head_logprobs(x, q, tok, scale=s, zero=zero, group_size=group)
+            assert all(torch.equal(u, v) for u, v in zip(got, want)), f"head, {M} rows"
+
+
 def fractional_w4(N, K, group, gen, which):
     """Zeros between whole numbers: everywhere, in one channel of forty, or in one group.  (For up to eight rows of the head from 2 on, so that
     (q - zero) * scale has 24 bits at most and the 64-bit reference's single rounding to half is that of a product in fp32.)"""
